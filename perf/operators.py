@@ -193,16 +193,16 @@ def run(s):
         if s["op"] == "quant":
             return _dequantize(*_quantize(s["x"]), s["x"].dtype)
         return {"matmul": _plain_matmul, "moe": _plain_moe, "norm": _plain_norm}[s["op"]](s)
-    from wisp_b200.mx4 import Mx4Tensor, mx4_dequantize, mx4_matmul, mx4_moe, mx4_quantize
-    from wisp_b200.norm import block_norm
+    from wisp_b200 import mx4, norm
     if s["op"] == "quant":
-        return mx4_dequantize(mx4_quantize(s["x"]), s["x"].dtype)
+        return mx4.mx4_dequantize(mx4.mx4_quantize(s["x"]), s["x"].dtype)
     if s["op"] == "matmul":
-        return mx4_matmul(Mx4Tensor(s["a"], s["a_scales"]), Mx4Tensor(s["w"], s["w_scales"]), s["offsets"])
+        return mx4.mx4_matmul(mx4.Mx4Tensor(s["a"], s["a_scales"]), mx4.Mx4Tensor(s["w"], s["w_scales"]), s["offsets"])
     if s["op"] == "moe":
-        return mx4_moe(s["x"], Mx4Tensor(s["w13"], s["s13"]), Mx4Tensor(s["w2"], s["s2"]), s["top_k"], router=s["gate"])
-    return block_norm(s["y"], s["residual"], s["pre"], post_weight=s["post"], gate=s["gate"], scale=s["scale"],
-                      eps=s["eps"])
+        return mx4.mx4_moe(s["x"], mx4.Mx4Tensor(s["w13"], s["s13"]), mx4.Mx4Tensor(s["w2"], s["s2"]), s["top_k"],
+                           router=s["gate"])
+    return norm.block_norm(s["y"], s["residual"], s["pre"], post_weight=s["post"], gate=s["gate"], scale=s["scale"],
+                           eps=s["eps"])
 
 
 # ---- what a pass cannot do without ----------------------------------------------------------------------------------

@@ -113,6 +113,49 @@ WISP_API int wisp_route_topk(const void *logits, int32_t logits_bf16, int32_t nu
                              void *stream);
 
 /*
+ * Stateless operators around a layer of 4-bit experts (no counterparts in the
+ * reference).  They run on the current device, asynchronously on `stream`,
+ * allocate nothing and may be captured into a CUDA graph.
+ *
+ * MXFP4: a matrix [rows][K], K a multiple of 32, is codes [rows][K / 2] (two
+ * E2M1 values a byte, the even column in the low nibble) and scales
+ * [rows][K / 32] (E8M0 bytes: b stands for 2^(b - 127), 255 for NaN), the
+ * layout of MXFP4 checkpoints.
+ */
+enum wisp_dtype { WISP_BF16 = 0, WISP_FP16 = 1, WISP_FP32 = 2 };
+
+/*
+ * x [rows][cols] (rows row_stride values apart, each on a 16-byte boundary)
+ * to MXFP4.  Per block of 32 values: scale 2^(floor(log2 max|x|) - 2), codes
+ * rounded to nearest even and saturating at 6; a block with an infinity or a
+ * NaN becomes NaN, a block of zeros has scale byte 0.
+ */
+WISP_API int wisp_mx4_quantize(const void *x, int32_t dtype, int64_t rows, int64_t cols, int64_t row_stride,
+                               void *codes, void *scales, void *stream);
+/* The values of codes and scales in `dtype` (rounded once where it cannot hold them), out [rows][cols]. */
+WISP_API int wisp_mx4_dequantize(const void *codes, const void *scales, int64_t rows, int64_t cols, void *out,
+                                 int32_t dtype, void *stream);
+
+/*
+ * The step between two blocks of a decoder layer:
+ *   z = y, or y * rsqrt(mean(y^2) + eps) * post_weight when that is not NULL;
+ *   residual_out = residual + scale * gate * z;
+ *   normed = r * rsqrt(mean(r^2) + eps) * pre_weight, r the unrounded residual_out.
+ * y [rows][cols] of `dtype` (also normed's and the gate's); residual and
+ * residual_out of residual_dtype, pre_weight and post_weight [cols] of
+ * weight_dtype, each `dtype` or fp32.  gate: none, one for each channel
+ * [cols], one for each token (gate_stride values apart) or [rows][cols].
+ * Rows are *_stride values apart; normed and residual_out are contiguous and
+ * may be y's and the residual's own memory where those are contiguous too.
+ */
+enum wisp_gate { WISP_GATE_NONE = 0, WISP_GATE_TOKEN = 1, WISP_GATE_CHANNEL = 2, WISP_GATE_FULL = 3 };
+WISP_API int wisp_block_norm(const void *y, int64_t y_stride, const void *residual, int64_t residual_stride,
+                             const void *pre_weight, const void *post_weight, const void *gate, int32_t gate_kind,
+                             int64_t gate_stride, int32_t dtype, int32_t residual_dtype, int32_t weight_dtype,
+                             int64_t rows, int32_t cols, float scale, float eps, void *normed, void *residual_out,
+                             void *stream);
+
+/*
  * One LRU admission step for an arbitrary id list, with page-in, finished
  * before returning.  Replaces WispMoEState.ensure_resident
  * (fused_moe.py:264-358).

@@ -1,0 +1,96 @@
+"""What the 4-bit operators and the block norm refuse (no GPU needed): the C entry points return
+WISP_ERR_INVALID with a message before they touch the device, the Python functions raise."""
+import pytest
+import torch
+
+from oracle import mx4 as ref
+from wisp_b200 import _lib
+from wisp_b200.mx4 import Mx4Tensor, mx4_dequantize, mx4_quantize
+from wisp_b200.norm import block_norm
+
+P = 1 << 20         # an aligned address that no refused call reads
+
+
+def refused(rc, word):
+    assert rc == _lib.WISP_ERR_INVALID and word in _lib.lib().wisp_last_error().decode()
+
+
+def test_quantize_refusals():
+    q = _lib.lib().wisp_mx4_quantize
+    refused(q(P, 3, 1, 32, 32, P, P, None), "dtype")
+    refused(q(P, 0, 1, 33, 33, P, P, None), "multiple of 32")
+    refused(q(P, 0, 1, 0, 0, P, P, None), "multiple of 32")
+    refused(q(P, 0, -1, 32, 32, P, P, None), "rows")
+    refused(q(P, 0, 1 << 40, 32, 32, P, P, None), "2^38")
+    refused(q(None, 0, 1, 32, 32, P, P, None), "NULL")
+    refused(q(P + 2, 0, 1, 32, 32, P, P, None), "16-byte")
+    refused(q(P, 0, 2, 64, 32, P, P, None), "overlap")
+    refused(q(P, 0, 2, 32, 33, P, P, None), "16-byte")
+    assert q(None, 0, 0, 32, 32, None, None, None) == _lib.WISP_OK
+    d = _lib.lib().wisp_mx4_dequantize
+    refused(d(P, P, 1, 32, P, 7, None), "dtype")
+    refused(d(P, P, 1, 16, P, 0, None), "multiple of 32")
+    refused(d(P, None, 1, 32, P, 0, None), "NULL")
+    refused(d(P + 1, P, 1, 32, P, 0, None), "aligned")
+    refused(d(P, P, 1, 32, P + 8, 0, None), "aligned")
+
+
+def test_block_norm_refusals():
+    n = _lib.lib().wisp_block_norm
+
+    def call(dtype=0, rdtype=0, wdtype=0, rows=1, cols=64, gate=None, kind=0, y=P, stride=64):
+        return n(y, stride, P, 64, P, None, gate, kind, 0, dtype, rdtype, wdtype, rows, cols, 1.0, 1e-6, P, P, None)
+    refused(call(dtype=5), "type")
+    refused(call(rdtype=1), "type")
+    refused(call(wdtype=1), "type")
+    refused(call(cols=0), "columns")
+    refused(call(cols=16385), "columns")
+    refused(call(rows=-1), "rows")
+    refused(call(gate=P), "gate_kind")
+    refused(call(kind=2), "gate_kind")
+    refused(call(kind=4, gate=P), "gate_kind")
+    refused(call(y=None), "NULL")
+    refused(call(rows=2, stride=-64), "stride")
+    assert call(rows=0) == _lib.WISP_OK
+
+
+def test_python_refusals():
+    x = torch.zeros(2, 64)
+    with pytest.raises(ValueError, match="CUDA"):
+        mx4_quantize(x)
+    with pytest.raises(TypeError, match="tensor"):
+        mx4_quantize([1.0])
+    codes, scales = ref.quantize(x)
+    with pytest.raises(ValueError, match="CUDA"):
+        mx4_dequantize(Mx4Tensor(codes, scales))
+    with pytest.raises(TypeError, match="uint8"):
+        Mx4Tensor(codes.int(), scales)
+    with pytest.raises(ValueError, match="match"):
+        Mx4Tensor(codes, scales[:, :1])
+    with pytest.raises(ValueError, match="match"):
+        Mx4Tensor(codes[:1], scales)
+    with pytest.raises(ValueError, match="contiguous"):
+        Mx4Tensor(codes.t().contiguous().t(), scales)
+    with pytest.raises(ValueError, match="CUDA"):
+        block_norm(x, x, x[0])
+
+
+def test_mx4_tensor():
+    codes, scales = ref.quantize(torch.randn(3, 4, 64))
+    t = Mx4Tensor(codes, scales.view(torch.float8_e8m0fnu))
+    assert t.shape == (3, 4, 64) and t.scales.dtype == torch.uint8 and t[1].shape == (4, 64)
+    assert torch.equal(t[1].codes, codes[1]) and t[0, 2].shape == (64,)
+    with pytest.raises(IndexError):
+        t[0, 0, 0]
+
+
+def test_oracle_quantizer_is_the_nearest_value():
+    """The oracle against its own definition: no E2M1 value lies nearer than the one it chose."""
+    x = torch.randn(64, 96, dtype=torch.float64, generator=torch.Generator().manual_seed(0)) * 10
+    codes, scales = ref.quantize(x)
+    v = ref.values(codes, scales)
+    s = torch.exp2(scales.double() - 127).repeat_interleave(32, -1)
+    grid = torch.tensor(ref.E2M1 + [-a for a in ref.E2M1], dtype=torch.float64)
+    best = (x.unsqueeze(-1) - s.unsqueeze(-1) * grid).abs().amin(-1)
+    assert torch.equal((x - v).abs(), best)
+    assert torch.equal(ref.values(*ref.quantize(v)), v) or bool((v.abs() / s <= 6).all())

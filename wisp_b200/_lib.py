@@ -50,6 +50,11 @@ SIGNATURES = {
     "wisp_layer_scale_buffers": (ctypes.c_int, [_vp, ctypes.POINTER(_vp), ctypes.POINTER(_vp)]),
     "wisp_moe_forward": (ctypes.c_int, [_vp, _vp, _pf, _vp, _c_int32, _c_int32, _c_int32, _vp, _vp]),
     "wisp_route_topk": (ctypes.c_int, [_vp, _c_int32, _c_int32, _c_int32, _c_int32, _c_int32, _vp, _vp, _vp]),
+    "wisp_mx4_quantize": (ctypes.c_int, [_vp, _c_int32, _c_int64, _c_int64, _c_int64, _vp, _vp, _vp]),
+    "wisp_mx4_dequantize": (ctypes.c_int, [_vp, _vp, _c_int64, _c_int64, _vp, _c_int32, _vp]),
+    "wisp_block_norm": (ctypes.c_int, [_vp, _c_int64, _vp, _c_int64, _vp, _vp, _vp, _c_int32, _c_int64, _c_int32,
+                                       _c_int32, _c_int32, _c_int64, _c_int32, ctypes.c_float, ctypes.c_float,
+                                       _vp, _vp, _vp]),
     "wisp_ensure_resident": (ctypes.c_int, [_vp, _vp, _c_int32, _c_int32, _vp]),
     "wisp_pager_step": (ctypes.c_int, [_vp, _vp, _c_int32, _c_int32, _c_int32, _vp, _vp]),
     "wisp_prefetch_async": (ctypes.c_int, [_vp, _p32, _c_int32, _vp]),

@@ -137,6 +137,34 @@ WISP_API int wisp_mx4_dequantize(const void *codes, const void *scales, int64_t 
                                  int32_t dtype, void *stream);
 
 /*
+ * A whole MoE layer for a few tokens from MXFP4 experts, in one (cooperative)
+ * launch: out[t] = sum over the token's experts e of p_e W2[e] (silu(g) u),
+ * [g; u] = W13[e] x[t].  x [T][hidden] bf16 (rows x_stride values apart).
+ * Routing: `router` [num_experts][hidden] bf16 -- softmax of the products
+ * with x over the top_k largest (over all experts when not renormalize; ties
+ * to the lower id) -- or, router NULL, topk_ids [T][top_k] int32 (int64 when
+ * ids_int64) and topk_weights [T][top_k] fp32.  Experts: w13 [num_slots]
+ * [2 inter][hidden] (gate rows, then up rows) and w2 [num_slots][hidden]
+ * [inter] in MXFP4; expert e lies in slot expert_map[e] (int32 [num_experts];
+ * NULL: slot e).  An id outside [0, num_experts) and an expert whose slot is
+ * outside [0, num_slots) contribute nothing; an expert a token names twice
+ * counts once, with the sum of the weights.  fp32 arithmetic; silu(g) u is
+ * rounded to bf16 and out once.  A token's result does not depend on the
+ * slots.  T <= 64, top_k <= 16, num_experts <= 1024, hidden and inter
+ * multiples of 32 up to 32768 and 65536.  workspace:
+ * wisp_mx4_moe_workspace() bytes, aligned to 16, any contents; calls that may
+ * overlap on the GPU need one each.
+ */
+WISP_API int wisp_mx4_moe_workspace(int32_t num_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,
+                                    int32_t inter, int64_t *bytes);
+WISP_API int wisp_mx4_moe(const void *x, int64_t x_stride, const void *router, const void *topk_ids,
+                          int32_t ids_int64, const float *topk_weights, const int32_t *expert_map,
+                          const void *w13_codes, const void *w13_scales, const void *w2_codes, const void *w2_scales,
+                          int32_t num_slots, int32_t num_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,
+                          int32_t inter, int32_t renormalize, void *workspace, int64_t workspace_bytes, void *out,
+                          void *stream);
+
+/*
  * The step between two blocks of a decoder layer:
  *   z = y, or y * rsqrt(mean(y^2) + eps) * post_weight when that is not NULL;
  *   residual_out = residual + scale * gate * z;

@@ -51,3 +51,33 @@ def block_norm(y, residual, weight, post_weight=None, gate=None, scale=1.0, eps=
         z = z * gate.double()
     r = residual.double() + scale * z
     return r / torch.sqrt(r.pow(2).mean(-1, keepdim=True) + eps) * weight.double(), r
+
+
+def route(x, router, top_k, renormalize=True):
+    """(weights, ids) [T, k]: softmax of x router^T in fp64, ties to the lower id."""
+    logits = x.double() @ router.double().T
+    order = torch.sort(logits, dim=-1, descending=True, stable=True)
+    p = torch.softmax(logits, -1).gather(1, order.indices[:, :top_k])
+    return (p / p.sum(-1, keepdim=True) if renormalize else p), order.indices[:, :top_k]
+
+
+def moe(x, w13, w2, weights, ids, expert_map=None):
+    """(out, size, slack) in fp64 of an MoE layer with dequantised w13 [S, 2I, H] and w2 [S, H, I].  `size`: the sum
+    of the magnitudes that meet in an output, sum p |a| |w2|; `slack`: what an error of one part of the magnitudes
+    that meet in g and u makes of the output."""
+    out, size, slack = (torch.zeros(x.shape, dtype=torch.float64, device=x.device) for _ in range(3))
+    xd = x.double()
+    for t in range(x.shape[0]):
+        for w, e in zip(weights[t].tolist(), ids[t].tolist()):
+            s = e if expert_map is None else (int(expert_map[e]) if 0 <= e < len(expert_map) else -1)
+            if not 0 <= s < w13.shape[0]:
+                continue
+            h, m = w13[s] @ xd[t], w13[s].abs() @ xd[t].abs()
+            n = h.shape[0] // 2
+            g, u = h[:n], h[n:]
+            a = g * torch.sigmoid(g) * u
+            out[t] += w * (w2[s] @ a)
+            size[t] += abs(w) * (w2[s].abs() @ a.abs())
+            slack[t] += abs(w) * (w2[s].abs() @ (1.1 * m[:n] * u.abs() + (g * torch.sigmoid(g)).abs() * m[n:]
+                                                 + 1.1 * m[:n] * m[n:] * 2.0 ** -12))
+    return out, size, slack

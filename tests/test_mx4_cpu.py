@@ -94,3 +94,39 @@ def test_oracle_quantizer_is_the_nearest_value():
     best = (x.unsqueeze(-1) - s.unsqueeze(-1) * grid).abs().amin(-1)
     assert torch.equal((x - v).abs(), best)
     assert torch.equal(ref.values(*ref.quantize(v)), v) or bool((v.abs() / s <= 6).all())
+
+
+def test_moe_refusals():
+    import ctypes
+    f = _lib.lib().wisp_mx4_moe
+
+    def call(T=1, E=4, k=2, H=64, I=32, slots=4, x=P, router=P, ids=None, w=None, emap=None, c13=P, s13=P, ws=P,
+             nbytes=1 << 30, stride=64):
+        return f(x, stride, router, ids, 0, w, emap, c13, s13, P, P, slots, T, E, k, H, I, 1, ws, nbytes, P, None)
+    refused(call(T=65), "64 tokens")
+    refused(call(T=-1), "64 tokens")
+    refused(call(E=1025), "1024 experts")
+    refused(call(k=0), "top_k")
+    refused(call(k=5), "top_k")
+    refused(call(k=17, E=64, slots=64), "top_k")
+    refused(call(slots=0), "top_k")
+    refused(call(H=48), "multiples of 32")
+    refused(call(I=16), "multiples of 32")
+    refused(call(H=65536), "at most")
+    refused(call(x=None), "NULL")
+    refused(call(ws=None), "NULL")
+    refused(call(router=None), "either")
+    refused(call(ids=P, w=P), "either")
+    refused(call(router=None, ids=P), "either")
+    refused(call(slots=3), "slots")
+    refused(call(c13=P + 8), "aligned")
+    refused(call(s13=P + 2), "aligned")
+    refused(call(ws=P + 4), "aligned")
+    refused(call(T=2, stride=32), "overlap")
+    refused(call(T=2, stride=68), "16-byte")
+    refused(call(nbytes=64), "workspace")
+    assert call(T=0) == _lib.WISP_OK
+    n = ctypes.c_int64()
+    refused(_lib.lib().wisp_mx4_moe_workspace(65, 4, 2, 64, 32, ctypes.byref(n)), "64 tokens")
+    refused(_lib.lib().wisp_mx4_moe_workspace(4, 4, 2, 64, 32, None), "NULL")
+    assert _lib.lib().wisp_mx4_moe_workspace(4, 4, 2, 64, 32, ctypes.byref(n)) == 0 and n.value >= 4 * 64 * 2

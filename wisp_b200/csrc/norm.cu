@@ -8,21 +8,20 @@
 // All of it in fp32; r' and n are rounded once each, n from the unrounded r'.
 //
 // Bound by HBM: y and the residual are read once, r' and n written once.  A
-// CTA holds a row in registers, so the two means cost no second read; the CTAs
-// are persistent (as many as fit the device) and load their next row before
-// they reduce the present one, and they keep the weights, which every row
-// shares, in registers.  A thread's pieces of a row are VEC values wide: 8
-// where the width and every address allow 16-byte accesses, else 2, else 1;
-// NV of them, so that a row takes 256 threads or fewer where it can (more
-// rows in flight on an SM, fewer warps in a reduction).
+// CTA holds a row in registers, so the two means cost no second read; several
+// CTAs share an SM, so that one row's loads cover another's reductions (a
+// thread that loads its next row early needs twice the registers, which
+// measured slower), and the weights, which every row shares, stay in L1.  A
+// thread's pieces of a row are VEC values wide: 8 where the width and every
+// address allow 16-byte accesses, else 2, else 1; NV of them, so that a row
+// takes 256 threads or fewer where it can (more rows in flight on an SM,
+// fewer warps in a reduction).
 #include <type_traits>
 
 #include "mx4.cuh"
 
 namespace wisp {
 namespace {
-
-constexpr int kMaxThreads = 1024;
 
 struct NormArgs {
     const void *y, *residual, *pre, *post, *gate;
@@ -85,102 +84,93 @@ __device__ __forceinline__ float block_sum(float v, float *buf) {
     return s;
 }
 
-template <typename T, typename R, typename W, int VEC, int NV>
-__global__ void __launch_bounds__(kMaxThreads) block_norm_kernel(const NormArgs a) {
+template <typename T, typename R, typename W, int VEC, int NV, int THREADS>
+__global__ void __launch_bounds__(THREADS) block_norm_kernel(const NormArgs a) {
     __shared__ float sums[2][32];
     const int units = a.cols / VEC;
     const T *y = reinterpret_cast<const T *>(a.y);
     const R *res = reinterpret_cast<const R *>(a.residual);
+    const W *pre = reinterpret_cast<const W *>(a.pre), *post = reinterpret_cast<const W *>(a.post);
     const T *gate = reinterpret_cast<const T *>(a.gate);
     T *normed = reinterpret_cast<T *>(a.normed);
     R *res_out = reinterpret_cast<R *>(a.residual_out);
     const float inv_cols = 1.f / (float)a.cols;
-    Piece<W, VEC> pre[NV], post[NV];
-    Piece<T, VEC> py[NV], pg[NV];
-    Piece<R, VEC> pr[NV];
-    auto column = [&](int i) { return (int)(threadIdx.x + i * blockDim.x); };
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (column(i) < units) {
-            pre[i].load(reinterpret_cast<const W *>(a.pre) + column(i) * VEC);
-            if (a.post) post[i].load(reinterpret_cast<const W *>(a.post) + column(i) * VEC);
-            if (a.gate_kind == WISP_GATE_CHANNEL) pg[i].load(gate + column(i) * VEC);
-        }
-    auto load_row = [&](int64_t row) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (column(i) < units) {
-                py[i].load(y + row * a.y_stride + column(i) * VEC);
-                pr[i].load(res + row * a.res_stride + column(i) * VEC);
-            }
-    };
-    int64_t row = blockIdx.x;
-    if (row < a.rows) load_row(row);
-    for (; row < a.rows; row += gridDim.x) {
-        float v[NV][VEC], r[NV][VEC];
-        float sum = 0.f;
-        float token_gate = a.scale;
-        if (a.gate_kind == WISP_GATE_TOKEN) token_gate *= to_f<T>(gate[row * a.gate_stride]);
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        Piece<T, VEC> py[NV];
+        Piece<R, VEC> pr[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const bool in = column(i) < units;
-            if (in && a.gate_kind == WISP_GATE_FULL) pg[i].load(gate + row * a.gate_stride + column(i) * VEC);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                v[i][j] = in ? py[i].get(j) : 0.f;
-                r[i][j] = in ? pr[i].get(j) : 0.f;
-                sum += v[i][j] * v[i][j];
+            const int c = threadIdx.x + i * blockDim.x;
+            if (c < units) {
+                py[i].load(y + row * a.y_stride + c * VEC);
+                pr[i].load(res + row * a.res_stride + c * VEC);
             }
         }
-        if (row + gridDim.x < a.rows) load_row(row + gridDim.x);
-        if (a.post) {
-            const float rms = rsqrtf(block_sum(sum, sums[0]) * inv_cols + a.eps);
+        const float token_gate =
+            a.gate_kind == WISP_GATE_TOKEN ? a.scale * to_f<T>(gate[row * a.gate_stride]) : a.scale;
+        float rms = 1.f;
+        if (post) {
+            float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < NV; ++i)
+                if (threadIdx.x + i * blockDim.x < units)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) v[i][j] *= rms * post[i].get(j);
+                    for (int j = 0; j < VEC; ++j) sum += py[i].get(j) * py[i].get(j);
+            rms = rsqrtf(block_sum(sum, sums[0]) * inv_cols + a.eps);
         }
-        sum = 0.f;
+        float r[NV][VEC];
+        float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const bool in = column(i) < units;
+            const int c = threadIdx.x + i * blockDim.x;
+            if (c >= units) continue;
+            float z[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) z[j] = py[i].get(j);
+            if (post) {
+                Piece<W, VEC> w;
+                w.load(post + c * VEC);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) z[j] *= rms * w.get(j);
+            }
+            if (a.gate_kind >= WISP_GATE_CHANNEL) {
+                Piece<T, VEC> g;
+                g.load(gate + (a.gate_kind == WISP_GATE_FULL ? row * a.gate_stride : 0) + c * VEC);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) z[j] *= g.get(j);
+            }
+            Piece<R, VEC> ro;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const float g = a.gate_kind >= WISP_GATE_CHANNEL ? token_gate * pg[i].get(j) : token_gate;
-                r[i][j] = in ? fmaf(g, v[i][j], r[i][j]) : 0.f;
+                r[i][j] = fmaf(token_gate, z[j], pr[i].get(j));
                 sum += r[i][j] * r[i][j];
+                ro.set(j, r[i][j]);
             }
+            ro.store(res_out + row * a.cols + c * VEC);
         }
-        const float rms = rsqrtf(block_sum(sum, sums[1]) * inv_cols + a.eps);
+        rms = rsqrtf(block_sum(sum, sums[1]) * inv_cols + a.eps);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (column(i) >= units) continue;
-            Piece<R, VEC> ro;
+            const int c = threadIdx.x + i * blockDim.x;
+            if (c >= units) continue;
+            Piece<W, VEC> w;
+            w.load(pre + c * VEC);
             Piece<T, VEC> no;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                ro.set(j, r[i][j]);
-                no.set(j, r[i][j] * rms * pre[i].get(j));
-            }
-            ro.store(res_out + row * a.cols + column(i) * VEC);
-            no.store(normed + row * a.cols + column(i) * VEC);
+            for (int j = 0; j < VEC; ++j) no.set(j, r[i][j] * rms * w.get(j));
+            no.store(normed + row * a.cols + c * VEC);
         }
-        if (!a.post) __syncthreads();  // sums[1] of this row is read before the next row's sum goes there
+        if (!post) __syncthreads();  // sums[1] of this row is read before the next row's sum goes there
     }
 }
 
-template <typename T, typename R, typename W, int VEC, int NV>
+template <typename T, typename R, typename W, int VEC, int NV, int THREADS>
 int launch(const NormArgs &a, cudaStream_t stream) {
     const int units = a.cols / VEC;
     const int threads = ((units + NV - 1) / NV + 31) / 32 * 32;
-    if (threads > kMaxThreads)
-        return set_error("wisp_block_norm: rows this wide are not supported"), WISP_ERR_UNSUPPORTED;
-    auto kernel = block_norm_kernel<T, R, W, VEC, NV>;
-    int dev = 0, sms = 0, per = 0;
-    WISP_CUDA_TRY(cudaGetDevice(&dev));
-    WISP_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    WISP_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, 0));
-    const int64_t most = (int64_t)sms * (per > 0 ? per : 1);
+    auto kernel = block_norm_kernel<T, R, W, VEC, NV, THREADS>;
+    // more CTAs than an SM holds: the next row starts when one ends
+    const int64_t most = 148 * 64;
     kernel<<<(unsigned)(a.rows < most ? a.rows : most), threads, 0, stream>>>(a);
     WISP_CUDA_TRY(cudaGetLastError());
     return WISP_OK;
@@ -201,16 +191,18 @@ int dispatch(const NormArgs &a, cudaStream_t stream) {
                ok(a.normed, a.cols, sizeof(T)) && ok(a.residual_out, a.cols, sizeof(R));
     };
     if (fits(8)) {
-        if (a.cols <= 8 * 256) return launch<T, R, W, 8, 1>(a, stream);
-        if (a.cols <= 8 * 512) return launch<T, R, W, 8, 2>(a, stream);
-        return launch<T, R, W, 8, 4>(a, stream);
+        if (a.cols <= 8 * 256) return launch<T, R, W, 8, 1, 256>(a, stream);
+        if (a.cols <= 8 * 512) return launch<T, R, W, 8, 2, 256>(a, stream);
+        return launch<T, R, W, 8, 2, 1024>(a, stream);
     }
     if (fits(2)) {
-        if (a.cols <= 2 * 512) return launch<T, R, W, 2, 2>(a, stream);
-        return launch<T, R, W, 2, 8>(a, stream);
+        if (a.cols <= 2 * 512) return launch<T, R, W, 2, 2, 256>(a, stream);
+        if (a.cols <= 2 * 2048) return launch<T, R, W, 2, 8, 256>(a, stream);
+        return launch<T, R, W, 2, 8, 1024>(a, stream);
     }
-    if (a.cols <= 1024) return launch<T, R, W, 1, 4>(a, stream);
-    return launch<T, R, W, 1, 16>(a, stream);
+    if (a.cols <= 1024) return launch<T, R, W, 1, 4, 256>(a, stream);
+    if (a.cols <= 4096) return launch<T, R, W, 1, 16, 256>(a, stream);
+    return launch<T, R, W, 1, 16, 1024>(a, stream);
 }
 
 template <typename T>

@@ -8,6 +8,9 @@ fallback and no autograd: weights in 4 bits are for serving.
 """
 from __future__ import annotations
 
+import ctypes
+import functools
+
 import torch
 
 from . import _lib
@@ -109,4 +112,79 @@ def mx4_dequantize(q: Mx4Tensor, dtype: torch.dtype = torch.bfloat16, out: torch
     return out
 
 
-__all__ = ["Mx4Tensor", "mx4_quantize", "mx4_dequantize"]
+MOE_MAX_TOKENS = 64
+
+
+@functools.lru_cache(maxsize=256)
+def _moe_workspace(tokens: int, experts: int, top_k: int, hidden: int, inter: int) -> int:
+    n = ctypes.c_int64(0)
+    _lib.check(_lib.lib().wisp_mx4_moe_workspace(tokens, experts, top_k, hidden, inter, ctypes.byref(n)), "mx4_moe")
+    return n.value
+
+
+def mx4_moe(x: torch.Tensor, w13: Mx4Tensor, w2: Mx4Tensor, top_k: int | None = None, *,
+            router: torch.Tensor | None = None, renormalize: bool = True, topk_weights: torch.Tensor | None = None,
+            topk_ids: torch.Tensor | None = None, expert_map: torch.Tensor | None = None,
+            out: torch.Tensor | None = None) -> torch.Tensor:
+    """A whole MoE layer for at most 64 tokens, in one launch (``wisp_mx4_moe``): routing, gate-up, SiLU, down and the
+    weighted sum, from MXFP4 experts and bf16 activations.
+
+    ``x [T, H]`` bf16; ``w13 [S, 2I, H]`` (gate rows, then up rows) and ``w2 [S, H, I]``.  Routing is either the
+    layer's ``router [E, H]`` (bf16) with ``top_k``: softmax over the ``top_k`` largest products (over all of them and
+    not renormalised with ``renormalize=False``), ties to the lower id; or ``topk_weights [T, k]`` (fp32) and
+    ``topk_ids [T, k]`` (int32 or int64).  ``expert_map [E]`` (int32) gives each expert's slot, the row of ``w13`` and
+    ``w2`` it lies in (a paged layer's ``expert_map_device``); without it the slot is the id.  Ids outside ``[0, E)``
+    and experts without a slot contribute nothing.  Returns ``[T, H]`` bf16."""
+    dev = need_cuda("x", x)
+    if x.dtype != torch.bfloat16:
+        raise TypeError(f"mx4_moe computes from bf16 activations; got {x.dtype}")
+    if x.dim() != 2 or w13.codes.dim() != 3 or w2.codes.dim() != 3:
+        raise ValueError("x is [T, H], w13 [S, 2I, H] and w2 [S, H, I]")
+    tokens, hidden = x.shape
+    slots, inter2, half = w13.codes.shape
+    if 2 * half != hidden or inter2 % 2 or w2.codes.shape != (slots, hidden, inter2 // 4):
+        raise ValueError(f"shapes do not match: x {tuple(x.shape)}, w13 {tuple(w13.shape)}, w2 {tuple(w2.shape)}")
+    if tokens > MOE_MAX_TOKENS:
+        raise ValueError(f"mx4_moe takes at most {MOE_MAX_TOKENS} tokens a call; got {tokens} (mx4_quantize and "
+                         "mx4_matmul serve longer ones)")
+    same_device(dev, w13=w13, w2=w2, router=router, topk_weights=topk_weights, topk_ids=topk_ids,
+                expert_map=expert_map)
+    experts = slots if expert_map is None else expert_map.numel()
+    if expert_map is not None and (expert_map.dtype != torch.int32 or not expert_map.is_contiguous()):
+        raise TypeError("expert_map must be a contiguous int32 tensor")
+    rp = ip = wp = None
+    ids64 = 0
+    if router is not None:
+        if topk_ids is not None or topk_weights is not None or top_k is None:
+            raise ValueError("give either router and top_k, or topk_weights and topk_ids")
+        if router.dtype != torch.bfloat16 or tuple(router.shape) != (experts, hidden) or not router.is_contiguous():
+            raise ValueError(f"router must be a contiguous bf16 [{experts}, {hidden}] tensor")
+        rp = router.data_ptr()
+    else:
+        if topk_ids is None or topk_weights is None:
+            raise ValueError("give either router and top_k, or topk_weights and topk_ids")
+        if topk_ids.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"topk_ids must be int32 or int64; got {topk_ids.dtype}")
+        if topk_ids.dim() != 2 or topk_ids.shape[0] != tokens or topk_weights.shape != topk_ids.shape:
+            raise ValueError("topk_ids and topk_weights are [T, k]")
+        if top_k is not None and top_k != topk_ids.shape[1]:
+            raise ValueError(f"top_k is {top_k}, topk_ids {tuple(topk_ids.shape)}")
+        top_k = topk_ids.shape[1]
+        topk_ids, topk_weights = topk_ids.contiguous(), topk_weights.to(torch.float32).contiguous()
+        ip, wp, ids64 = topk_ids.data_ptr(), topk_weights.data_ptr(), int(topk_ids.dtype == torch.int64)
+    if x.stride(1) != 1 or (tokens > 1 and (x.stride(0) < hidden or x.stride(0) % 8)) or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    out = (torch.empty((tokens, hidden), dtype=torch.bfloat16, device=dev) if out is None
+           else need_out("out", out, (tokens, hidden), torch.bfloat16, dev))
+    need = _moe_workspace(tokens, experts, top_k, hidden, inter2 // 2)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    with on(dev):
+        _lib.check(_lib.lib().wisp_mx4_moe(
+            x.data_ptr(), x.stride(0), rp, ip, ids64, wp, None if expert_map is None else expert_map.data_ptr(),
+            w13.codes.data_ptr(), w13.scales.data_ptr(), w2.codes.data_ptr(), w2.scales.data_ptr(), slots, tokens,
+            experts, top_k, hidden, inter2 // 2, int(renormalize), ws.data_ptr(), need, out.data_ptr(),
+            stream_of(dev)), "mx4_moe")
+    return out
+
+
+__all__ = ["Mx4Tensor", "mx4_quantize", "mx4_dequantize", "mx4_moe"]

@@ -137,6 +137,23 @@ WISP_API int wisp_mx4_dequantize(const void *codes, const void *scales, int64_t 
                                  int32_t dtype, void *stream);
 
 /*
+ * Products of MXFP4 matrices, grouped (the products of MoE experts over many
+ * tokens): out[r] = A[r] W[g]^T for offsets[g] <= r < offsets[g + 1].
+ * A [rows][k]; W [groups][n][k]; out [rows][n] bf16, fp32 accumulation, one
+ * rounding.  offsets: int32 [groups + 1] on the device, ascending, or NULL
+ * for one group of all rows; rows of no group are left as they are.  Codes
+ * aligned to 16 bytes; at most 1024 groups.
+ */
+WISP_API int wisp_mx4_matmul(const void *a_codes, const void *a_scales, int64_t rows, const void *w_codes,
+                             const void *w_scales, int32_t groups, int32_t n, int32_t k, const int32_t *offsets,
+                             void *out, void *stream);
+/*
+ * Wait for `stream` and report (then clear) a bounded wait that ran out inside
+ * wisp_mx4_matmul on the current device (WISP_ERR_TIMEOUT).
+ */
+WISP_API int wisp_mx4_sync(void *stream);
+
+/*
  * A whole MoE layer for a few tokens from MXFP4 experts, in one (cooperative)
  * launch: out[t] = sum over the token's experts e of p_e W2[e] (silu(g) u),
  * [g; u] = W13[e] x[t].  x [T][hidden] bf16 (rows x_stride values apart).

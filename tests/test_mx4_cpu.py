@@ -130,3 +130,25 @@ def test_moe_refusals():
     refused(_lib.lib().wisp_mx4_moe_workspace(65, 4, 2, 64, 32, ctypes.byref(n)), "64 tokens")
     refused(_lib.lib().wisp_mx4_moe_workspace(4, 4, 2, 64, 32, None), "NULL")
     assert _lib.lib().wisp_mx4_moe_workspace(4, 4, 2, 64, 32, ctypes.byref(n)) == 0 and n.value >= 4 * 64 * 2
+
+
+def test_matmul_refusals():
+    f = _lib.lib().wisp_mx4_matmul
+
+    def call(rows=1, groups=1, n=8, k=32, a=P, s=P, w=P, offsets=None, out=P):
+        return f(a, s, rows, w, P, groups, n, k, offsets, out, None)
+    refused(call(rows=-1), "rows")
+    refused(call(rows=(1 << 30) + 1), "rows")
+    refused(call(groups=0), "groups")
+    refused(call(groups=1025, offsets=P), "groups")
+    refused(call(n=0), "n >= 1")
+    refused(call(k=48), "multiple of 32")
+    refused(call(k=0), "multiple of 32")
+    refused(call(groups=1024, n=1 << 22, offsets=P), "too large")
+    refused(call(groups=2), "offsets")
+    refused(call(a=None), "NULL")
+    refused(call(out=None), "NULL")
+    refused(call(a=P + 8), "aligned")
+    refused(call(w=P + 4), "aligned")
+    refused(call(out=P + 1), "out")
+    assert call(rows=0) == _lib.WISP_OK

@@ -52,6 +52,8 @@ SIGNATURES = {
     "wisp_route_topk": (ctypes.c_int, [_vp, _c_int32, _c_int32, _c_int32, _c_int32, _c_int32, _vp, _vp, _vp]),
     "wisp_mx4_quantize": (ctypes.c_int, [_vp, _c_int32, _c_int64, _c_int64, _c_int64, _vp, _vp, _vp]),
     "wisp_mx4_dequantize": (ctypes.c_int, [_vp, _vp, _c_int64, _c_int64, _vp, _c_int32, _vp]),
+    "wisp_mx4_matmul": (ctypes.c_int, [_vp, _vp, _c_int64, _vp, _vp, _c_int32, _c_int32, _c_int32, _vp, _vp, _vp]),
+    "wisp_mx4_sync": (ctypes.c_int, [_vp]),
     "wisp_mx4_moe_workspace": (ctypes.c_int, [_c_int32] * 5 + [_p64]),
     "wisp_mx4_moe": (ctypes.c_int, [_vp, _c_int64, _vp, _vp, _c_int32, _vp, _vp, _vp, _vp, _vp, _vp] +
                      [_c_int32] * 7 + [_vp, _c_int64, _vp, _vp]),

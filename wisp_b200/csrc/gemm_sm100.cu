@@ -527,6 +527,20 @@ int make_map(CUtensorMap *map, const void *base, uint64_t rows, uint64_t cols, u
     return WISP_OK;
 }
 
+int make_byte_map(CUtensorMap *map, const void *base, uint64_t rows, uint64_t row_bytes, uint32_t box_rows) {
+    std::call_once(g_encode_once, init_encode);
+    if (!g_encode) return set_error("wisp: cuTensorMapEncodeTiled is not available"), WISP_ERR_UNSUPPORTED;
+    const cuuint64_t dims[2] = {row_bytes, rows};
+    const cuuint64_t strides[1] = {row_bytes};
+    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box,
+                                estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error("wisp: cuTensorMapEncodeTiled failed"), WISP_ERR_CUDA;
+    return WISP_OK;
+}
+
 int launch_gather(const PrefillGroup &p, cudaStream_t stream) {
     const int warps = 8;
     const int blocks = (p.npairs + warps - 1) / warps;

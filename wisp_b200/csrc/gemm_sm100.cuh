@@ -298,6 +298,9 @@ __device__ __forceinline__ int group_experts(const int32_t *nu_dev, const int32_
 // Row-major bf16 matrix [rows][cols] (16-byte aligned base, cols % 8 == 0) as
 // 64 x box_rows boxes with 128-byte swizzle.
 int make_map(CUtensorMap *map, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows);
+// Rows of bytes (16-byte aligned base, row_bytes % 16 == 0) as 128 x box_rows
+// boxes with 128-byte swizzle.
+int make_byte_map(CUtensorMap *map, const void *base, uint64_t rows, uint64_t row_bytes, uint32_t box_rows);
 // X_perm rows of the group.
 int launch_gather(const PrefillGroup &p, cudaStream_t stream);
 // out rows [t0, t1) = routing-order sum of the weighted rows y.

@@ -1,0 +1,110 @@
+// tcgen05.mma on MXFP4 operands (kind::mxf4, one E8M0 scale for 32 values).
+//
+// Operand tiles lie in shared memory as TMA boxes of 128 bytes (256 values) a
+// row with 128-byte swizzle; one instruction takes 64 values of K, 32 bytes
+// along the row.  The scales of an instruction lie in tensor memory: of 128
+// rows, row 32 g + l in lane l, column c + g (all four lane quarters hold a
+// copy), its four scale bytes of 128 values of K in one 32-bit cell, of which
+// an instruction of K 64 uses the lower or the upper half (the scale id of
+// the instruction descriptor, 0 or 2).  tcgen05.cp 32x128b.warpx4 brings such
+// a block there from 512 bytes of shared memory in which row 32 g + l's word
+// lies at 16 l + 4 g ("scale atom").
+#pragma once
+#include "gemm_sm100.cuh"
+#include "mx4.cuh"
+
+namespace wisp {
+namespace mx4 {
+
+using gemm::mbar_arrive;
+using gemm::mbar_expect_tx;
+using gemm::mbar_init;
+using gemm::mbar_try;
+using gemm::s_addr;
+using gemm::smem_desc_k_sw128;
+using gemm::tc_fence_after;
+using gemm::tc_fence_before;
+using gemm::tma_load_2d;
+using gemm::umma_commit;
+
+constexpr int kStepK = 256;                 // values of K in a stage: 128 bytes a row
+constexpr int kStepBlocks = kStepK / kBlock;  // scale bytes of a row in a stage
+constexpr int kAtomBytes = 512;             // scales of 128 rows x 128 values
+constexpr long long kWaitNs = 2000000000;   // limit of one wait
+
+// Device word of the kernels' sticky status on the current device (mx4_matmul.cu).
+int status_word(int **word);
+
+// Instruction descriptor: E2M1 A and B, K-major, E8M0 scales, fp32 D, M x N;
+// `sf` 0 or 2: which half of the scale words (K 64 of 128).
+__host__ __device__ constexpr uint32_t idesc_mxf4(int M, int N, int sf) {
+    return ((uint32_t)sf << 4)            // scale id of B
+           | (1u << 7)                    // A: E2M1
+           | (1u << 10)                   // B: E2M1
+           | ((uint32_t)(N >> 3) << 17)   // N / 8
+           | (1u << 23)                   // scales: E8M0
+           | ((uint32_t)(M >> 7) << 27)   // M / 128
+           | ((uint32_t)sf << 29);        // scale id of A
+}
+__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                          uint32_t tmem_sfa, uint32_t tmem_sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(
+            tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sfa), "r"(tmem_sfb), "r"(accumulate)
+        : "memory");
+}
+// Scale atom: 32 rows of 16 bytes, groups of 8 rows 128 bytes apart, no swizzle.
+__device__ __forceinline__ uint64_t smem_desc_atom(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t)1u << 16;           // leading byte offset (one column of core matrices: not used)
+    d |= (uint64_t)(128u >> 4) << 32;  // stride byte offset
+    d |= (uint64_t)1u << 46;           // version
+    return d;
+}
+// One scale atom to four columns of tensor memory, in every lane quarter.
+__device__ __forceinline__ void copy_atom(uint32_t taddr, uint32_t saddr) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc_atom(saddr)) : "memory");
+}
+// Byte offset of row r's word in a scale atom.
+__device__ __forceinline__ int atom_at(int r) { return (r & 31) * 16 + (r >> 5) * 4; }
+
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Bounded wait; a wait that runs out sets the status and the CTA's abort word.
+__device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
+    if (gemm::mbar_wait(bar, parity, kWaitNs, abort)) return true;
+    *abort = 1;
+    *reinterpret_cast<volatile int *>(status) = WISP_ERR_TIMEOUT;
+    return false;
+}
+
+// The eight scale bytes of a row in stage kb (bytes behind the row's last: 0).
+// `align`: what the rows' scale bytes are aligned to.
+__device__ __forceinline__ uint2 load_scales(const uint8_t *row, int kb, int blocks, int align) {
+    const uint8_t *p = row + kb * kStepBlocks;
+    const int left = blocks - kb * kStepBlocks;
+    if (align >= 8) return __ldg(reinterpret_cast<const uint2 *>(p));
+    uint2 v = make_uint2(0, 0);
+    if (align >= 4) {
+        v.x = __ldg(reinterpret_cast<const uint32_t *>(p));
+        if (left > 4) v.y = __ldg(reinterpret_cast<const uint32_t *>(p) + 1);
+        return v;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (i < left) v.x |= (uint32_t)__ldg(p + i) << (8 * i);
+        if (i + 4 < left) v.y |= (uint32_t)__ldg(p + i + 4) << (8 * i);
+    }
+    return v;
+}
+// What a matrix's rows of scale bytes are aligned to.
+__host__ __device__ inline int scale_align(const void *scales, int blocks) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(scales) | (uintptr_t)blocks;
+    return p % 8 == 0 ? 8 : p % 4 == 0 ? 4 : 1;
+}
+
+}  // namespace mx4
+}  // namespace wisp

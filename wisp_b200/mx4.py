@@ -112,6 +112,45 @@ def mx4_dequantize(q: Mx4Tensor, dtype: torch.dtype = torch.bfloat16, out: torch
     return out
 
 
+def mx4_matmul(a: Mx4Tensor, w: Mx4Tensor, offsets: torch.Tensor | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """Products of MXFP4 matrices on the block-scaled tensor cores (``wisp_mx4_matmul``).
+
+    ``a [M, K]`` times ``w [N, K]`` transposed; or, grouped, ``w [G, N, K]`` with ``offsets [G + 1]`` (int32, ascending,
+    on the device): rows ``offsets[g]`` to ``offsets[g + 1]`` times ``w[g]`` transposed, the products of MoE experts
+    over rows sorted by expert.  Returns ``[M, N]`` bf16 (fp32 accumulation, one rounding).  Rows behind the last
+    offset are left as they are in ``out`` (undefined in a new tensor)."""
+    dev = need_cuda("a", a.codes)
+    if a.codes.dim() != 2 or w.codes.dim() not in (2, 3) or w.codes.shape[-1] != a.codes.shape[1]:
+        raise ValueError(f"a is [M, K], w [N, K] or [G, N, K]; got {tuple(a.shape)} and {tuple(w.shape)}")
+    rows, half = a.codes.shape
+    n = w.codes.shape[-2]
+    groups = w.codes.shape[0] if w.codes.dim() == 3 else 1
+    op = None
+    if offsets is not None:
+        if offsets.dtype != torch.int32 or offsets.shape != (groups + 1,) or not offsets.is_contiguous():
+            raise ValueError(f"offsets must be a contiguous int32 [{groups + 1}] tensor; got {offsets.dtype} "
+                             f"{tuple(offsets.shape)}")
+        op = offsets.data_ptr()
+    elif groups != 1:
+        raise ValueError(f"{groups} groups need offsets")
+    same_device(dev, w=w, offsets=offsets)
+    out = (torch.empty((rows, n), dtype=torch.bfloat16, device=dev) if out is None
+           else need_out("out", out, (rows, n), torch.bfloat16, dev))
+    with on(dev):
+        _lib.check(_lib.lib().wisp_mx4_matmul(
+            a.codes.data_ptr(), a.scales.data_ptr(), rows, w.codes.data_ptr(), w.scales.data_ptr(), groups, n, 2 * half,
+            op, out.data_ptr(), stream_of(dev)), "mx4_matmul")
+    return out
+
+
+def mx4_synchronize(device: torch.device | None = None) -> None:
+    """Wait for the device's current stream and raise if a bounded wait inside an :func:`mx4_matmul` ran out."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with on(dev):
+        _lib.check(_lib.lib().wisp_mx4_sync(stream_of(dev)), "mx4_synchronize")
+
+
 MOE_MAX_TOKENS = 64
 
 
@@ -187,4 +226,4 @@ def mx4_moe(x: torch.Tensor, w13: Mx4Tensor, w2: Mx4Tensor, top_k: int | None = 
     return out
 
 
-__all__ = ["Mx4Tensor", "mx4_quantize", "mx4_dequantize", "mx4_moe"]
+__all__ = ["Mx4Tensor", "mx4_quantize", "mx4_dequantize", "mx4_matmul", "mx4_moe", "mx4_synchronize"]

@@ -100,9 +100,9 @@ def test_moe_refusals():
     import ctypes
     f = _lib.lib().wisp_mx4_moe
 
-    def call(T=1, E=4, k=2, H=64, I=32, slots=4, x=P, router=P, ids=None, w=None, emap=None, c13=P, s13=P, ws=P,
-             nbytes=1 << 30, stride=64):
-        return f(x, stride, router, ids, 0, w, emap, c13, s13, P, P, slots, T, E, k, H, I, 1, ws, nbytes, P, None)
+    def call(T=1, E=4, k=2, H=64, I=32, slots=4, x=P, router=P, ids=None, w=None, emap=None, c13=P, ws=P,
+             nbytes=1 << 30, stride=64, out=P):
+        return f(x, stride, router, ids, 0, w, emap, c13, P, P, P, slots, T, E, k, H, I, 1, ws, nbytes, out, None)
     refused(call(T=65), "64 tokens")
     refused(call(T=-1), "64 tokens")
     refused(call(E=1025), "1024 experts")
@@ -120,8 +120,9 @@ def test_moe_refusals():
     refused(call(router=None, ids=P), "either")
     refused(call(slots=3), "slots")
     refused(call(c13=P + 8), "aligned")
-    refused(call(s13=P + 2), "aligned")
+    refused(call(out=P + 8), "aligned")
     refused(call(ws=P + 4), "aligned")
+    refused(call(slots=1 << 26, I=32), "rows")
     refused(call(T=2, stride=32), "overlap")
     refused(call(T=2, stride=68), "16-byte")
     refused(call(nbytes=64), "workspace")

@@ -5,37 +5,42 @@
 //   h = W13[e] x, a = silu(h[:I]) h[I:], y = W2[e] a     for each routed e
 //   out = sum over the token's experts of p_e y_e
 //
-// Weights are MXFP4 in checkpoint layout, activations 16-bit floats: a product
-// multiplies the E2M1 value (exact in fp16) with the activation (fp16, scaled
-// by a power of two of its own row so that the largest lies in [2^14, 2^15):
-// exact for bf16 activations down to 2^-29 of the row's largest), sums 32 of
-// them in fp32 on the tensor cores, and adds the block's sum times the block's
-// scale to the fp32 accumulator.  h, the SiLU and the weighted sum are fp32; a
-// is rounded to fp16 once (half a step of 2^-11; groups of 8 share a power of
-// two, which the down product brings to one for the pair) and out to bf16 once.
+// Weights are MXFP4 in checkpoint layout and go to the block-scaled tensor
+// cores (tcgen05.mma kind::mxf4) as they are: nothing is unpacked on the way.
+// Activations keep their precision: a block of 32 of them is written as a sum
+// of six MXFP4 terms, each the rounding of what the terms before it left.  A
+// term's scale is the smallest power of two under which the remainder's
+// largest value is at most 6, so a term leaves less than a quarter of it (a
+// sixth, mostly): six leave between 2^-12 and 2^-15 of the block's largest
+// value, below the 2^-9 that bf16 activations carry.  The terms of a token are
+// rows of the product's small operand: 8 rows a token (the rows of a swizzle
+// pattern, two of them unused), 16 tokens a tile; weights take the 128 rows of
+// the other side, a token's result is the sum of its six accumulator columns.
+// h, the SiLU and the weighted sum are fp32; out is rounded to bf16 once.
+// (Unpacking to fp16 for mma.sync instead cost 110 us at 16 tokens of a
+// Qwen3-30B-A3B layer, three times this kernel: it is bound by the four
+// hundred instructions that 128 columns of 16 rows take.)
 //
 // Bound by HBM: a few tokens use every byte of a routed expert once.  A
-// cooperative launch of one 512-thread CTA per SM runs
-//   R  router products (a warp per expert row and four tokens), x to fp16
+// cooperative launch of one CTA of ten warps per SM runs
+//   R  router products (a warp per expert row and token group), x to terms
 //   S  (after a grid barrier, every CTA for itself) top-k and the lists of
-//      each expert's tokens
-//   G  gate-up: a warp takes 8 gate rows and the matching 8 up rows of an
-//      expert as the 16 rows of mma.m16n8k16, so g and u of a value meet in
-//      one thread; tokens are the 8 columns (1, 2, 4 or 8 column tiles)
-//   D  (after a second grid barrier) down: a CTA takes 16 rows of the hidden
-//      size, its warps the experts (and pieces of I, when there are few), so
-//      that a token's sum over its experts ends in one CTA: no partial sums in
-//      memory, no atomics, the same bits every run.
-// A warp streams its rows through a ring of its own in shared memory: 16 rows
-// x 128 columns (1 KB of codes and 64 scale bytes) a stage, cp.async of 16
-// bytes a lane, 7 stages ahead across its units; the 16-byte pieces of a row
-// are swizzled so that reading one word a lane is free of conflicts.  With 8
-// token columns the tensor core work is far from its limit; what counts is the
-// number of instructions a weight costs (about 1.6 a value and lane: 4
-// conversions, 2 matrix instructions and 4 multiply-adds per 16 values).
+//      each expert's tokens in groups of at most 16
+//   G  gate-up: tiles of 64 gate rows and the matching 64 up rows of a group's
+//      expert; the epilogue brings g and u of a value together through shared
+//      memory and writes silu(g) u as terms again
+//   D  (after a barrier; its first weights are on their way before it) down:
+//      tiles of 128 rows of the hidden size, the intermediate size in pieces
+//      where there are too few tiles to fill the SMs evenly; p_e y_e in fp32
+//   C  (after a barrier) the sum over a token's experts, in routing order: no
+//      atomics, the same bits every run
+// In G and D a warp each feeds a ring of 5 stages of 256 values of K (weights
+// by TMA, the terms by bulk copies of 1 KB a token, laid out by their writers
+// as the swizzle wants them) and issues the products, four bring the scale
+// bytes to shared memory four stages ahead, four read the accumulators.
 #include <cooperative_groups.h>
 
-#include "mx4.cuh"
+#include "mx4_mma.cuh"
 
 namespace wisp {
 namespace mx4 {
@@ -43,19 +48,27 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kWarps = 16;
+constexpr int kWarps = 10;
 constexpr int kThreads = kWarps * 32;
-constexpr int kStages = 2;
-constexpr int kChunk = 512;                    // columns of a stage
-constexpr int kSub = 128;                      // columns a thread's registers hold at a time
-constexpr int kRowBytes = kChunk / 2;          // codes of a row in a stage
-constexpr int kRowBlocks = kChunk / kBlock;    // 16-byte pieces of a row, and its scale bytes
-constexpr int kCodeBytes = 16 * kRowBytes;
-constexpr int kStageBytes = kCodeBytes + 16 * kRowBlocks;
+constexpr int kEpiWarp = 2, kSfWarp = 6;       // four warps each; 0: copies, 1: products
+constexpr int kTerms = 6;                      // terms of an activation
+constexpr int kRows = 8;                       // rows of a token in the small operand
+constexpr int kGroup = 16;                     // tokens of a tile
+constexpr int kStages = 5;
+constexpr int kTermBytes = kRows * 128;        // terms of a token in a stage
+constexpr int kScaleBytes = kRows * kStepBlocks;
+constexpr int kABytes = 128 * 128, kBBytes = kGroup * kTermBytes;
+constexpr int kStageBytes = kABytes + kBBytes + 4 * kAtomBytes;
+constexpr int kAccCols = kGroup * kRows;       // of an accumulator; two of them
+constexpr int kSfCol0 = 2 * kAccCols, kSfCols = 16;
+constexpr int kTmemCols = 512;
+static_assert(kSfCol0 + kStages * kSfCols <= kTmemCols, "tensor memory");
 constexpr int kMaxTokens = 64;
 constexpr int kMaxTopK = 16;
 constexpr int kMaxPairs = kMaxTokens * kMaxTopK;
 constexpr int kMaxExperts = 1024;
+constexpr int kMaxGroups = kMaxPairs;          // no group is empty
+constexpr int kMaxSplit = 8;                   // pieces of the intermediate size in D
 
 struct MoeArgs {
     const __nv_bfloat16 *x;
@@ -64,101 +77,77 @@ struct MoeArgs {
     const void *ids;
     const float *weights;
     const int32_t *expert_map;    // [E] slot of each expert, or nullptr: slot = expert
-    const uint8_t *w13, *s13, *w2, *s2;
+    const uint8_t *s13, *s2;
     __nv_bfloat16 *out;
     float *logits;                // [T][E]
-    __half *xs;                   // [T][H]
-    float *x_scale;               // [T]: x = xs * x_scale
-    __half *act;                  // [T * k][I]: silu(g) u = act * 2^(its group's exponent - 141)
-    uint8_t *act_exp;             // [T * k][exp_stride]: exponent of each group of 8 (exp_at)
-    uint32_t *act_max;            // [T * k]: the pair's largest exponent
-    int T, E, k, H, I, slots, ids64, renormalize, exp_stride;
+    uint8_t *xq, *xs;             // terms of x: [T][steps][kTermBytes], scales [T][steps][kScaleBytes]
+    uint8_t *aq, *as;             // terms of silu(g) u: the same for each pair
+    float *y;                     // [split][T * k][H]
+    int *status;
+    int T, E, k, H, I, slots, ids64, renormalize, s13_align, s2_align, max_split;
 };
 
-struct Lists {
-    int ids[kMaxPairs];             // expert of pair t * k + j, -1: none
-    float w[kMaxPairs];             // its weight
-    unsigned short pair[kMaxPairs];  // pairs by expert
+// What the lists are built from; lies where the ring will be.
+struct Scratch {
+    int ids[kMaxPairs];  // expert of pair t * k + j, -1: none
     unsigned short rank[kMaxPairs];
     int count[kMaxExperts];
-    int uslot[kMaxExperts];         // slots of the experts that have pairs
-    unsigned short uoff[kMaxExperts + 1];
     int scan[kWarps];
-    int n;                          // how many
+};
+struct Lists {
+    float w[kMaxPairs];                // routing weight of a pair
+    unsigned short pair[kMaxPairs];    // pairs by group
+    unsigned short off[kMaxGroups + 1];  // where a group's pairs begin
+    int slots[kMaxGroups];             // its expert's slot
+    unsigned char has[kMaxPairs];      // whether the pair is in a group
+    int n;                             // groups
+};
+struct Control {
+    uint64_t full[kStages], sf_full[kStages], empty[kStages];
+    uint64_t acc_full[2], acc_empty[2], mma_done;
+    uint32_t tmem_base;
+    int abort, issued, consumed;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-template <int BYTES>
-__device__ __forceinline__ void cp_async_ca(uint32_t dst, const void *src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1, const float (&c)[4]) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, "
-        "%12, %13};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
-}
-
-// Power of two that brings values whose largest has the fp32 exponent field
-// `e` into fp16, the largest in [2^14, 2^15), and its reciprocal.  e is held
-// to [15, 254].
-__device__ __forceinline__ int half_exponent(uint32_t e) { return min(max((int)e, 15), 254); }
-__device__ __forceinline__ float half_back(int e) { return __uint_as_float((uint32_t)(e - 14) << 23); }  // 2^(e - 141)
-__device__ __forceinline__ void half_scale(uint32_t field, float &to_half, float &back) {
-    const int e = half_exponent(field);
-    to_half = __uint_as_float((uint32_t)(268 - e) << 23);  // 2^(141 - e)
-    back = half_back(e);
-}
-// Where the exponent of the group of 8 intermediate values 8 g .. lies in its
-// pair's row: the four of a thread's columns in a stage of 128 are one word.
-__device__ __forceinline__ int exp_at(int g) { return (g & ~15) | ((g & 3) << 2) | ((g >> 2) & 3); }
-__device__ __forceinline__ uint32_t bf16x2_to_f16x2(uint32_t v, float s) {
-    const __half2 h = __floats2half2_rn(bf16lo(v) * s, bf16hi(v) * s);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
 // ---- phase R ------------------------------------------------------------------
-constexpr int kAhead = 8;  // 16-byte loads of a lane in flight
-
-__device__ void convert_token(const MoeArgs &a, int t, int lane) {
-    const __nv_bfloat16 *row = a.x + t * a.x_stride;
-    uint32_t m = 0;
-    for (int h0 = lane * 8; h0 < a.H; h0 += 256 * kAhead) {
-        uint4 v[kAhead];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i)
-            v[i] = h0 + i * 256 < a.H ? ld_cached16(row + h0 + i * 256) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) m = max(m, max((w[j] << 16) & 0x7FFFFFFFu, w[j] & 0x7FFF0000u));
-        }
+// One block of 32 values, one a lane, as terms: codes to `codes` (16 bytes of
+// row 0, rows 128 bytes apart, 16-byte pieces swizzled by the row) and scale
+// bytes to `scales` (rows kStepBlocks apart).
+__device__ __forceinline__ void write_terms(float v, uint8_t *codes, uint8_t *scales, int piece, int lane) {
+    for (int q = 0; q < kTerms; ++q) {
+        const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v) & 0x7FFFFFFFu);
+        const int e = (int)(m >> 23);
+        // the smallest scale under which the largest value is at most 6
+        int byte = e - 2 + ((m & 0x7FFFFFu) > 0x400000u);
+        byte = e == 255 ? 255 : max(byte, 0);
+        const float inv = byte == 255 ? 0.f : __uint_as_float((uint32_t)(254 - byte) << 23);
+        uint32_t c;
+        asm("{\n .reg .b8 b;\n cvt.rn.satfinite.e2m1x2.f32 b, %2, %1;\n cvt.u32.u8 %0, b;\n}"
+            : "=r"(c)
+            : "f"(v * inv), "f"(0.f));
+        const uint32_t h = e2m1x2_to_f16x2(c);
+        v = fmaf(-__low2float(*reinterpret_cast<const __half2 *>(&h)), scale_value(byte), v);
+        uint32_t w = c & 15;
+        w |= __shfl_down_sync(0xFFFFFFFFu, w, 1) << 4;
+        w |= __shfl_down_sync(0xFFFFFFFFu, w, 2) << 8;
+        w |= __shfl_down_sync(0xFFFFFFFFu, w, 4) << 16;
+        if ((lane & 7) == 0)
+            *reinterpret_cast<uint32_t *>(codes + q * 128 + ((piece ^ q) << 4) + (lane >> 3) * 4) = w;
+        if (lane == 0) scales[q * kStepBlocks] = (uint8_t)byte;
     }
-    m = __reduce_max_sync(0xFFFFFFFFu, m);
-    float s, back;
-    half_scale(m >> 23, s, back);
-    for (int h = lane * 8; h < a.H; h += 256) {
-        uint4 v = ld_cached16(row + h);
-        v.x = bf16x2_to_f16x2(v.x, s), v.y = bf16x2_to_f16x2(v.y, s);
-        v.z = bf16x2_to_f16x2(v.z, s), v.w = bf16x2_to_f16x2(v.w, s);
-        *reinterpret_cast<uint4 *>(a.xs + (size_t)t * a.H + h) = v;
-    }
-    if (lane == 0) a.x_scale[t] = back;
 }
+
+__device__ void convert_tokens(const MoeArgs &a, int gw, int nw, int lane) {
+    const int blocks = a.H / kBlock, steps = (blocks + kStepBlocks - 1) / kStepBlocks;
+    for (int u = gw; u < a.T * blocks; u += nw) {
+        const int t = u / blocks, b = u - t * blocks, kb = b / kStepBlocks, piece = b % kStepBlocks;
+        const float v = __bfloat162float(a.x[t * a.x_stride + b * kBlock + lane]);
+        write_terms(v, a.xq + ((size_t)t * steps + kb) * kTermBytes,
+                    a.xs + ((size_t)t * steps + kb) * kScaleBytes + piece, piece, lane);
+    }
+}
+
+constexpr int kAhead = 8;  // 16-byte loads of a lane in flight
 
 // One expert's row times TOKENS tokens.
 template <int TOKENS>
@@ -207,7 +196,7 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
 
 // Top-k of token t by (logit descending, id ascending), softmax weights.
 template <int PER_LANE>
-__device__ void route_token(const MoeArgs &a, Lists &L, int t, int lane) {
+__device__ void route_token(const MoeArgs &a, Lists &L, Scratch &S, int t, int lane) {
     uint32_t key[PER_LANE];
 #pragma unroll
     for (int i = 0; i < PER_LANE; ++i) {
@@ -244,512 +233,525 @@ __device__ void route_token(const MoeArgs &a, Lists &L, int t, int lane) {
     const float p = lane < a.k ? expf(mine - mx) : 0.f;
     const float sum = warp_sum(a.renormalize ? p : all);
     if (lane < a.k) {
-        L.ids[t * a.k + lane] = my_id;
+        S.ids[t * a.k + lane] = my_id;
         L.w[t * a.k + lane] = p / sum;
     }
 }
 
 // The caller's routing of token t; an expert named twice is taken once, with
 // the sum of its weights.
-__device__ void given_token(const MoeArgs &a, Lists &L, int t) {
+__device__ void given_token(const MoeArgs &a, Lists &L, Scratch &S, int t) {
     for (int j = 0; j < a.k; ++j) {
         const int p = t * a.k + j;
         const long long e = load_id64(a.ids, a.ids64, p);
         int id = e < 0 || e >= a.E ? -1 : (int)e;
         for (int i = 0; i < j && id >= 0; ++i)
-            if (L.ids[t * a.k + i] == id) {
+            if (S.ids[t * a.k + i] == id) {
                 L.w[t * a.k + i] += a.weights[p];
                 id = -1;
             }
-        L.ids[p] = id;
+        S.ids[p] = id;
         L.w[p] = a.weights[p];
     }
 }
 
-// Pairs by expert, experts with a slot in ascending order.  (The order of an
-// expert's pairs is not fixed: each is a column of its own.)
-__device__ void build_lists(const MoeArgs &a, Lists &L) {
+// Pairs by expert, the experts with a slot in ascending order, in groups of at
+// most kGroup.  Every CTA has to come to the same groups, so an expert's pairs
+// keep their order: one warp counts them, 32 at a time.
+__device__ void build_lists(const MoeArgs &a, Lists &L, Scratch &S) {
+    constexpr int kPer = (kMaxExperts + kThreads - 1) / kThreads;
     const int P = a.T * a.k, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    for (int p = tid; p < P; p += kThreads) {
-        const int e = L.ids[p];
-        L.rank[p] = (unsigned short)(e >= 0 ? atomicAdd(&L.count[e], 1) : 0);
-    }
+    if (warp == 0)
+        for (int p0 = 0; p0 < P; p0 += 32) {
+            const int p = p0 + lane, e = p < P ? S.ids[p] : -1;
+            const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
+            const int before = e >= 0 ? S.count[e] : 0;
+            __syncwarp();
+            if (e >= 0) {
+                S.rank[p] = (unsigned short)(before + __popc(same & ((1u << lane) - 1)));
+                if (lane == __ffs(same) - 1) S.count[e] = before + __popc(same);
+            }
+            __syncwarp();
+        }
     __syncthreads();
-    int count[2], slot[2];
+    int count[kPer], slot[kPer], own = 0;  // pairs in the low half of `own`, groups in the high half
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int e = tid * 2 + i;
-        count[i] = e < a.E ? L.count[e] : 0;
+    for (int i = 0; i < kPer; ++i) {
+        const int e = tid * kPer + i;
+        count[i] = e < a.E ? S.count[e] : 0;
         if (!count[i]) continue;
         slot[i] = a.expert_map ? a.expert_map[e] : e;
         if (slot[i] < 0 || slot[i] >= a.slots) count[i] = 0;
+        own += count[i] + ((count[i] + kGroup - 1) / kGroup << 16);
     }
-    // pairs in the low half, experts in the high half
-    const int own = count[0] + count[1] + (((count[0] > 0) + (count[1] > 0)) << 16);
     int run = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xFFFFFFFFu, run, o);
         if (lane >= o) run += v;
     }
-    if (lane == 31) L.scan[warp] = run;
+    if (lane == 31) S.scan[warp] = run;
     __syncthreads();
     int before = run - own, total = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-        const int v = L.scan[w];
+        const int v = S.scan[w];
         if (w < warp) before += v;
         total += v;
     }
-    int pos = before & 0xFFFF, u = before >> 16;
+    int pos = before & 0xFFFF, g = before >> 16;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int e = tid * 2 + i;
-        if (e < a.E) L.count[e] = count[i] ? pos : -1;  // from here on: where the expert's pairs begin
-        if (!count[i]) continue;
-        L.uslot[u] = slot[i];
-        L.uoff[u++] = (unsigned short)pos;
+    for (int i = 0; i < kPer; ++i) {
+        const int e = tid * kPer + i;
+        if (e < a.E) S.count[e] = count[i] ? pos : -1;  // from here on: where the expert's pairs begin
+        for (int done = 0; done < count[i]; done += kGroup, ++g) {
+            L.slots[g] = slot[i];
+            L.off[g] = (unsigned short)(pos + done);
+        }
         pos += count[i];
     }
     if (tid == 0) {
         L.n = total >> 16;
-        L.uoff[total >> 16] = (unsigned short)(total & 0xFFFF);
+        L.off[total >> 16] = (unsigned short)(total & 0xFFFF);
     }
     __syncthreads();
     for (int p = tid; p < P; p += kThreads) {
-        const int e = L.ids[p], at = e >= 0 ? L.count[e] : -1;
-        if (at >= 0) L.pair[at + L.rank[p]] = (unsigned short)p;
+        const int e = S.ids[p], at = e >= 0 ? S.count[e] : -1;
+        L.has[p] = at >= 0;
+        if (at >= 0) L.pair[at + S.rank[p]] = (unsigned short)p;
     }
     __syncthreads();
 }
 
-// ---- the weight stream of a warp ------------------------------------------------
-// 16 rows: 8 from `a` on and 8 from `b` on, row_bytes apart; their scale bytes
-// from `sa` and `sb` on, blocks apart.
-struct Source {
-    const uint8_t *a, *b, *sa, *sb;
+// ---- phases G and D ---------------------------------------------------------------
+// The tiles of a phase: tile t belongs to group t / per_group.  Weight rows:
+// the first 64 from slot * slot_rows + m0 on, the second 64 from `second`
+// rows further on.  K: `blocks` scale bytes a row, steps of 256 values, in
+// `split` pieces.
+struct Phase {
+    const CUtensorMap *map;
+    const uint8_t *w_scales, *b_codes, *b_scales;
+    int64_t w_rows;  // rows of the weight matrix
+    int tiles, per_group, m_tiles, split, rows_m, slot_rows, second, blocks, steps, align, token_div;
 };
-// 16-byte piece (row r of 16, block b of the stage): swizzled, so that the
-// words that 8 rows' lanes read together lie in different banks.
-__device__ __forceinline__ uint32_t piece_at(int r, int b) {
-    return (uint32_t)(r * kRowBytes + (((b ^ r) & 7) << 4) + (b & ~7) * 16);
+struct MoeTile {
+    int g, piece, m0, kb0, kb1, off, n;
+    int64_t row;  // of the weight matrix
+};
+__device__ __forceinline__ MoeTile moe_tile(const Phase &ph, const Lists &L, int t) {
+    MoeTile r;
+    r.g = t / ph.per_group;
+    const int in = t - r.g * ph.per_group;
+    r.piece = in / ph.m_tiles;
+    r.m0 = (in - r.piece * ph.m_tiles) * ph.rows_m;
+    r.kb0 = r.piece * ph.steps / ph.split, r.kb1 = (r.piece + 1) * ph.steps / ph.split;
+    r.off = L.off[r.g];
+    r.n = min(L.off[r.g + 1] - r.off, kGroup);
+    r.row = (int64_t)L.slots[r.g] * ph.slot_rows + r.m0;
+    return r;
 }
 
-__device__ __forceinline__ void issue_chunk(uint32_t slot, const Source &src, int c, int blocks, int lane) {
-    constexpr int kPerPass = 32 / kRowBlocks;  // rows of one instruction
-    const int b = lane % kRowBlocks, r0 = lane / kRowBlocks;
-    const bool valid = c * kRowBlocks + b < blocks;
-    const int64_t row_bytes = blocks * 16;
-    const uint8_t *pa = src.a + r0 * row_bytes + (valid ? c * kRowBytes + b * 16 : 0);
-    const uint8_t *pb = src.b + r0 * row_bytes + (valid ? c * kRowBytes + b * 16 : 0);
-#pragma unroll
-    for (int i = 0; i < 8 / kPerPass; ++i) {
-        cp_async16(slot + piece_at(r0 + i * kPerPass, b), pa + i * kPerPass * row_bytes, valid);
-        cp_async16(slot + piece_at(8 + r0 + i * kPerPass, b), pb + i * kPerPass * row_bytes, valid);
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     s_addr(dst)),
+                 "l"(src), "r"(bytes), "r"(s_addr(bar))
+                 : "memory");
+}
+
+// Ring position that lives on from phase to phase.
+struct Cursor {
+    int k = 0;     // step
+    int tile = 0;  // tile of the phase's MMA and epilogue order (accumulator turn)
+};
+
+__device__ __forceinline__ void load_weights(unsigned char *st, const Phase &ph, const MoeTile &t, int kb, uint64_t *bar) {
+    tma_load_2d(st, ph.map, kb * 128, (int)t.row, bar);
+    tma_load_2d(st + kABytes / 2, ph.map, kb * 128, (int)t.row + ph.second, bar);
+}
+__device__ __forceinline__ void load_terms(unsigned char *st, const Phase &ph, const Lists &L, const MoeTile &t, int kb,
+                                           uint64_t *bar) {
+    for (int i = 0; i < t.n; ++i)
+        bulk_load(st + kABytes + i * kTermBytes,
+                  ph.b_codes + ((size_t)(L.pair[t.off + i] / ph.token_div) * ph.steps + kb) * kTermBytes, kTermBytes, bar);
+}
+
+// Copies of a phase's steps; the weights of the first `early` steps are on
+// their way already.
+__device__ void run_copies(Control &C, unsigned char *stages, const Phase &ph, const Lists &L, Cursor &cur, int early,
+                           int *status) {
+    volatile int *abort = &C.abort;
+    for (int t = blockIdx.x; t < ph.tiles; t += gridDim.x) {
+        const MoeTile tile = moe_tile(ph, L, t);
+        for (int kb = tile.kb0; kb < tile.kb1; ++kb, ++cur.k) {
+            const int s = cur.k % kStages;
+            unsigned char *st = stages + s * kStageBytes;
+            if (early > 0) {
+                --early;
+            } else {
+                if (cur.k >= kStages && !wait_or_abort(&C.empty[s], ((cur.k / kStages) - 1) & 1, abort, status)) return;
+                mbar_expect_tx(&C.full[s], kABytes + tile.n * kTermBytes);
+                load_weights(st, ph, tile, kb, &C.full[s]);
+            }
+            load_terms(st, ph, L, tile, kb, &C.full[s]);
+            C.issued = cur.k + 1;
+        }
     }
-    if (lane < 16) {
-        const uint32_t at = slot + kCodeBytes + lane * kRowBlocks;
-        const uint8_t *s = (lane < 8 ? src.sa : src.sb) + (lane & 7) * blocks + c * kRowBlocks;
-        if (blocks % kRowBlocks == 0) {
-            cp_async_ca<kRowBlocks>(at, s);
-        } else {  // the rows' scale bytes are not aligned, or end within the stage
+}
+// The weights of the phase's first steps, as many as the ring holds; returns
+// how many.
+__device__ int copy_early(Control &C, unsigned char *stages, const Phase &ph, const Lists &L, int k, int *status) {
+    volatile int *abort = &C.abort;
+    int early = 0;
+    for (int t = blockIdx.x; t < ph.tiles; t += gridDim.x) {
+        const MoeTile tile = moe_tile(ph, L, t);
+        for (int kb = tile.kb0; kb < tile.kb1; ++kb, ++k) {
+            if (early == kStages) return early;
+            const int s = k % kStages;
+            if (k >= kStages && !wait_or_abort(&C.empty[s], ((k / kStages) - 1) & 1, abort, status)) return early;
+            mbar_expect_tx(&C.full[s], kABytes + tile.n * kTermBytes);
+            load_weights(stages + s * kStageBytes, ph, tile, kb, &C.full[s]);
+            ++early;
+        }
+    }
+    return early;
+}
+
+// Scale bytes written by this kernel: not through the read-only path.
+__device__ __forceinline__ uint2 load_term_scales(const uint8_t *p, int left) {
+    uint2 v = __ldcg(reinterpret_cast<const uint2 *>(p));
+    if (left < 8) {  // blocks behind the last: whatever lies there is not a scale
+        const uint64_t keep = (1ull << (8 * left)) - 1;
+        v.x &= (uint32_t)keep, v.y &= (uint32_t)(keep >> 32);
+    }
+    return v;
+}
+
+__device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, const Lists &L, Cursor &cur, int *status) {
+    constexpr int kDeep = 4;  // stages whose scale bytes are in registers
+    const int tid = threadIdx.x - kSfWarp * 32;
+    volatile int *abort = &C.abort;
+    int lt = blockIdx.x, lkb = 0, lend = 0, total = 0;
+    const uint8_t *pw = nullptr, *pb = nullptr;
+    auto point = [&] {
+        if (lt >= ph.tiles) return;
+        const MoeTile tile = moe_tile(ph, L, lt);
+        lkb = tile.kb0, lend = tile.kb1;
+        const int64_t row = tile.row + (tid < 64 ? tid : ph.second + tid - 64);
+        pw = row < ph.w_rows ? ph.w_scales + row * ph.blocks : nullptr;
+        const int i = tid / kRows, q = tid % kRows;
+        pb = i < tile.n && q < kTerms
+                 ? ph.b_scales + (size_t)(L.pair[tile.off + i] / ph.token_div) * ph.steps * kScaleBytes + q * kStepBlocks
+                 : nullptr;
+    };
+    auto load = [&](uint2 &x, uint2 &y) {
+        if (lt >= ph.tiles) return;
+        x = pw ? load_scales(pw, lkb, ph.blocks, ph.align) : make_uint2(0, 0);
+        y = pb ? load_term_scales(pb + (size_t)lkb * kScaleBytes, ph.blocks - lkb * kStepBlocks) : make_uint2(0, 0);
+        if (++lkb == lend) {
+            lt += gridDim.x;
+            point();
+        }
+    };
+    for (int t = blockIdx.x; t < ph.tiles; t += gridDim.x) {
+        const int piece = (t % ph.per_group) / ph.m_tiles;
+        total += (piece + 1) * ph.steps / ph.split - piece * ph.steps / ph.split;
+    }
+    point();
+    uint2 vw[kDeep], vb[kDeep];
 #pragma unroll
-            for (int w = 0; w < kRowBlocks / 4; ++w) {
-                uint32_t v = 0;
-                for (int i = 0; i < 4; ++i)
-                    if (c * kRowBlocks + w * 4 + i < blocks) v |= (uint32_t)s[w * 4 + i] << (8 * i);
-                asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + w * 4), "r"(v) : "memory");
+    for (int i = 0; i < kDeep; ++i) load(vw[i], vb[i]);
+    for (int n0 = 0; n0 < total; n0 += kDeep) {
+#pragma unroll
+        for (int i = 0; i < kDeep; ++i) {
+            if (n0 + i >= total) break;
+            const int k = cur.k + n0 + i, s = k % kStages;
+            if (k >= kStages && !wait_or_abort(&C.empty[s], ((k / kStages) - 1) & 1, abort, status)) return;
+            unsigned char *sf = stages + s * kStageBytes + kABytes + kBBytes + atom_at(tid);
+            *reinterpret_cast<uint32_t *>(sf) = vw[i].x;
+            *reinterpret_cast<uint32_t *>(sf + kAtomBytes) = vw[i].y;
+            *reinterpret_cast<uint32_t *>(sf + 2 * kAtomBytes) = vb[i].x;
+            *reinterpret_cast<uint32_t *>(sf + 3 * kAtomBytes) = vb[i].y;
+            fence_async_shared();
+            __syncwarp();
+            if ((tid & 31) == 0) mbar_arrive(&C.sf_full[s]);
+            load(vw[i], vb[i]);
+        }
+    }
+    cur.k += total;
+}
+
+__device__ void run_products(Control &C, unsigned char *stages, const Phase &ph, const Lists &L, Cursor &cur, int *status) {
+    volatile int *abort = &C.abort;
+    for (int t = blockIdx.x; t < ph.tiles; t += gridDim.x, ++cur.tile) {
+        const MoeTile tile = moe_tile(ph, L, t);
+        const int b = cur.tile & 1;
+        if (cur.tile >= 2 && !wait_or_abort(&C.acc_empty[b], ((cur.tile / 2) - 1) & 1, abort, status)) return;
+        tc_fence_after();
+        const uint32_t acc = C.tmem_base + b * kAccCols;
+        const int N = (tile.n * kRows + 15) / 16 * 16;
+        const uint32_t id0 = idesc_mxf4(128, N, 0), id1 = idesc_mxf4(128, N, 2);
+        for (int kb = tile.kb0; kb < tile.kb1; ++kb, ++cur.k) {
+            const int s = cur.k % kStages;
+            if (!wait_or_abort(&C.full[s], (cur.k / kStages) & 1, abort, status) ||
+                !wait_or_abort(&C.sf_full[s], (cur.k / kStages) & 1, abort, status))
+                return;
+            tc_fence_after();
+            const uint32_t a0 = s_addr(stages + s * kStageBytes), b0 = a0 + kABytes, sf = b0 + kBBytes;
+            const uint32_t cols = C.tmem_base + kSfCol0 + s * kSfCols;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) copy_atom(cols + i * 4, sf + i * kAtomBytes);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)  // 64 values = 32 bytes further along K
+                umma_mxf4(acc, smem_desc_k_sw128(a0 + kk * 32), smem_desc_k_sw128(b0 + kk * 32), kk & 1 ? id1 : id0,
+                          cols + (kk >> 1) * 4, cols + 8 + (kk >> 1) * 4, kb != tile.kb0 || kk != 0);
+            umma_commit(&C.empty[s]);
+            C.consumed = cur.k + 1;
+        }
+        umma_commit(&C.acc_full[b]);
+    }
+}
+
+// Four tokens' columns of this thread's row.
+__device__ __forceinline__ void read_rows(uint32_t taddr, float (&v)[4]) {
+    uint32_t r[32];
+    gemm::tmem_ld32(taddr, r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] = 0.f;
+#pragma unroll
+        for (int q = 0; q < kTerms; ++q) v[i] += __uint_as_float(r[i * kRows + q]);
+    }
+}
+__device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+__device__ void run_gate_up(Control &C, const Phase &ph, const Lists &L, Cursor &cur, const MoeArgs &a, float *ex,
+                            int steps_out) {
+    volatile int *abort = &C.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3;
+    for (int t = blockIdx.x; t < ph.tiles; t += gridDim.x, ++cur.tile) {
+        const MoeTile tile = moe_tile(ph, L, t);
+        const int b = cur.tile & 1;
+        const bool ok = wait_or_abort(&C.acc_full[b], (cur.tile / 2) & 1, abort, a.status);
+        if (ok) {
+            tc_fence_after();
+            for (int i = 0; i < tile.n; i += 4) {
+                float v[4];
+                read_rows(C.tmem_base + b * kAccCols + ((uint32_t)(quarter * 32) << 16) + i * kRows, v);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) ex[(i + j) * 128 + quarter * 32 + lane] = v[j];
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&C.acc_empty[b]);
+        }
+        epilogue_barrier();
+        // warp: one block of 32 intermediate values, every other token
+        const int j0 = tile.m0 + (quarter & 1) * 32;
+        if (ok && j0 < a.I)
+            for (int i = quarter >> 1; i < tile.n; i += 2) {
+                const float g = ex[i * 128 + (quarter & 1) * 32 + lane], u = ex[i * 128 + 64 + (quarter & 1) * 32 + lane];
+                const int p = L.pair[tile.off + i], kb = j0 / kStepK, piece = j0 / kBlock % kStepBlocks;
+                write_terms(g / (1.f + __expf(-g)) * u, a.aq + ((size_t)p * steps_out + kb) * kTermBytes,
+                            a.as + ((size_t)p * steps_out + kb) * kScaleBytes + piece, piece, lane);
+            }
+        epilogue_barrier();
+    }
+}
+
+__device__ void run_down(Control &C, const Phase &ph, const Lists &L, Cursor &cur, const MoeArgs &a) {
+    volatile int *abort = &C.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3;
+    for (int t = blockIdx.x; t < ph.tiles; t += gridDim.x, ++cur.tile) {
+        const MoeTile tile = moe_tile(ph, L, t);
+        const int b = cur.tile & 1;
+        if (!wait_or_abort(&C.acc_full[b], (cur.tile / 2) & 1, abort, a.status)) return;
+        tc_fence_after();
+        const int h = tile.m0 + quarter * 32 + lane;
+        for (int i = 0; i < tile.n; i += 4) {
+            float v[4];
+            read_rows(C.tmem_base + b * kAccCols + ((uint32_t)(quarter * 32) << 16) + i * kRows, v);
+            if (h >= a.H) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (i + j >= tile.n) break;
+                const int p = L.pair[tile.off + i + j];
+                a.y[((size_t)tile.piece * a.T * a.k + p) * a.H + h] = v[j] * L.w[p];
             }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&C.acc_empty[b]);
     }
 }
 
-// Byte i of w as an exponent field: 2^(byte - 127), 0 for byte 0 (a block of
-// zeros).  Two instructions; the special values of scale_value() cost as much
-// as the rest of a block's arithmetic (246 cycles a stage against 132), so a
-// NaN (255) is looked for once a word instead (nan_bytes).
-template <int I>
-__device__ __forceinline__ float scale_bits(uint32_t w) {
-    return __uint_as_float((I < 3 ? w << (23 - 8 * I) : w >> 1) & 0x7F800000u);
-}
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return (~w - 0x01010101u) & w & 0x80808080u; }
-
-// acc[nt] += rows of the stage times the columns of token tile nt, 128 columns
-// from 128 h on.  `take(nt, b)`: eight fp16 activations of this lane's token,
-// columns 32 b + 8 (lane % 4) of them on.
-template <int NT, class TakeB>
-__device__ __forceinline__ void chunk_mma(uint32_t slot, int h, int lane, float (&acc)[NT][4], uint32_t (&nan)[2], TakeB take) {
-    const int r = lane >> 2, t = lane & 3;
-    const uint32_t sc = slot + kCodeBytes + r * kRowBlocks + h * 4;
-    const uint32_t sa = lds32(sc), sb = lds32(sc + 8 * kRowBlocks);
-    nan[0] |= nan_bytes(sa), nan[1] |= nan_bytes(sb);
-    uint32_t wa[4], wb[4];
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        const uint32_t at = slot + piece_at(r, h * 4 + b) + t * 4;
-        wa[b] = lds32(at), wb[b] = lds32(at + 8 * kRowBytes);
+// Pieces of the intermediate size in D: the fewest with which the last round
+// of tiles leaves less than a tenth of the SMs' time unused.
+__device__ __forceinline__ int choose_split(int tiles, int steps, int most) {
+    int best = 1, best_use = 0;
+    for (int s = 1; s <= min(most, steps); ++s) {
+        const int n = tiles * s, use = 1000 * n / ((n + (int)gridDim.x - 1) / (int)gridDim.x * (int)gridDim.x);
+        if (use > best_use) best = s, best_use = use;
+        if (use >= 900) break;
     }
-    const float fa[4] = {scale_bits<0>(sa), scale_bits<1>(sa), scale_bits<2>(sa), scale_bits<3>(sa)};
-    const float fb[4] = {scale_bits<0>(sb), scale_bits<1>(sb), scale_bits<2>(sb), scale_bits<3>(sb)};
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        uint32_t ha[4], hb[4];
-        e2m1x8_to_f16(wa[b], ha);
-        e2m1x8_to_f16(wb[b], hb);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const uint4 x = take(nt, b);
-            const float zero[4] = {};
-            float d[4];
-            mma_f16(d, ha[0], hb[0], ha[1], hb[1], x.x, x.y, zero);
-            mma_f16(d, ha[2], hb[2], ha[3], hb[3], x.z, x.w, d);
-            acc[nt][0] = fmaf(fa[b], d[0], acc[nt][0]), acc[nt][1] = fmaf(fa[b], d[1], acc[nt][1]);
-            acc[nt][2] = fmaf(fb[b], d[2], acc[nt][2]), acc[nt][3] = fmaf(fb[b], d[3], acc[nt][3]);
-        }
-    }
-}
-// Rows that met a NaN scale.
-template <int NT>
-__device__ __forceinline__ void mark_nan(float (&acc)[NT][4], const uint32_t (&nan)[2]) {
-    if (!(nan[0] | nan[1])) return;
-    // a row's four lanes read the same scale bytes
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (nan[i >> 1]) acc[nt][i] = NAN;
+    return best;
 }
 
-// Eight fp16 activations of the c-th 128 columns, or zeros behind the last column.
-__device__ __forceinline__ uint4 load_b(const __half *row, int c, int b, int blocks) {
-    return c * 4 + b < blocks ? *reinterpret_cast<const uint4 *>(row + c * kSub + b * 32)
-                              : make_uint4(0, 0, 0, 0);
-}
-
-// Ring of a warp: stage i of the stream lies in slot i % kStages.
-struct Ring {
-    uint32_t base;
-    int issued, taken;
-    __device__ __forceinline__ uint32_t slot(int i) const { return base + (uint32_t)(i % kStages) * kStageBytes; }
-};
-
-__global__ void __launch_bounds__(kThreads, 1) moe_kernel(const MoeArgs a) {
-    extern __shared__ __align__(16) unsigned char smem[];
-    Lists &L = *reinterpret_cast<Lists *>(smem);
-    unsigned char *rings = smem + (sizeof(Lists) + 15) / 16 * 16;
-    float *sums = reinterpret_cast<float *>(rings + kWarps * kStages * kStageBytes);  // [kWarps][T][16]
+__global__ void __launch_bounds__(kThreads, 1)
+    moe_kernel(const __grid_constant__ CUtensorMap map13, const __grid_constant__ CUtensorMap map2, const MoeArgs a) {
+    extern __shared__ unsigned char raw[];
+    unsigned char *stages = raw + ((1024u - (s_addr(raw) & 1023u)) & 1023u);
+    float *ex = reinterpret_cast<float *>(stages + kStages * kStageBytes);  // [kGroup][128]
+    Control &C = *reinterpret_cast<Control *>(ex + kGroup * 128);
+    Lists &L = *reinterpret_cast<Lists *>(&C + 1);
+    Scratch &S = *reinterpret_cast<Scratch *>(stages);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int nw = gridDim.x * kWarps, gw = blockIdx.x * kWarps + warp;
-    const int P = a.T * a.k;
+    const int nw = gridDim.x * kWarps;
 
-    // R
-    for (int i = blockIdx.x * kThreads + tid; i < P; i += gridDim.x * kThreads) a.act_max[i] = 0;
-    for (int t = nw - 1 - gw; t < a.T; t += nw) convert_token(a, t, lane);
+    if (tid == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&C.full[s], 1);
+            mbar_init(&C.sf_full[s], 4);
+            mbar_init(&C.empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&C.acc_full[b], 1);
+            mbar_init(&C.acc_empty[b], 4);
+        }
+        mbar_init(&C.mma_done, 1);
+        C.abort = C.issued = C.consumed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) gemm::tmem_alloc(&C.tmem_base, kTmemCols);
+    tc_fence_before();
+
+    // R: warps in turn over the SMs, so that few units spread
+    const int gw = warp * gridDim.x + blockIdx.x;
     if (a.router) {
         if (a.E * a.T <= nw)  // a warp for each product
             route_products<1>(a, gw, nw, lane);
         else
             route_products<4>(a, gw, nw, lane);
     }
-    for (int e = tid; e < a.E; e += kThreads) L.count[e] = 0;
+    convert_tokens(a, nw - 1 - gw, nw, lane);
+    for (int e = tid; e < a.E; e += kThreads) S.count[e] = 0;
+    asm volatile("fence.proxy.async;" ::: "memory");  // the terms are read by bulk copies
     cg::this_grid().sync();
+    tc_fence_after();
 
     // S
     if (a.router) {
         for (int t = warp; t < a.T; t += kWarps) {
             if (a.E <= 128)
-                route_token<4>(a, L, t, lane);
+                route_token<4>(a, L, S, t, lane);
             else if (a.E <= 256)
-                route_token<8>(a, L, t, lane);
+                route_token<8>(a, L, S, t, lane);
             else
-                route_token<32>(a, L, t, lane);
+                route_token<32>(a, L, S, t, lane);
         }
     } else if (tid < a.T) {
-        given_token(a, L, tid);
+        given_token(a, L, S, tid);
     }
     __syncthreads();
-    build_lists(a, L);
-    const int U = L.n;
+    build_lists(a, L, S);
+    // the ring's memory was written as plain memory, the copies come next
+    asm volatile("fence.proxy.async;" ::: "memory");
+    __syncthreads();
 
-    Ring ring{(uint32_t)__cvta_generic_to_shared(rings) + warp * kStages * kStageBytes, 0, 0};
-    const int r = lane >> 2, tcol = lane & 3;
+    Phase up{}, down{};
+    up.map = &map13, up.w_scales = a.s13, up.b_codes = a.xq, up.b_scales = a.xs;
+    up.blocks = a.H / kBlock, up.steps = (up.blocks + kStepBlocks - 1) / kStepBlocks, up.align = a.s13_align;
+    up.m_tiles = up.per_group = (a.I + 63) / 64, up.tiles = L.n * up.per_group, up.split = 1, up.rows_m = 64;
+    up.slot_rows = 2 * a.I, up.second = a.I, up.w_rows = (int64_t)a.slots * 2 * a.I, up.token_div = a.k;
+    down.map = &map2, down.w_scales = a.s2, down.b_codes = a.aq, down.b_scales = a.as;
+    down.blocks = a.I / kBlock, down.steps = (down.blocks + kStepBlocks - 1) / kStepBlocks, down.align = a.s2_align;
+    down.m_tiles = (a.H + 127) / 128, down.split = choose_split(L.n * down.m_tiles, down.steps, a.max_split);
+    down.per_group = down.m_tiles * down.split, down.tiles = L.n * down.per_group, down.rows_m = 128;
+    down.slot_rows = a.H, down.second = 64, down.w_rows = (int64_t)a.slots * a.H, down.token_div = 1;
 
-    // G: unit u = (expert u / JT, intermediate values 8 (u % JT) ..)
-    {
-        const int JT = a.I / 8, chunks = (a.H + kChunk - 1) / kChunk, blocks = a.H / kBlock;
-        const int64_t N = (int64_t)U * JT;
-        const int lo = (int)(N * blockIdx.x / gridDim.x), hi = (int)(N * (blockIdx.x + 1) / gridDim.x);
-        const int64_t row_bytes = a.H / 2;
-        int pu = lo + warp, pc = 0;  // next chunk to issue
-        Source src{};
-        auto issue = [&] {
-            if (pu < hi) {
-                if (pc == 0) {
-                    const int ue = pu / JT, j = (pu - ue * JT) * 8;
-                    const int64_t base = (int64_t)L.uslot[ue] * 2 * a.I;
-                    src.a = a.w13 + (base + j) * row_bytes;
-                    src.b = src.a + a.I * row_bytes;
-                    src.sa = a.s13 + (base + j) * blocks;
-                    src.sb = src.sa + (int64_t)a.I * blocks;
-                }
-                issue_chunk(ring.slot(ring.issued), src, pc, blocks, lane);
-                if (++pc == chunks) pc = 0, pu += kWarps;
-            }
-            ++ring.issued;
-            cp_async_commit();
-        };
-        for (int i = 0; i < kStages - 1; ++i) issue();
-        // the first token tile's activations are loaded a stage ahead, across units
-        auto token_row = [&](int ue, int nt) {
-            const int off = L.uoff[ue], n = L.uoff[ue + 1] - off;
-            return (uint32_t)(L.pair[off + min(nt * 8 + r, n - 1)] / a.k) * a.H + tcol * 8;
-        };
-        uint4 ahead[4];
-        if (lo + warp < hi) {
-            const uint32_t row = token_row((lo + warp) / JT, 0);
-#pragma unroll
-            for (int b = 0; b < 4; ++b) ahead[b] = load_b(a.xs + row, 0, b, blocks);
+    // G
+    Cursor cur;
+    int early = 0;
+    if (warp == 0) {
+        if (lane == 0) {
+            run_copies(C, stages, up, L, cur, 0, a.status);
+            early = copy_early(C, stages, down, L, cur.k, a.status);
         }
-        auto unit = [&](auto tiles, int ue, int j0, int next_ue) {
-            constexpr int NT = decltype(tiles)::value;
-            const int off = L.uoff[ue], n = L.uoff[ue + 1] - off;
-            float acc[NT][4] = {};
-            uint32_t nan[2] = {};
-            uint32_t xrow[NT];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) xrow[nt] = token_row(ue, nt);
-            const uint32_t next_row = token_row(next_ue, 0);
-            for (int c = 0; c < chunks; ++c) {
-                cp_async_wait<kStages - 2>();
-                __syncwarp();
-                issue();
-                const uint32_t slot = ring.slot(ring.taken++);
-#pragma unroll 1
-                for (int h = 0; h < kChunk / kSub; ++h) {
-                    const int k = c * (kChunk / kSub) + h;
-                    const bool last = (k + 1) * 4 >= blocks;
-                    const uint32_t ahead_row = last ? next_row : xrow[0];
-                    const int ahead_k = last ? 0 : k + 1;
-                    chunk_mma<NT>(slot, h, lane, acc, nan, [&](int nt, int b) {
-                        if (nt) return load_b(a.xs + xrow[nt], k, b, blocks);
-                        const uint4 v = ahead[b];
-                        ahead[b] = load_b(a.xs + ahead_row, ahead_k, b, blocks);
-                        return v;
-                    });
-                    if (last) break;
-                }
-            }
-            mark_nan<NT>(acc, nan);
-            const int j = j0 + r;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int q = nt * 8 + tcol * 2 + i;
-                    const int p = L.pair[off + min(q, n - 1)];
-                    const float xs = a.x_scale[p / a.k];
-                    const float g = acc[nt][i] * xs, u = acc[nt][2 + i] * xs;
-                    const float v = g / (1.f + __expf(-g)) * u;
-                    // the 8 lanes that share lane % 4 hold 8 intermediate values of the pair
-                    uint32_t m = __float_as_uint(v) & 0x7FFFFFFFu;
-                    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 4));
-                    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 8));
-                    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));
-                    if (q >= n) continue;
-                    float to_half, back;
-                    half_scale(m >> 23, to_half, back);
-                    a.act[(size_t)p * a.I + j] = __float2half_rn(v * to_half);
-                    if (r == 0) {
-                        const int e = half_exponent(m >> 23);
-                        a.act_exp[(size_t)p * a.exp_stride + exp_at(j0 >> 3)] = (uint8_t)e;
-                        atomicMax(a.act_max + p, (uint32_t)e);
-                    }
-                }
-        };
-        for (int u = lo + warp; u < hi; u += kWarps) {
-            const int ue = u / JT, j0 = (u - ue * JT) * 8, n = L.uoff[ue + 1] - L.uoff[ue];
-            const int next = u + kWarps < hi ? (u + kWarps) / JT : ue;
-            if (n <= 8)
-                unit(std::integral_constant<int, 1>(), ue, j0, next);
-            else if (n <= 16)
-                unit(std::integral_constant<int, 2>(), ue, j0, next);
-            else if (n <= 32)
-                unit(std::integral_constant<int, 4>(), ue, j0, next);
-            else
-                unit(std::integral_constant<int, 8>(), ue, j0, next);
-        }
-        cp_async_wait<0>();
-        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) run_products(C, stages, up, L, cur, a.status);
+    } else if (warp < kSfWarp) {
+        run_gate_up(C, up, L, cur, a, ex, down.steps);
+    } else {
+        run_scales(C, stages, up, L, cur, a.status);
     }
+    __syncwarp();
+    asm volatile("fence.proxy.async;" ::: "memory");  // the terms are read by bulk copies
+    cg::this_grid().sync();
+    asm volatile("fence.proxy.async;" ::: "memory");
 
-    // D: tile = 16 rows of the hidden size; unit v = (expert v / segs, piece v % segs of I)
-    {
-        const int tiles = a.H / 16, chunks = (a.I + kChunk - 1) / kChunk, blocks = a.I / kBlock;
-        // at least four units a warp, where I has the chunks for it
-        const int segs = U ? max(1, min(chunks, (2 * kWarps + U - 1) / U)) : 1;
-        const int V = U * segs;
-        const int64_t row_bytes = a.I / 2;
-        float *mine = sums + warp * a.T * 16;
-        for (int i = lane; i < a.T * 16; i += 32) mine[i] = 0.f;
-        ring.issued = ring.taken = 0;
-        int ptile = blockIdx.x, pv = warp, pc = 0, pend = 0;
-        if (pv >= V) ptile = tiles;
-        Source src{};
-        bool fresh = true;
-        auto issue = [&] {
-            if (ptile < tiles) {
-                if (fresh) {
-                    const int ue = pv / segs, seg = pv - ue * segs;
-                    pc = seg * chunks / segs, pend = (seg + 1) * chunks / segs;
-                    const int64_t row = (int64_t)L.uslot[ue] * a.H + ptile * 16;
-                    src.a = a.w2 + row * row_bytes;
-                    src.b = src.a + 8 * row_bytes;
-                    src.sa = a.s2 + row * blocks;
-                    src.sb = src.sa + 8 * blocks;
-                    fresh = false;
-                }
-                issue_chunk(ring.slot(ring.issued), src, pc, blocks, lane);
-                if (++pc == pend) {
-                    fresh = true;
-                    pv += kWarps;
-                    if (pv >= V) pv = warp, ptile += gridDim.x;
-                }
-            }
-            ++ring.issued;
-            cp_async_commit();
-        };
-        for (int i = 0; i < kStages - 1; ++i) issue();
-        cg::this_grid().sync();
-        // the first token tile's activations are loaded a stage ahead, across units
-        auto pair_of = [&](int ue, int nt) {
-            const int off = L.uoff[ue], n = L.uoff[ue + 1] - off;
-            return (int)L.pair[off + min(nt * 8 + r, n - 1)];
-        };
-        auto load_exp = [&](int p, int c) {
-            return *reinterpret_cast<const uint32_t *>(a.act_exp + (size_t)p * a.exp_stride + c * 16 + tcol * 4);
-        };
-        // to the pair's common scale: groups 2^24 below the largest vanish
-        auto common = [&](uint4 v, uint32_t exps, int b, int top) {
-            const float f = __uint_as_float((uint32_t)max(127 - max(top - (int)((exps >> (8 * b)) & 255), 0), 0) << 23);
-            const __half2 s = __floats2half2_rn(f, f);
-            __half2 h[4];
-            memcpy(h, &v, 16);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) h[i] = __hmul2(h[i], s);
-            memcpy(&v, h, 16);
-            return v;
-        };
-        uint4 ahead[4];
-        uint32_t ahead_exp = 0;
-        if (V > warp && blockIdx.x < tiles) {
-            const int ue = warp / segs, p = pair_of(ue, 0);
-            const int c = (warp - ue * segs) * chunks / segs * (kChunk / kSub);
-            ahead_exp = load_exp(p, c);
-#pragma unroll
-            for (int b = 0; b < 4; ++b) ahead[b] = load_b(a.act + (uint32_t)p * a.I + tcol * 8, c, b, blocks);
+    // D
+    if (warp == 0) {
+        if (lane == 0) run_copies(C, stages, down, L, cur, early, a.status);
+    } else if (warp == 1) {
+        if (lane == 0) {
+            run_products(C, stages, down, L, cur, a.status);
+            umma_commit(&C.mma_done);
         }
-        auto unit = [&](auto tiles_, int ue, int seg, int next_ue, int next_c) {
-            constexpr int NT = decltype(tiles_)::value;
-            const int off = L.uoff[ue], n = L.uoff[ue + 1] - off;
-            float acc[NT][4] = {};
-            uint32_t nan[2] = {};
-            int pr[NT], top[NT];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                pr[nt] = pair_of(ue, nt);
-                top[nt] = (int)a.act_max[pr[nt]];
-            }
-            const int next_p = pair_of(next_ue, 0);
-            const int end = (seg + 1) * chunks / segs;
-            for (int c = seg * chunks / segs; c < end; ++c) {
-                cp_async_wait<kStages - 2>();
-                __syncwarp();
-                issue();
-                const uint32_t slot = ring.slot(ring.taken++);
-#pragma unroll 1
-                for (int h = 0; h < kChunk / kSub; ++h) {
-                    const int k = c * (kChunk / kSub) + h;
-                    const bool done = (k + 1) * 4 >= blocks, last = done || (h + 1 == kChunk / kSub && c + 1 == end);
-                    const int ahead_p = last ? next_p : pr[0], ahead_k = last ? next_c * (kChunk / kSub) : k + 1;
-                    uint32_t exps[NT];
-                    exps[0] = ahead_exp;
-                    ahead_exp = load_exp(ahead_p, ahead_k);
-#pragma unroll
-                    for (int nt = 1; nt < NT; ++nt) exps[nt] = load_exp(pr[nt], k);
-                    chunk_mma<NT>(slot, h, lane, acc, nan, [&](int nt, int b) {
-                        if (nt)
-                            return common(load_b(a.act + (uint32_t)pr[nt] * a.I + tcol * 8, k, b, blocks), exps[nt], b,
-                                          top[nt]);
-                        const uint4 v = common(ahead[b], exps[0], b, top[0]);
-                        ahead[b] = load_b(a.act + (uint32_t)ahead_p * a.I + tcol * 8, ahead_k, b, blocks);
-                        return v;
-                    });
-                    if (done) break;
-                }
-            }
-            mark_nan<NT>(acc, nan);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int q = nt * 8 + tcol * 2 + i;
-                    if (q >= n) continue;
-                    const int p = L.pair[off + q];
-                    const float back = half_back((int)a.act_max[p]) * L.w[p];
-                    float *at = mine + (p / a.k) * 16 + r;
-                    at[0] = fmaf(acc[nt][i], back, at[0]);
-                    at[8] = fmaf(acc[nt][2 + i], back, at[8]);
-                }
-            __syncwarp();
-        };
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-            for (int v = warp; v < V; v += kWarps) {
-                const int ue = v / segs, seg = v - ue * segs, n = L.uoff[ue + 1] - L.uoff[ue];
-                const int nv = v + kWarps < V ? v + kWarps : warp;  // the next tile's units are the same
-                const int next = nv / segs, next_c = (nv - next * segs) * chunks / segs;
-                if (n <= 8)
-                    unit(std::integral_constant<int, 1>(), ue, seg, next, next_c);
-                else if (n <= 16)
-                    unit(std::integral_constant<int, 2>(), ue, seg, next, next_c);
-                else if (n <= 32)
-                    unit(std::integral_constant<int, 4>(), ue, seg, next, next_c);
-                else
-                    unit(std::integral_constant<int, 8>(), ue, seg, next, next_c);
-            }
-            __syncthreads();
-            for (int i = tid; i < a.T * 16; i += kThreads) {
-                float s = 0.f;
-                for (int w = 0; w < kWarps; ++w) {
-                    s += sums[w * a.T * 16 + i];
-                    sums[w * a.T * 16 + i] = 0.f;
-                }
-                a.out[(size_t)(i >> 4) * a.H + tile * 16 + (i & 15)] = __float2bfloat16_rn(s);
-            }
-            __syncthreads();
-        }
-        cp_async_wait<0>();
+    } else if (warp < kSfWarp) {
+        run_down(C, down, L, cur, a);
+    } else {
+        run_scales(C, stages, down, L, cur, a.status);
     }
+    __syncwarp();
+    tc_fence_before();
+    cg::this_grid().sync();
+
+    // C
+    const int P = a.T * a.k;
+    for (int i = blockIdx.x * kThreads + tid; i < a.T * (a.H / 4); i += gridDim.x * kThreads) {
+        const int t = i / (a.H / 4), h = (i - t * (a.H / 4)) * 4;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j = 0; j < a.k; ++j) {
+            const int p = t * a.k + j;
+            if (!L.has[p]) continue;
+            for (int s = 0; s < down.split; ++s) {
+                const float4 v = __ldcg(reinterpret_cast<const float4 *>(a.y + ((size_t)s * P + p) * a.H + h));
+                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+            }
+        }
+        __nv_bfloat162 o[2] = {__floats2bfloat162_rn(sum.x, sum.y), __floats2bfloat162_rn(sum.z, sum.w)};
+        memcpy(a.out + (size_t)t * a.H + h, o, 8);
+    }
+    if (tid == 0) {
+        // after an abort: copies and products in flight end before the memory is given back
+        volatile int no_abort = 0;
+        for (int k = C.consumed; k < C.issued; ++k)
+            gemm::mbar_wait(&C.full[k % kStages], (k / kStages) & 1, kWaitNs, &no_abort);
+        gemm::mbar_wait(&C.mma_done, 0, kWaitNs, &no_abort);
+    }
+    __syncthreads();
+    if (warp == 0) gemm::tmem_dealloc(C.tmem_base, kTmemCols);
 }
 
-size_t align16(size_t v) { return (v + 15) / 16 * 16; }
-constexpr int exp_stride(int I) { return (I + kSub - 1) / kSub * 16; }
 struct Workspace {
-    size_t logits, xs, x_scale, act, act_exp, act_max, bytes;
+    size_t logits, xq, xs, aq, as, y, bytes;
+    int split;  // pieces of D that y has room for
     Workspace(int T, int E, int k, int H, int I) {
         size_t at = 0;
         const auto take = [&](size_t n) { const size_t here = at; at += (n + 255) / 256 * 256; return here; };
+        const size_t up = (H + kStepK - 1) / kStepK, down = (I + kStepK - 1) / kStepK, P = (size_t)T * k;
         logits = take((size_t)T * E * 4);
-        xs = take((size_t)T * H * 2);
-        x_scale = take((size_t)T * 4);
-        act = take((size_t)T * k * I * 2);
-        act_exp = take((size_t)T * k * exp_stride(I));
-        act_max = take((size_t)T * k * 4);
+        xq = take(T * up * kTermBytes);
+        xs = take(T * up * kScaleBytes);
+        aq = take(P * down * kTermBytes);
+        as = take(P * down * kScaleBytes);
+        split = (int)(down < kMaxSplit ? down : kMaxSplit);
+        y = take((size_t)split * P * H * 4);
         bytes = at;
     }
 };
-size_t smem_bytes(int T) {
-    return align16(sizeof(Lists)) + (size_t)kWarps * kStages * kStageBytes + (size_t)kWarps * T * 16 * sizeof(float);
-}
+constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kGroup * 128 * 4 + sizeof(Control) + sizeof(Lists);
+static_assert(kSmemBytes <= 232448, "shared memory");
+static_assert(sizeof(Scratch) <= kStages * kStageBytes, "the lists' scratch lies in the ring");
 
 int check_shape(int32_t T, int32_t E, int32_t k, int32_t H, int32_t I, int32_t slots) {
     if (T < 0 || T > kMaxTokens || E < 1 || E > kMaxExperts || k < 1 || k > kMaxTopK || k > E || slots < 1)
@@ -758,6 +760,8 @@ int check_shape(int32_t T, int32_t E, int32_t k, int32_t H, int32_t I, int32_t s
     if (H < 32 || H % 32 || H > 32768 || I < 32 || I % 32 || I > 65536)
         return set_error("wisp_mx4_moe: hidden and intermediate sizes are multiples of 32, at most 32768 and 65536"),
                WISP_ERR_INVALID;
+    if ((int64_t)slots * 2 * I > INT32_MAX || (int64_t)slots * H > INT32_MAX)
+        return set_error("wisp_mx4_moe: too many weight rows"), WISP_ERR_INVALID;
     return WISP_OK;
 }
 
@@ -790,13 +794,10 @@ extern "C" int wisp_mx4_moe(const void *x, int64_t x_stride, const void *router,
         return set_error("wisp_mx4_moe: give either the router's weights or ids and weights"), WISP_ERR_INVALID;
     if (!expert_map && num_slots < num_experts)
         return set_error("wisp_mx4_moe: fewer slots than experts, and no expert map"), WISP_ERR_INVALID;
-    for (const void *p : {x, router, w13_codes, w2_codes, (const void *)workspace})
+    for (const void *p : {x, router, w13_codes, w2_codes, (const void *)workspace, (const void *)out})
         if (reinterpret_cast<uintptr_t>(p) % 16)
-            return set_error("wisp_mx4_moe: x, router, codes and workspace must be aligned to 16 bytes"),
+            return set_error("wisp_mx4_moe: x, router, codes, workspace and out must be aligned to 16 bytes"),
                    WISP_ERR_INVALID;
-    for (const void *p : {w13_scales, w2_scales})
-        if (reinterpret_cast<uintptr_t>(p) % 4)
-            return set_error("wisp_mx4_moe: scales must be aligned to 4 bytes"), WISP_ERR_INVALID;
     if (num_tokens > 1 && (x_stride < hidden || x_stride % 8))
         return set_error("wisp_mx4_moe: rows of x must not overlap and must start on 16-byte boundaries"),
                WISP_ERR_INVALID;
@@ -811,28 +812,26 @@ extern "C" int wisp_mx4_moe(const void *x, int64_t x_stride, const void *router,
     a.ids = topk_ids;
     a.weights = topk_weights;
     a.expert_map = expert_map;
-    a.w13 = reinterpret_cast<const uint8_t *>(w13_codes);
     a.s13 = reinterpret_cast<const uint8_t *>(w13_scales);
-    a.w2 = reinterpret_cast<const uint8_t *>(w2_codes);
     a.s2 = reinterpret_cast<const uint8_t *>(w2_scales);
+    a.s13_align = scale_align(w13_scales, hidden / kBlock), a.s2_align = scale_align(w2_scales, inter / kBlock);
     a.out = reinterpret_cast<__nv_bfloat16 *>(out);
     a.logits = reinterpret_cast<float *>(ws + w.logits);
-    a.xs = reinterpret_cast<__half *>(ws + w.xs);
-    a.x_scale = reinterpret_cast<float *>(ws + w.x_scale);
-    a.act = reinterpret_cast<__half *>(ws + w.act);
-    a.act_exp = ws + w.act_exp;
-    a.exp_stride = exp_stride(inter);
-    a.act_max = reinterpret_cast<uint32_t *>(ws + w.act_max);
+    a.xq = ws + w.xq, a.xs = ws + w.xs, a.aq = ws + w.aq, a.as = ws + w.as;
+    a.y = reinterpret_cast<float *>(ws + w.y);
+    a.max_split = w.split;
+    if (const int rc = status_word(&a.status)) return rc;
+    CUtensorMap m13, m2;
+    if (const int rc = gemm::make_byte_map(&m13, w13_codes, (uint64_t)num_slots * 2 * inter, hidden / 2, 64)) return rc;
+    if (const int rc = gemm::make_byte_map(&m2, w2_codes, (uint64_t)num_slots * hidden, inter / 2, 64)) return rc;
     a.T = num_tokens, a.E = num_experts, a.k = top_k, a.H = hidden, a.I = inter, a.slots = num_slots;
     a.ids64 = ids_int64, a.renormalize = renormalize;
     int dev = 0, sms = 0;
     WISP_CUDA_TRY(cudaGetDevice(&dev));
     WISP_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    const size_t smem = smem_bytes(num_tokens);
-    WISP_CUDA_TRY(cudaFuncSetAttribute(moe_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)smem_bytes(kMaxTokens)));
-    void *params[] = {&a};
+    WISP_CUDA_TRY(cudaFuncSetAttribute(moe_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+    void *params[] = {&m13, &m2, &a};
     WISP_CUDA_TRY(cudaLaunchCooperativeKernel(reinterpret_cast<const void *>(moe_kernel), dim3(sms), dim3(kThreads),
-                                              params, smem, reinterpret_cast<cudaStream_t>(stream)));
+                                              params, kSmemBytes, reinterpret_cast<cudaStream_t>(stream)));
     return WISP_OK;
 }

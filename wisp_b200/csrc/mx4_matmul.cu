@@ -62,10 +62,6 @@ struct Control {
     int first[kMaxGroups + 1];  // first row tile of each group
 };
 
-struct Tile {
-    int row0, rows, n0, wrow0;  // first row, rows of the group from there on, first column, its row of W
-};
-
 // Rows [begin, end) of group g; offsets that are not in order, or outside the
 // matrix, make an empty or a shorter group.
 __device__ __forceinline__ void group_rows(const MatmulArgs &a, int g, int &begin, int &end) {
@@ -74,29 +70,39 @@ __device__ __forceinline__ void group_rows(const MatmulArgs &a, int g, int &begi
     end = a.offsets ? min(max(__ldg(a.offsets + g + 1), begin), rows) : rows;
 }
 
-__device__ __forceinline__ Tile tile_of(const Control &C, const MatmulArgs &a, int t, int ntiles_n) {
-    // the last group whose first tile is not behind this one
-    const int mt = t / ntiles_n;  // tiles of a group are consecutive: groups * column tiles keep the order
-    int lo = 0, hi = a.groups - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (C.first[mid] <= mt)
-            lo = mid;
-        else
-            hi = mid - 1;
+// A CTA's walk over the tiles of all groups, gridDim.x apart; row tiles fastest
+// within a group.  For a converged warp: 32 groups are looked at together.
+struct Walk {
+    int t, tiles, ntiles_n, g = 0;
+    // the tile: first row, rows of the group from there on, first column, its row of W
+    int row0, rows, n0, wrow0;
+    __device__ __forceinline__ Walk(const Control &C, const MatmulArgs &a) {
+        ntiles_n = (a.N + kTileN - 1) / kTileN;
+        tiles = C.first[a.groups] * ntiles_n;
+        t = blockIdx.x;
     }
-    const int mtiles = C.first[lo + 1] - C.first[lo];
-    const int in = t - C.first[lo] * ntiles_n;
-    const int n = in / mtiles, m = in - n * mtiles;
-    Tile r;
-    int begin, end;
-    group_rows(a, lo, begin, end);
-    r.row0 = begin + m * kTileM;
-    r.rows = end - r.row0;
-    r.n0 = n * kTileN;
-    r.wrow0 = lo * a.N + r.n0;
-    return r;
-}
+    // False behind the last tile.
+    __device__ __forceinline__ bool at(const Control &C, const MatmulArgs &a) {
+        if (t >= tiles) return false;
+        const int lane = threadIdx.x & 31;
+        while (true) {  // groups that end before this tile
+            const int i = g + 1 + lane;
+            const unsigned behind = __ballot_sync(0xFFFFFFFFu, i <= a.groups && C.first[min(i, a.groups)] * ntiles_n <= t);
+            g += __popc(behind);
+            if (behind != 0xFFFFFFFFu) break;
+        }
+        const int mtiles = C.first[g + 1] - C.first[g], in = t - C.first[g] * ntiles_n;
+        const int n = in / mtiles;
+        int begin, end;
+        group_rows(a, g, begin, end);
+        row0 = begin + (in - n * mtiles) * kTileM;
+        rows = end - row0;
+        n0 = n * kTileN;
+        wrow0 = g * a.N + n0;
+        return true;
+    }
+    __device__ __forceinline__ void next() { t += gridDim.x; }
+};
 
 // Row tiles of every group.
 __device__ void scan_groups(Control &C, const MatmulArgs &a) {
@@ -134,140 +140,151 @@ __device__ void scan_groups(Control &C, const MatmulArgs &a) {
 }
 
 __device__ void load_operands(Control &C, unsigned char *stages, const CUtensorMap *map_a, const CUtensorMap *map_w,
-                              const MatmulArgs &a, int tiles, int ntiles_n, int steps) {
+                              const MatmulArgs &a, int steps) {
     volatile int *abort = &C.abort;
-    int k = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-        const Tile tile = tile_of(C, a, t, ntiles_n);
-        for (int kb = 0; kb < steps; ++kb, ++k) {
-            const int s = k % kStages;
-            if (k >= kStages && !wait_or_abort(&C.empty[s], ((k / kStages) - 1) & 1, abort, a.status)) return;
-            unsigned char *st = stages + s * kStageBytes;
-            mbar_expect_tx(&C.full[s], kABytes + kBBytes);
-            tma_load_2d(st, map_a, kb * 128, tile.row0, &C.full[s]);
-            tma_load_2d(st + kABytes, map_w, kb * 128, tile.wrow0, &C.full[s]);
-            C.issued = k + 1;
+    RingPos<kStages> ring;
+    int issued = 0;
+    for (Walk t(C, a); t.at(C, a); t.next())
+        for (int kb = 0; kb < steps; ++kb, ring.next()) {
+            if (!warp_wait(&C.empty[ring.slot], ring.turn ^ 1, abort, a.status)) return;
+            if (elect_one()) {
+                unsigned char *st = stages + ring.slot * kStageBytes;
+                mbar_expect_tx(&C.full[ring.slot], kABytes + kBBytes);
+                tma_load_2d(st, map_a, kb * 128, t.row0, &C.full[ring.slot]);
+                tma_load_2d(st + kABytes, map_w, kb * 128, t.wrow0, &C.full[ring.slot]);
+                C.issued = ++issued;
+            }
         }
-    }
 }
 
-__device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulArgs &a, int tiles, int ntiles_n,
-                                int steps) {
+__device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulArgs &a, int steps) {
     constexpr int kDeep = 4;  // stages whose scale bytes are in registers
     const int tid = threadIdx.x - kSfWarp * 32;
     volatile int *abort = &C.abort;
     const int64_t wrows = (int64_t)a.groups * a.N;
-    // the load side runs kDeep steps ahead
-    int lt = blockIdx.x, lkb = 0;
-    const uint8_t *pa = nullptr, *pw[2] = {};
+    unsigned char *sf = stages + kABytes + kBBytes + atom_at(tid);
+    RingPos<kStages> ring;
+    // the loads run kDeep steps ahead of the stores
+    Walk ahead(C, a);
+    bool more = ahead.at(C, a);
+    int kb = 0;
+    const uint8_t *pa = nullptr, *pw[2] = {};  // of step kb
     auto point = [&] {
-        if (lt >= tiles) return;
-        const Tile tile = tile_of(C, a, lt, ntiles_n);
-        const int64_t ra = tile.row0 + tid;
+        kb = 0;
+        const int64_t ra = ahead.row0 + tid;
         pa = ra < a.rows ? a.a_scales + ra * a.blocks : nullptr;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int64_t rw = (int64_t)tile.wrow0 + tid + i * 128;
+            const int64_t rw = (int64_t)ahead.wrow0 + tid + i * 128;
             pw[i] = tid + i * 128 < kTileN && rw < wrows ? a.w_scales + rw * a.blocks : nullptr;
         }
     };
-    const uint2 none = make_uint2(0, 0);
-    uint2 va[kDeep], vw[kDeep][2];
-    auto load = [&](uint2 &x, uint2 (&y)[2]) {
-        if (lt >= tiles) return;
-        x = pa ? load_scales(pa, lkb, a.blocks, a.a_align) : none;
+    // nothing here may wait for what it loads: the values are used kDeep steps later
+    auto load = [&](uint2 &x, uint2 (&y)[2], bool &valid) {
+        valid = more;
+        if (!more) return;
+        const int left = a.blocks - kb * kStepBlocks;
+        x = y[0] = y[1] = make_uint2(0, 0);
+        if (pa) {
+            x = load_scales(pa, left, a.a_align);
+            pa += kStepBlocks;
+        }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) y[i] = pw[i] ? load_scales(pw[i], lkb, a.blocks, a.w_align) : none;
-        if (++lkb == steps) {
-            lkb = 0;
-            lt += gridDim.x;
-            point();
+        for (int i = 0; i < 2; ++i)
+            if (pw[i]) {
+                y[i] = load_scales(pw[i], left, a.w_align);
+                pw[i] += kStepBlocks;
+            }
+        if (++kb == steps) {
+            ahead.next();
+            more = ahead.at(C, a);
+            if (more) point();
         }
     };
-    point();
+    if (more) point();
+    uint2 va[kDeep], vw[kDeep][2];
+    bool valid[kDeep];
 #pragma unroll
-    for (int i = 0; i < kDeep; ++i) load(va[i], vw[i]);
-    const int mine = blockIdx.x < tiles ? (tiles - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
-    const int total = mine * steps;
-    for (int k0 = 0; k0 < total; k0 += kDeep) {
+    for (int i = 0; i < kDeep; ++i) load(va[i], vw[i], valid[i]);
+    while (true) {
 #pragma unroll
         for (int i = 0; i < kDeep; ++i) {
-            const int k = k0 + i;
-            if (k >= total) break;
-            const int s = k % kStages;
-            if (k >= kStages && !wait_or_abort(&C.empty[s], ((k / kStages) - 1) & 1, abort, a.status)) return;
-            unsigned char *sfa = stages + s * kStageBytes + kABytes + kBBytes, *sfw = sfa + kSfABytes;
-            *reinterpret_cast<uint32_t *>(sfa + atom_at(tid)) = va[i].x;
-            *reinterpret_cast<uint32_t *>(sfa + kAtomBytes + atom_at(tid)) = va[i].y;
-            *reinterpret_cast<uint32_t *>(sfw + atom_at(tid)) = vw[i][0].x;
-            *reinterpret_cast<uint32_t *>(sfw + 2 * kAtomBytes + atom_at(tid)) = vw[i][0].y;
+            if (!valid[i]) return;
+            if (!warp_wait(&C.empty[ring.slot], ring.turn ^ 1, abort, a.status)) return;
+            unsigned char *sfa = sf + ring.slot * kStageBytes, *sfw = sfa + kSfABytes;
+            *reinterpret_cast<uint32_t *>(sfa) = va[i].x;
+            *reinterpret_cast<uint32_t *>(sfa + kAtomBytes) = va[i].y;
+            *reinterpret_cast<uint32_t *>(sfw) = vw[i][0].x;
+            *reinterpret_cast<uint32_t *>(sfw + 2 * kAtomBytes) = vw[i][0].y;
             if (tid < kTileN - 128) {
-                *reinterpret_cast<uint32_t *>(sfw + kAtomBytes + atom_at(tid)) = vw[i][1].x;
-                *reinterpret_cast<uint32_t *>(sfw + 3 * kAtomBytes + atom_at(tid)) = vw[i][1].y;
+                *reinterpret_cast<uint32_t *>(sfw + kAtomBytes) = vw[i][1].x;
+                *reinterpret_cast<uint32_t *>(sfw + 3 * kAtomBytes) = vw[i][1].y;
             }
             fence_async_shared();
             __syncwarp();
-            if ((tid & 31) == 0) mbar_arrive(&C.sf_full[s]);
-            load(va[i], vw[i]);
+            if ((tid & 31) == 0) mbar_arrive(&C.sf_full[ring.slot]);
+            ring.next();
+            load(va[i], vw[i], valid[i]);
         }
     }
 }
 
-__device__ void issue_products(Control &C, unsigned char *stages, const MatmulArgs &a, int tiles, int steps) {
+__device__ void issue_products(Control &C, unsigned char *stages, const MatmulArgs &a, int steps) {
     volatile int *abort = &C.abort;
-    int k = 0, i = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
-        const int b = i & 1;
-        if (i >= 2 && !wait_or_abort(&C.acc_empty[b], ((i / 2) - 1) & 1, abort, a.status)) break;
+    const uint32_t base = s_addr(stages), tmem = C.tmem_base;
+    const uint64_t a0 = smem_desc_k_sw128(base), b0 = smem_desc_k_sw128(base + kABytes),
+                   sf0 = smem_desc_atom(base + kABytes + kBBytes);
+    RingPos<kStages> ring;
+    RingPos<2> accs;
+    int consumed = 0;
+    for (Walk t(C, a); t.at(C, a); t.next(), accs.next()) {
+        if (!warp_wait(&C.acc_empty[accs.slot], accs.turn ^ 1, abort, a.status)) return;
         tc_fence_after();
-        const uint32_t acc = C.tmem_base + b * kTileN;
-        bool ok = true;
-        for (int kb = 0; kb < steps && ok; ++kb, ++k) {
-            const int s = k % kStages;
-            ok = wait_or_abort(&C.full[s], (k / kStages) & 1, abort, a.status) &&
-                 wait_or_abort(&C.sf_full[s], (k / kStages) & 1, abort, a.status);
-            if (!ok) break;
+        const uint32_t acc = tmem + accs.slot * kTileN;
+        for (int kb = 0; kb < steps; ++kb, ring.next()) {
+            const int s = ring.slot;
+            if (!warp_wait(&C.full[s], ring.turn, abort, a.status) ||
+                !warp_wait(&C.sf_full[s], ring.turn, abort, a.status))
+                return;
             tc_fence_after();
-            const uint32_t a0 = s_addr(stages + s * kStageBytes), b0 = a0 + kABytes, sfa = b0 + kBBytes,
-                           sfw = sfa + kSfABytes;
-            const uint32_t cols = C.tmem_base + kSfCol0 + s * kSfCols;
+            // addresses are in units of 16 bytes; 64 values are 32 bytes further along K
+            const uint64_t step = (uint64_t)(s * (kStageBytes >> 4));
+            const uint64_t da = a0 + step, db = b0 + step, ds = sf0 + step;
+            const uint32_t cols = tmem + kSfCol0 + s * kSfCols;
+            if (elect_one()) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                copy_atom(cols + h * 12, sfa + h * kAtomBytes);
-                copy_atom(cols + h * 12 + 4, sfw + h * 2 * kAtomBytes);
-                copy_atom(cols + h * 12 + 8, sfw + h * 2 * kAtomBytes + kAtomBytes);
+                for (int h = 0; h < 2; ++h) {
+                    copy_atom(cols + h * 12, ds + h * (kAtomBytes >> 4));
+                    copy_atom(cols + h * 12 + 4, ds + ((kSfABytes + h * 2 * kAtomBytes) >> 4));
+                    copy_atom(cols + h * 12 + 8, ds + ((kSfABytes + (h * 2 + 1) * kAtomBytes) >> 4));
+                }
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                    umma_mxf4(acc, da + kk * 2, db + kk * 2, idesc_mxf4(kTileM, kTileN, (kk & 1) * 2),
+                              cols + (kk >> 1) * 12, cols + (kk >> 1) * 12 + 4, kb | kk);
+                umma_commit(&C.empty[s]);
+                C.consumed = ++consumed;
             }
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)  // 64 values = 32 bytes further along K
-                umma_mxf4(acc, smem_desc_k_sw128(a0 + kk * 32), smem_desc_k_sw128(b0 + kk * 32),
-                          idesc_mxf4(kTileM, kTileN, (kk & 1) * 2), cols + (kk >> 1) * 12, cols + (kk >> 1) * 12 + 4,
-                          (kb | kk) != 0);
-            umma_commit(&C.empty[s]);
-            C.consumed = k + 1;
         }
-        if (!ok) break;
-        umma_commit(&C.acc_full[b]);
+        if (elect_one()) umma_commit(&C.acc_full[accs.slot]);
     }
-    umma_commit(&C.mma_done);
 }
 
-__device__ void store_tiles(Control &C, const MatmulArgs &a, int tiles, int ntiles_n) {
+__device__ void store_tiles(Control &C, const MatmulArgs &a) {
     volatile int *abort = &C.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3;
-    int i = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
-        const Tile tile = tile_of(C, a, t, ntiles_n);
-        const int b = i & 1;
-        if (!wait_or_abort(&C.acc_full[b], (i / 2) & 1, abort, a.status)) return;
+    RingPos<2> accs;
+    for (Walk t(C, a); t.at(C, a); t.next(), accs.next()) {
+        if (!warp_wait(&C.acc_full[accs.slot], accs.turn, abort, a.status)) return;
         tc_fence_after();
         const int r = quarter * 32 + lane;
-        __nv_bfloat16 *row = a.out + ((int64_t)tile.row0 + r) * a.N + tile.n0;
-        const int cols = min(kTileN, a.N - tile.n0);
+        __nv_bfloat16 *row = a.out + ((int64_t)t.row0 + r) * a.N + t.n0;
+        const int cols = min(kTileN, a.N - t.n0);
 #pragma unroll 1
         for (int c0 = 0; c0 < kTileN; c0 += 32) {
             uint32_t v[32];
-            gemm::tmem_ld32(C.tmem_base + b * kTileN + ((uint32_t)(quarter * 32) << 16) + c0, v);
-            if (r >= tile.rows || c0 >= cols) continue;
+            gemm::tmem_ld32(C.tmem_base + accs.slot * kTileN + ((uint32_t)(quarter * 32) << 16) + c0, v);
+            if (r >= t.rows || c0 >= cols) continue;
             if (a.vec_out) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -285,7 +302,7 @@ __device__ void store_tiles(Control &C, const MatmulArgs &a, int tiles, int ntil
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&C.acc_empty[b]);
+        if (lane == 0) mbar_arrive(&C.acc_empty[accs.slot]);
     }
 }
 
@@ -295,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ unsigned char raw[];
     unsigned char *stages = raw + ((1024u - (s_addr(raw) & 1023u)) & 1023u);
     Control &C = *reinterpret_cast<Control *>(stages + kStages * kStageBytes);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = tid >> 5;
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&C.full[s], 1);
@@ -314,16 +331,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     scan_groups(C, a);  // with barriers of the whole CTA
     tc_fence_after();
-    const int ntiles_n = (a.N + kTileN - 1) / kTileN, tiles = C.first[a.groups] * ntiles_n;
     const int steps = (a.blocks + kStepBlocks - 1) / kStepBlocks;
     if (warp == 0) {
-        if (lane == 0) load_operands(C, stages, &map_a, &map_w, a, tiles, ntiles_n, steps);
+        load_operands(C, stages, &map_a, &map_w, a, steps);
     } else if (warp == 1) {
-        if (lane == 0) issue_products(C, stages, a, tiles, steps);
+        issue_products(C, stages, a, steps);
+        __syncwarp();
+        if (elect_one()) umma_commit(&C.mma_done);
     } else if (warp < kSfWarp) {
-        store_tiles(C, a, tiles, ntiles_n);
+        store_tiles(C, a);
     } else {
-        load_all_scales(C, stages, a, tiles, ntiles_n, steps);
+        load_all_scales(C, stages, a, steps);
     }
     __syncwarp();
     tc_fence_before();
@@ -332,8 +350,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // after an abort: copies and products in flight end before the memory is given back
         volatile int no_abort = 0;
         for (int k = C.consumed; k < C.issued; ++k)
-            gemm::mbar_wait(&C.full[k % kStages], (k / kStages) & 1, kWaitNs, &no_abort);
-        gemm::mbar_wait(&C.mma_done, 0, kWaitNs, &no_abort);
+            wait_tries(&C.full[k % kStages], (k / kStages) & 1, &no_abort);
+        wait_tries(&C.mma_done, 0, &no_abort);
     }
     __syncthreads();
     if (warp == 0) gemm::tmem_dealloc(C.tmem_base, kTmemCols);

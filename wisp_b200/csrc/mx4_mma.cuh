@@ -30,7 +30,7 @@ using gemm::umma_commit;
 constexpr int kStepK = 256;                 // values of K in a stage: 128 bytes a row
 constexpr int kStepBlocks = kStepK / kBlock;  // scale bytes of a row in a stage
 constexpr int kAtomBytes = 512;             // scales of 128 rows x 128 values
-constexpr long long kWaitNs = 2000000000;   // limit of one wait
+constexpr uint32_t kTries = 1u << 26;       // limit of one wait
 
 // Device word of the kernels' sticky status on the current device (mx4_matmul.cu).
 int status_word(int **word);
@@ -55,6 +55,23 @@ __device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t adesc, uint6
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sfa), "r"(tmem_sfb), "r"(accumulate)
         : "memory");
 }
+// One lane of the (converged) warp, the same every time: the instructions of
+// the tensor cores are issued by it, while the whole warp computes their
+// addresses, which keeps them in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one != 0;
+}
+// Position in a ring of STAGES: slot, and the parity of its turn.
+template <int STAGES>
+struct RingPos {
+    int slot = 0;
+    uint32_t turn = 0;
+    __device__ __forceinline__ void next() {
+        if (++slot == STAGES) slot = 0, turn ^= 1;
+    }
+};
 // Scale atom: 32 rows of 16 bytes, groups of 8 rows 128 bytes apart, no swizzle.
 __device__ __forceinline__ uint64_t smem_desc_atom(uint32_t saddr) {
     uint64_t d = 0;
@@ -65,27 +82,37 @@ __device__ __forceinline__ uint64_t smem_desc_atom(uint32_t saddr) {
     return d;
 }
 // One scale atom to four columns of tensor memory, in every lane quarter.
-__device__ __forceinline__ void copy_atom(uint32_t taddr, uint32_t saddr) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc_atom(saddr)) : "memory");
+__device__ __forceinline__ void copy_atom(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 // Byte offset of row r's word in a scale atom.
 __device__ __forceinline__ int atom_at(int r) { return (r & 31) * 16 + (r >> 5) * 4; }
 
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Bounded wait; a wait that runs out sets the status and the CTA's abort word.
+// Bounded wait: kTries attempts (a second or more; reading a timer in the loop
+// would delay every wait that does not succeed at once).
+__device__ __forceinline__ bool wait_tries(uint64_t *bar, uint32_t parity, const volatile int *abort) {
+    for (uint32_t i = 1; !mbar_try(bar, parity); ++i)
+        if (i % 256 == 0 && (*abort || i >= kTries)) return false;
+    return true;
+}
+// The same; a wait that runs out sets the status and the CTA's abort word.
 __device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
-    if (gemm::mbar_wait(bar, parity, kWaitNs, abort)) return true;
+    if (wait_tries(bar, parity, abort)) return true;
     *abort = 1;
     *reinterpret_cast<volatile int *>(status) = WISP_ERR_TIMEOUT;
     return false;
 }
 
-// The eight scale bytes of a row in stage kb (bytes behind the row's last: 0).
-// `align`: what the rows' scale bytes are aligned to.
-__device__ __forceinline__ uint2 load_scales(const uint8_t *row, int kb, int blocks, int align) {
-    const uint8_t *p = row + kb * kStepBlocks;
-    const int left = blocks - kb * kStepBlocks;
+// For a converged warp: all lanes wait, all go on or none does.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
+    return __all_sync(0xFFFFFFFFu, wait_or_abort(bar, parity, abort, status));
+}
+
+// The eight scale bytes of a row in a stage, of which `left` are the row's (the
+// others: 0).  `align`: what the rows' scale bytes are aligned to.
+__device__ __forceinline__ uint2 load_scales(const uint8_t *p, int left, int align) {
     if (align >= 8) return __ldg(reinterpret_cast<const uint2 *>(p));
     uint2 v = make_uint2(0, 0);
     if (align >= 4) {

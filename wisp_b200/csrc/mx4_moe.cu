@@ -107,6 +107,7 @@ struct Control {
     uint64_t acc_full[2], acc_empty[2], mma_done;
     uint32_t tmem_base;
     int abort, issued, consumed;
+    int cut[kMaxSplit + 1];  // K steps at which the pieces of D begin
 };
 
 // ---- phase R ------------------------------------------------------------------
@@ -324,32 +325,49 @@ __device__ void build_lists(const MoeArgs &a, Lists &L, Scratch &S) {
 }
 
 // ---- phases G and D ---------------------------------------------------------------
-// The tiles of a phase: tile t belongs to group t / per_group.  Weight rows:
-// the first 64 from slot * slot_rows + m0 on, the second 64 from `second`
-// rows further on.  K: `blocks` scale bytes a row, steps of 256 values, in
-// `split` pieces.
+// The tiles of a phase, in the order group, piece of K, rows; a CTA takes every
+// gridDim.x-th.  Weight rows: the first 64 of a tile from slot * slot_rows +
+// m0 on, the second 64 from `second` rows further on.  K: `blocks` scale bytes
+// a row, `steps` steps of 256 values, in `split` pieces.
 struct Phase {
     const CUtensorMap *map;
     const uint8_t *w_scales, *b_codes, *b_scales;
     int64_t w_rows;  // rows of the weight matrix
-    int tiles, per_group, m_tiles, split, rows_m, slot_rows, second, blocks, steps, align, token_div;
+    int groups, m_tiles, split, rows_m, slot_rows, second, blocks, steps, align, token_div;
 };
-struct MoeTile {
-    int g, piece, m0, kb0, kb1, off, n;
-    int64_t row;  // of the weight matrix
+// A CTA's walk over the tiles.  (Roles that are one thread or warp feel every
+// instruction: no divisions here, nor remainders in the ring's positions.)
+struct Walk {
+    int per_group, dg, din;  // gridDim.x in groups and tiles
+    int g, in;
+    // the tile
+    int m0, kb0, kb1, off, n, piece;
+    int64_t row;
+    __device__ __forceinline__ Walk(const Phase &ph) {
+        per_group = ph.m_tiles * ph.split;
+        dg = gridDim.x / per_group, din = gridDim.x - dg * per_group;
+        g = blockIdx.x / per_group, in = blockIdx.x - g * per_group;
+    }
+    // False behind the last tile.
+    __device__ __forceinline__ bool at(const Phase &ph, const Lists &L, const Control &C) {
+        if (g >= ph.groups) return false;
+        int m = in;
+        piece = 0, kb0 = 0, kb1 = ph.steps;
+        if (ph.split > 1) {
+            for (; m >= ph.m_tiles; m -= ph.m_tiles) ++piece;
+            kb0 = C.cut[piece], kb1 = C.cut[piece + 1];
+        }
+        m0 = m * ph.rows_m;
+        off = L.off[g];
+        n = L.off[g + 1] - off;
+        row = (int64_t)L.slots[g] * ph.slot_rows + m0;
+        return true;
+    }
+    __device__ __forceinline__ void next() {
+        g += dg, in += din;
+        if (in >= per_group) in -= per_group, ++g;
+    }
 };
-__device__ __forceinline__ MoeTile moe_tile(const Phase &ph, const Lists &L, int t) {
-    MoeTile r;
-    r.g = t / ph.per_group;
-    const int in = t - r.g * ph.per_group;
-    r.piece = in / ph.m_tiles;
-    r.m0 = (in - r.piece * ph.m_tiles) * ph.rows_m;
-    r.kb0 = r.piece * ph.steps / ph.split, r.kb1 = (r.piece + 1) * ph.steps / ph.split;
-    r.off = L.off[r.g];
-    r.n = min(L.off[r.g + 1] - r.off, kGroup);
-    r.row = (int64_t)L.slots[r.g] * ph.slot_rows + r.m0;
-    return r;
-}
 
 __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -358,68 +376,73 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t b
                  : "memory");
 }
 
-// Ring position that lives on from phase to phase.
+// What of a role lives on from phase to phase.
 struct Cursor {
-    int k = 0;     // step
-    int tile = 0;  // tile of the phase's MMA and epilogue order (accumulator turn)
+    RingPos<kStages> ring;
+    RingPos<2> acc;
 };
 
-__device__ __forceinline__ void load_weights(unsigned char *st, const Phase &ph, const MoeTile &t, int kb, uint64_t *bar) {
+__device__ __forceinline__ void load_weights(unsigned char *st, const Phase &ph, const Walk &t, int kb, uint64_t *bar) {
     tma_load_2d(st, ph.map, kb * 128, (int)t.row, bar);
     tma_load_2d(st + kABytes / 2, ph.map, kb * 128, (int)t.row + ph.second, bar);
 }
-__device__ __forceinline__ void load_terms(unsigned char *st, const Phase &ph, const Lists &L, const MoeTile &t, int kb,
-                                           uint64_t *bar) {
-    for (int i = 0; i < t.n; ++i)
-        bulk_load(st + kABytes + i * kTermBytes,
-                  ph.b_codes + ((size_t)(L.pair[t.off + i] / ph.token_div) * ph.steps + kb) * kTermBytes, kTermBytes, bar);
-}
 
-// Copies of a phase's steps; the weights of the first `early` steps are on
-// their way already.
+// Copies of a phase's steps: the first lane brings the weights (those of the
+// first `early` steps are on their way already), lane i token i's terms.
 __device__ void run_copies(Control &C, unsigned char *stages, const Phase &ph, const Lists &L, Cursor &cur, int early,
                            int *status) {
     volatile int *abort = &C.abort;
-    for (int t = blockIdx.x; t < ph.tiles; t += gridDim.x) {
-        const MoeTile tile = moe_tile(ph, L, t);
-        for (int kb = tile.kb0; kb < tile.kb1; ++kb, ++cur.k) {
-            const int s = cur.k % kStages;
-            unsigned char *st = stages + s * kStageBytes;
+    const int lane = threadIdx.x & 31;
+    int issued = C.issued;
+    for (Walk t(ph); t.at(ph, L, C); t.next()) {
+        const uint8_t *terms =
+            lane < t.n ? ph.b_codes + ((size_t)(L.pair[t.off + lane] / ph.token_div) * ph.steps + t.kb0) * kTermBytes
+                       : nullptr;
+        const uint32_t bytes = kABytes + t.n * kTermBytes;
+        for (int kb = t.kb0; kb < t.kb1; ++kb, cur.ring.next()) {
+            unsigned char *st = stages + cur.ring.slot * kStageBytes;
+            uint64_t *full = &C.full[cur.ring.slot];
             if (early > 0) {
                 --early;
             } else {
-                if (cur.k >= kStages && !wait_or_abort(&C.empty[s], ((cur.k / kStages) - 1) & 1, abort, status)) return;
-                mbar_expect_tx(&C.full[s], kABytes + tile.n * kTermBytes);
-                load_weights(st, ph, tile, kb, &C.full[s]);
+                if (!warp_wait(&C.empty[cur.ring.slot], cur.ring.turn ^ 1, abort, status)) return;
+                if (lane == 0) {
+                    mbar_expect_tx(full, bytes);
+                    load_weights(st, ph, t, kb, full);
+                }
+                __syncwarp();  // the bytes are announced before any of them can arrive
             }
-            load_terms(st, ph, L, tile, kb, &C.full[s]);
-            C.issued = cur.k + 1;
+            if (terms) {
+                bulk_load(st + kABytes + lane * kTermBytes, terms, kTermBytes, full);
+                terms += kTermBytes;
+            }
+            if (lane == 0) C.issued = ++issued;
         }
     }
 }
 // The weights of the phase's first steps, as many as the ring holds; returns
 // how many.
-__device__ int copy_early(Control &C, unsigned char *stages, const Phase &ph, const Lists &L, int k, int *status) {
+__device__ int copy_early(Control &C, unsigned char *stages, const Phase &ph, const Lists &L, RingPos<kStages> ring,
+                          int *status) {
     volatile int *abort = &C.abort;
+    const int lane = threadIdx.x & 31;
     int early = 0;
-    for (int t = blockIdx.x; t < ph.tiles; t += gridDim.x) {
-        const MoeTile tile = moe_tile(ph, L, t);
-        for (int kb = tile.kb0; kb < tile.kb1; ++kb, ++k) {
-            if (early == kStages) return early;
-            const int s = k % kStages;
-            if (k >= kStages && !wait_or_abort(&C.empty[s], ((k / kStages) - 1) & 1, abort, status)) return early;
-            mbar_expect_tx(&C.full[s], kABytes + tile.n * kTermBytes);
-            load_weights(stages + s * kStageBytes, ph, tile, kb, &C.full[s]);
+    for (Walk t(ph); t.at(ph, L, C); t.next())
+        for (int kb = t.kb0; kb < t.kb1; ++kb, ring.next()) {
+            if (early == kStages || !warp_wait(&C.empty[ring.slot], ring.turn ^ 1, abort, status)) return early;
+            if (lane == 0) {
+                mbar_expect_tx(&C.full[ring.slot], kABytes + t.n * kTermBytes);
+                load_weights(stages + ring.slot * kStageBytes, ph, t, kb, &C.full[ring.slot]);
+            }
             ++early;
         }
-    }
     return early;
 }
 
-// Scale bytes written by this kernel: not through the read-only path.
-__device__ __forceinline__ uint2 load_term_scales(const uint8_t *p, int left) {
-    uint2 v = __ldcg(reinterpret_cast<const uint2 *>(p));
-    if (left < 8) {  // blocks behind the last: whatever lies there is not a scale
+// The first `left` of eight scale bytes; what lies behind a row's last block is
+// not a scale.
+__device__ __forceinline__ uint2 first_bytes(uint2 v, int left) {
+    if (left < 8) {
         const uint64_t keep = (1ull << (8 * left)) - 1;
         v.x &= (uint32_t)keep, v.y &= (uint32_t)(keep >> 32);
     }
@@ -430,84 +453,103 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
     constexpr int kDeep = 4;  // stages whose scale bytes are in registers
     const int tid = threadIdx.x - kSfWarp * 32;
     volatile int *abort = &C.abort;
-    int lt = blockIdx.x, lkb = 0, lend = 0, total = 0;
-    const uint8_t *pw = nullptr, *pb = nullptr;
+    unsigned char *sf = stages + kABytes + kBBytes + atom_at(tid);
+    // the loads run kDeep steps ahead of the stores
+    Walk ahead(ph);
+    bool more = ahead.at(ph, L, C);
+    int kb = 0;
+    const uint8_t *pw = nullptr, *pb = nullptr;  // of step kb
     auto point = [&] {
-        if (lt >= ph.tiles) return;
-        const MoeTile tile = moe_tile(ph, L, lt);
-        lkb = tile.kb0, lend = tile.kb1;
-        const int64_t row = tile.row + (tid < 64 ? tid : ph.second + tid - 64);
-        pw = row < ph.w_rows ? ph.w_scales + row * ph.blocks : nullptr;
+        kb = ahead.kb0;
+        const int64_t row = ahead.row + (tid < 64 ? tid : ph.second + tid - 64);
+        pw = row < ph.w_rows ? ph.w_scales + row * ph.blocks + kb * kStepBlocks : nullptr;
         const int i = tid / kRows, q = tid % kRows;
-        pb = i < tile.n && q < kTerms
-                 ? ph.b_scales + (size_t)(L.pair[tile.off + i] / ph.token_div) * ph.steps * kScaleBytes + q * kStepBlocks
+        pb = i < ahead.n && q < kTerms
+                 ? ph.b_scales + ((size_t)(L.pair[ahead.off + i] / ph.token_div) * ph.steps + kb) * kScaleBytes +
+                       q * kStepBlocks
                  : nullptr;
     };
-    auto load = [&](uint2 &x, uint2 &y) {
-        if (lt >= ph.tiles) return;
-        x = pw ? load_scales(pw, lkb, ph.blocks, ph.align) : make_uint2(0, 0);
-        y = pb ? load_term_scales(pb + (size_t)lkb * kScaleBytes, ph.blocks - lkb * kStepBlocks) : make_uint2(0, 0);
-        if (++lkb == lend) {
-            lt += gridDim.x;
-            point();
+    // nothing here may wait for what it loads: the values are used kDeep steps later
+    auto load = [&](uint2 &x, uint2 &y, int &left) {
+        left = more ? ph.blocks - kb * kStepBlocks : 0;
+        if (!more) return;
+        x = y = make_uint2(0, 0);
+        if (pw) {
+            x = load_scales(pw, left, ph.align);
+            pw += kStepBlocks;
+        }
+        if (pb) {  // (written by this kernel: not through the read-only path)
+            y = __ldcg(reinterpret_cast<const uint2 *>(pb));
+            pb += kScaleBytes;
+        }
+        if (++kb == ahead.kb1) {
+            ahead.next();
+            more = ahead.at(ph, L, C);
+            if (more) point();
         }
     };
-    for (int t = blockIdx.x; t < ph.tiles; t += gridDim.x) {
-        const int piece = (t % ph.per_group) / ph.m_tiles;
-        total += (piece + 1) * ph.steps / ph.split - piece * ph.steps / ph.split;
-    }
-    point();
+    if (more) point();
     uint2 vw[kDeep], vb[kDeep];
+    int left[kDeep];
 #pragma unroll
-    for (int i = 0; i < kDeep; ++i) load(vw[i], vb[i]);
-    for (int n0 = 0; n0 < total; n0 += kDeep) {
+    for (int i = 0; i < kDeep; ++i) load(vw[i], vb[i], left[i]);
+    while (true) {
 #pragma unroll
         for (int i = 0; i < kDeep; ++i) {
-            if (n0 + i >= total) break;
-            const int k = cur.k + n0 + i, s = k % kStages;
-            if (k >= kStages && !wait_or_abort(&C.empty[s], ((k / kStages) - 1) & 1, abort, status)) return;
-            unsigned char *sf = stages + s * kStageBytes + kABytes + kBBytes + atom_at(tid);
-            *reinterpret_cast<uint32_t *>(sf) = vw[i].x;
-            *reinterpret_cast<uint32_t *>(sf + kAtomBytes) = vw[i].y;
-            *reinterpret_cast<uint32_t *>(sf + 2 * kAtomBytes) = vb[i].x;
-            *reinterpret_cast<uint32_t *>(sf + 3 * kAtomBytes) = vb[i].y;
+            if (left[i] <= 0) return;
+            if (!warp_wait(&C.empty[cur.ring.slot], cur.ring.turn ^ 1, abort, status)) return;
+            unsigned char *at = sf + cur.ring.slot * kStageBytes;
+            const uint2 terms = first_bytes(vb[i], left[i]);
+            *reinterpret_cast<uint32_t *>(at) = vw[i].x;
+            *reinterpret_cast<uint32_t *>(at + kAtomBytes) = vw[i].y;
+            *reinterpret_cast<uint32_t *>(at + 2 * kAtomBytes) = terms.x;
+            *reinterpret_cast<uint32_t *>(at + 3 * kAtomBytes) = terms.y;
             fence_async_shared();
             __syncwarp();
-            if ((tid & 31) == 0) mbar_arrive(&C.sf_full[s]);
-            load(vw[i], vb[i]);
+            if ((tid & 31) == 0) mbar_arrive(&C.sf_full[cur.ring.slot]);
+            cur.ring.next();
+            load(vw[i], vb[i], left[i]);
         }
     }
-    cur.k += total;
 }
 
+// The whole warp walks, one lane issues.
 __device__ void run_products(Control &C, unsigned char *stages, const Phase &ph, const Lists &L, Cursor &cur, int *status) {
     volatile int *abort = &C.abort;
-    for (int t = blockIdx.x; t < ph.tiles; t += gridDim.x, ++cur.tile) {
-        const MoeTile tile = moe_tile(ph, L, t);
-        const int b = cur.tile & 1;
-        if (cur.tile >= 2 && !wait_or_abort(&C.acc_empty[b], ((cur.tile / 2) - 1) & 1, abort, status)) return;
+    const uint32_t base = s_addr(stages);
+    const uint64_t a0 = smem_desc_k_sw128(base), b0 = smem_desc_k_sw128(base + kABytes),
+                   sf0 = smem_desc_atom(base + kABytes + kBBytes);
+    const uint32_t tmem = C.tmem_base;
+    int consumed = C.consumed;
+    for (Walk t(ph); t.at(ph, L, C); t.next(), cur.acc.next()) {
+        if (!warp_wait(&C.acc_empty[cur.acc.slot], cur.acc.turn ^ 1, abort, status)) return;
         tc_fence_after();
-        const uint32_t acc = C.tmem_base + b * kAccCols;
-        const int N = (tile.n * kRows + 15) / 16 * 16;
-        const uint32_t id0 = idesc_mxf4(128, N, 0), id1 = idesc_mxf4(128, N, 2);
-        for (int kb = tile.kb0; kb < tile.kb1; ++kb, ++cur.k) {
-            const int s = cur.k % kStages;
-            if (!wait_or_abort(&C.full[s], (cur.k / kStages) & 1, abort, status) ||
-                !wait_or_abort(&C.sf_full[s], (cur.k / kStages) & 1, abort, status))
+        const uint32_t acc = tmem + cur.acc.slot * kAccCols;
+        const uint32_t id0 = idesc_mxf4(128, (t.n * kRows + 15) / 16 * 16, 0), id1 = id0 | (2u << 4) | (2u << 29);
+        uint32_t more = 0;
+        for (int kb = t.kb0; kb < t.kb1; ++kb, cur.ring.next()) {
+            const int s = cur.ring.slot;
+            if (!warp_wait(&C.full[s], cur.ring.turn, abort, status) ||
+                !warp_wait(&C.sf_full[s], cur.ring.turn, abort, status))
                 return;
             tc_fence_after();
-            const uint32_t a0 = s_addr(stages + s * kStageBytes), b0 = a0 + kABytes, sf = b0 + kBBytes;
-            const uint32_t cols = C.tmem_base + kSfCol0 + s * kSfCols;
+            // addresses are in units of 16 bytes; 64 values are 32 bytes further along K
+            const uint64_t step = (uint64_t)(s * (kStageBytes >> 4));
+            const uint64_t da = a0 + step, db = b0 + step, ds = sf0 + step;
+            const uint32_t cols = tmem + kSfCol0 + s * kSfCols;
+            if (elect_one()) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) copy_atom(cols + i * 4, sf + i * kAtomBytes);
+                for (int i = 0; i < 4; ++i) copy_atom(cols + i * 4, ds + i * (kAtomBytes >> 4));
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)  // 64 values = 32 bytes further along K
-                umma_mxf4(acc, smem_desc_k_sw128(a0 + kk * 32), smem_desc_k_sw128(b0 + kk * 32), kk & 1 ? id1 : id0,
-                          cols + (kk >> 1) * 4, cols + 8 + (kk >> 1) * 4, kb != tile.kb0 || kk != 0);
-            umma_commit(&C.empty[s]);
-            C.consumed = cur.k + 1;
+                for (int kk = 0; kk < 4; ++kk)
+                    umma_mxf4(acc, da + kk * 2, db + kk * 2, kk & 1 ? id1 : id0, cols + (kk >> 1) * 4,
+                              cols + 8 + (kk >> 1) * 4, more | kk);
+                umma_commit(&C.empty[s]);
+                C.consumed = ++consumed;
+            }
+            more = 1;
         }
-        umma_commit(&C.acc_full[b]);
+        if (elect_one()) umma_commit(&C.acc_full[cur.acc.slot]);
     }
 }
 
@@ -528,10 +570,9 @@ __device__ void run_gate_up(Control &C, const Phase &ph, const Lists &L, Cursor 
                             int steps_out) {
     volatile int *abort = &C.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3;
-    for (int t = blockIdx.x; t < ph.tiles; t += gridDim.x, ++cur.tile) {
-        const MoeTile tile = moe_tile(ph, L, t);
-        const int b = cur.tile & 1;
-        const bool ok = wait_or_abort(&C.acc_full[b], (cur.tile / 2) & 1, abort, a.status);
+    for (Walk tile(ph); tile.at(ph, L, C); tile.next(), cur.acc.next()) {
+        const int b = cur.acc.slot;
+        const bool ok = warp_wait(&C.acc_full[b], cur.acc.turn, abort, a.status);
         if (ok) {
             tc_fence_after();
             for (int i = 0; i < tile.n; i += 4) {
@@ -561,10 +602,9 @@ __device__ void run_gate_up(Control &C, const Phase &ph, const Lists &L, Cursor 
 __device__ void run_down(Control &C, const Phase &ph, const Lists &L, Cursor &cur, const MoeArgs &a) {
     volatile int *abort = &C.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3;
-    for (int t = blockIdx.x; t < ph.tiles; t += gridDim.x, ++cur.tile) {
-        const MoeTile tile = moe_tile(ph, L, t);
-        const int b = cur.tile & 1;
-        if (!wait_or_abort(&C.acc_full[b], (cur.tile / 2) & 1, abort, a.status)) return;
+    for (Walk tile(ph); tile.at(ph, L, C); tile.next(), cur.acc.next()) {
+        const int b = cur.acc.slot;
+        if (!warp_wait(&C.acc_full[b], cur.acc.turn, abort, a.status)) return;
         tc_fence_after();
         const int h = tile.m0 + quarter * 32 + lane;
         for (int i = 0; i < tile.n; i += 4) {
@@ -660,24 +700,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     Phase up{}, down{};
     up.map = &map13, up.w_scales = a.s13, up.b_codes = a.xq, up.b_scales = a.xs;
     up.blocks = a.H / kBlock, up.steps = (up.blocks + kStepBlocks - 1) / kStepBlocks, up.align = a.s13_align;
-    up.m_tiles = up.per_group = (a.I + 63) / 64, up.tiles = L.n * up.per_group, up.split = 1, up.rows_m = 64;
+    up.groups = L.n, up.m_tiles = (a.I + 63) / 64, up.split = 1, up.rows_m = 64;
     up.slot_rows = 2 * a.I, up.second = a.I, up.w_rows = (int64_t)a.slots * 2 * a.I, up.token_div = a.k;
     down.map = &map2, down.w_scales = a.s2, down.b_codes = a.aq, down.b_scales = a.as;
     down.blocks = a.I / kBlock, down.steps = (down.blocks + kStepBlocks - 1) / kStepBlocks, down.align = a.s2_align;
-    down.m_tiles = (a.H + 127) / 128, down.split = choose_split(L.n * down.m_tiles, down.steps, a.max_split);
-    down.per_group = down.m_tiles * down.split, down.tiles = L.n * down.per_group, down.rows_m = 128;
+    down.groups = L.n, down.m_tiles = (a.H + 127) / 128, down.rows_m = 128;
+    down.split = choose_split(L.n * down.m_tiles, down.steps, a.max_split);
     down.slot_rows = a.H, down.second = 64, down.w_rows = (int64_t)a.slots * a.H, down.token_div = 1;
+
+    if (tid <= down.split) C.cut[tid] = tid * down.steps / down.split;
+    __syncthreads();
 
     // G
     Cursor cur;
     int early = 0;
     if (warp == 0) {
-        if (lane == 0) {
-            run_copies(C, stages, up, L, cur, 0, a.status);
-            early = copy_early(C, stages, down, L, cur.k, a.status);
-        }
+        run_copies(C, stages, up, L, cur, 0, a.status);
+        early = copy_early(C, stages, down, L, cur.ring, a.status);
     } else if (warp == 1) {
-        if (lane == 0) run_products(C, stages, up, L, cur, a.status);
+        run_products(C, stages, up, L, cur, a.status);
     } else if (warp < kSfWarp) {
         run_gate_up(C, up, L, cur, a, ex, down.steps);
     } else {
@@ -690,12 +731,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // D
     if (warp == 0) {
-        if (lane == 0) run_copies(C, stages, down, L, cur, early, a.status);
+        run_copies(C, stages, down, L, cur, early, a.status);
     } else if (warp == 1) {
-        if (lane == 0) {
-            run_products(C, stages, down, L, cur, a.status);
-            umma_commit(&C.mma_done);
-        }
+        run_products(C, stages, down, L, cur, a.status);
+        __syncwarp();
+        if (elect_one()) umma_commit(&C.mma_done);
     } else if (warp < kSfWarp) {
         run_down(C, down, L, cur, a);
     } else {
@@ -725,8 +765,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // after an abort: copies and products in flight end before the memory is given back
         volatile int no_abort = 0;
         for (int k = C.consumed; k < C.issued; ++k)
-            gemm::mbar_wait(&C.full[k % kStages], (k / kStages) & 1, kWaitNs, &no_abort);
-        gemm::mbar_wait(&C.mma_done, 0, kWaitNs, &no_abort);
+            wait_tries(&C.full[k % kStages], (k / kStages) & 1, &no_abort);
+        wait_tries(&C.mma_done, 0, &no_abort);
     }
     __syncthreads();
     if (warp == 0) gemm::tmem_dealloc(C.tmem_base, kTmemCols);

@@ -89,9 +89,9 @@ struct MoeArgs {
 
 // What the lists are built from; lies where the ring will be.
 struct Scratch {
-    int ids[kMaxPairs];  // expert of pair t * k + j, -1: none
-    unsigned short rank[kMaxPairs];
-    int count[kMaxExperts];
+    int ids[kMaxPairs];              // expert of pair t * k + j, -1: none
+    uint32_t tokens[kMaxExperts][2];  // the tokens routed to an expert, a bit each
+    int begin[kMaxExperts];          // where its pairs begin, -1: no slot
     int scan[kWarps];
 };
 struct Lists {
@@ -153,7 +153,7 @@ constexpr int kAhead = 8;  // 16-byte loads of a lane in flight
 // One expert's row times TOKENS tokens.
 template <int TOKENS>
 __device__ void route_products(const MoeArgs &a, int gw, int nw, int lane) {
-    constexpr int kDeep = TOKENS == 1 ? kAhead : 2;
+    constexpr int kDeep = TOKENS == 1 ? kAhead : TOKENS == 2 ? 4 : 2;
     const int groups = (a.T + TOKENS - 1) / TOKENS;
     for (int u = gw; u < a.E * groups; u += nw) {
         const int e = u % a.E, t0 = u / a.E * TOKENS;
@@ -195,44 +195,47 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
     return key == 1 ? NAN : __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
-// Top-k of token t by (logit descending, id ascending), softmax weights.
+// Top-k of token t by (logit descending, id ascending), softmax weights.  A
+// lane keeps its best key; only the lane that wins a round looks for its next.
 template <int PER_LANE>
 __device__ void route_token(const MoeArgs &a, Lists &L, Scratch &S, int t, int lane) {
-    uint32_t key[PER_LANE];
+    const float *logits = a.logits + (size_t)t * a.E;
+    uint32_t key[PER_LANE], best = 0;
+    int at = 0, my_id = -1;
+    uint32_t mine = 0;
 #pragma unroll
     for (int i = 0; i < PER_LANE; ++i) {
         const int e = i * 32 + lane;
-        key[i] = e < a.E ? key_of(__ldcg(a.logits + (size_t)t * a.E + e)) : 0;
+        key[i] = e < a.E ? key_of(__ldcg(logits + e)) : 0;
+        if (key[i] > best) best = key[i], at = i;
     }
-    float mx = 0.f, all = 0.f, mine = 0.f;
-    int my_id = -1;
     for (int j = 0; j < a.k; ++j) {
-        uint32_t best = 0;
-        int id = 0;
-#pragma unroll
-        for (int i = 0; i < PER_LANE; ++i)
-            if (key[i] > best) best = key[i], id = i * 32 + lane;
         const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
-        const unsigned who = __ballot_sync(0xFFFFFFFFu, best == top);
-        if (who & (who - 1))  // equal logits: the lowest id
-            id = (int)__reduce_min_sync(0xFFFFFFFFu, best == top ? (uint32_t)id : 0x7FFFFFFFu);
-        else
-            id = __shfl_sync(0xFFFFFFFFu, id, __ffs(who) - 1);
-        if (j == 0) {
-            mx = logit_of(top);
-            if (!a.renormalize) {
+        unsigned who = __ballot_sync(0xFFFFFFFFu, best == top);
+        if (who & (who - 1)) {  // equal logits: the lowest id
+            const uint32_t low = __reduce_min_sync(0xFFFFFFFFu, best == top ? (uint32_t)(at * 32 + lane) : 0x7FFFFFFFu);
+            who = 1u << (low & 31);
+        }
+        const int winner = __ffs(who) - 1, id = __shfl_sync(0xFFFFFFFFu, at, winner) * 32 + winner;
+        if (lane == j) mine = top, my_id = id;
+        if (lane == winner) {
+            const int gone = at;
+            best = 0;
 #pragma unroll
-                for (int i = 0; i < PER_LANE; ++i)
-                    if (key[i]) all += expf(logit_of(key[i]) - mx);
+            for (int i = 0; i < PER_LANE; ++i) {
+                if (i == gone) key[i] = 0;
+                if (key[i] > best) best = key[i], at = i;
             }
         }
-#pragma unroll
-        for (int i = 0; i < PER_LANE; ++i)
-            if (i * 32 + lane == id) key[i] = 0;
-        if (lane == j) mine = logit_of(top), my_id = id;
     }
-    const float p = lane < a.k ? expf(mine - mx) : 0.f;
-    const float sum = warp_sum(a.renormalize ? p : all);
+    const float l = logit_of(mine), mx = __shfl_sync(0xFFFFFFFFu, l, 0);
+    float p = 0.f, all = 0.f;
+    if (lane < a.k) p = all = expf(l - mx);
+    if (!a.renormalize) {
+        all = 0.f;
+        for (int e = lane; e < a.E; e += 32) all += expf(__ldcg(logits + e) - mx);
+    }
+    const float sum = warp_sum(all);
     if (lane < a.k) {
         S.ids[t * a.k + lane] = my_id;
         L.w[t * a.k + lane] = p / sum;
@@ -258,28 +261,22 @@ __device__ void given_token(const MoeArgs &a, Lists &L, Scratch &S, int t) {
 
 // Pairs by expert, the experts with a slot in ascending order, in groups of at
 // most kGroup.  Every CTA has to come to the same groups, so an expert's pairs
-// keep their order: one warp counts them, 32 at a time.
+// lie in the order of their tokens (a token names an expert at most once): the
+// expert's set of tokens, a bit each, gives count and rank whatever the order
+// in which the bits were set.
 __device__ void build_lists(const MoeArgs &a, Lists &L, Scratch &S) {
     constexpr int kPer = (kMaxExperts + kThreads - 1) / kThreads;
     const int P = a.T * a.k, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (warp == 0)
-        for (int p0 = 0; p0 < P; p0 += 32) {
-            const int p = p0 + lane, e = p < P ? S.ids[p] : -1;
-            const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
-            const int before = e >= 0 ? S.count[e] : 0;
-            __syncwarp();
-            if (e >= 0) {
-                S.rank[p] = (unsigned short)(before + __popc(same & ((1u << lane) - 1)));
-                if (lane == __ffs(same) - 1) S.count[e] = before + __popc(same);
-            }
-            __syncwarp();
-        }
+    for (int p = tid; p < P; p += kThreads) {
+        const int e = S.ids[p], t = p / a.k;
+        if (e >= 0) atomicOr(&S.tokens[e][t >> 5], 1u << (t & 31));
+    }
     __syncthreads();
     int count[kPer], slot[kPer], own = 0;  // pairs in the low half of `own`, groups in the high half
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int e = tid * kPer + i;
-        count[i] = e < a.E ? S.count[e] : 0;
+        count[i] = e < a.E ? __popc(S.tokens[e][0]) + __popc(S.tokens[e][1]) : 0;
         if (!count[i]) continue;
         slot[i] = a.expert_map ? a.expert_map[e] : e;
         if (slot[i] < 0 || slot[i] >= a.slots) count[i] = 0;
@@ -304,7 +301,7 @@ __device__ void build_lists(const MoeArgs &a, Lists &L, Scratch &S) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int e = tid * kPer + i;
-        if (e < a.E) S.count[e] = count[i] ? pos : -1;  // from here on: where the expert's pairs begin
+        if (e < a.E) S.begin[e] = count[i] ? pos : -1;
         for (int done = 0; done < count[i]; done += kGroup, ++g) {
             L.slots[g] = slot[i];
             L.off[g] = (unsigned short)(pos + done);
@@ -317,9 +314,13 @@ __device__ void build_lists(const MoeArgs &a, Lists &L, Scratch &S) {
     }
     __syncthreads();
     for (int p = tid; p < P; p += kThreads) {
-        const int e = S.ids[p], at = e >= 0 ? S.count[e] : -1;
+        const int e = S.ids[p], at = e >= 0 ? S.begin[e] : -1, t = p / a.k;
         L.has[p] = at >= 0;
-        if (at >= 0) L.pair[at + S.rank[p]] = (unsigned short)p;
+        if (at < 0) continue;
+        const uint32_t before = (1u << (t & 31)) - 1;
+        const int rank = t < 32 ? __popc(S.tokens[e][0] & before)
+                                : __popc(S.tokens[e][0]) + __popc(S.tokens[e][1] & before);
+        L.pair[at + rank] = (unsigned short)p;
     }
     __syncthreads();
 }
@@ -667,13 +668,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     // R: warps in turn over the SMs, so that few units spread
     const int gw = warp * gridDim.x + blockIdx.x;
     if (a.router) {
-        if (a.E * a.T <= nw)  // a warp for each product
+        // as many warps at work as there are: the fewest tokens a unit with which no warp has two
+        if (a.E * a.T <= nw)
             route_products<1>(a, gw, nw, lane);
+        else if (a.E * ((a.T + 1) / 2) <= nw)
+            route_products<2>(a, gw, nw, lane);
         else
             route_products<4>(a, gw, nw, lane);
     }
     convert_tokens(a, nw - 1 - gw, nw, lane);
-    for (int e = tid; e < a.E; e += kThreads) S.count[e] = 0;
+    for (int i = tid; i < 2 * a.E; i += kThreads) (&S.tokens[0][0])[i] = 0;
     asm volatile("fence.proxy.async;" ::: "memory");  // the terms are read by bulk copies
     cg::this_grid().sync();
     tc_fence_after();

@@ -7,15 +7,16 @@
 //
 // All of it in fp32; r' and n are rounded once each, n from the unrounded r'.
 //
-// Bound by HBM: y and the residual are read once, r' and n written once.  A
-// CTA holds a row in registers, so the two means cost no second read; several
-// CTAs share an SM, so that one row's loads cover another's reductions (a
-// thread that loads its next row early needs twice the registers, which
-// measured slower), and the weights, which every row shares, stay in L1.  A
-// thread's pieces of a row are VEC values wide: 8 where the width and every
-// address allow 16-byte accesses, else 2, else 1; NV of them, so that a row
-// takes 256 threads or fewer where it can (more rows in flight on an SM,
-// fewer warps in a reduction).
+// Bound by HBM: y and the residual are read once, r' and n written once.  The
+// CTAs are persistent; a thread copies the pieces of its CTA's next two rows
+// to shared memory (cp.async, its own pieces only, so nothing but its own
+// copies has to be waited for) while the present row lies in registers, which
+// covers the two reductions of a row without the registers of a second row.
+// The weights, which every row shares, stay in L1.  A thread's pieces of a row
+// are VEC values wide: 8 where the width and every address allow 16-byte
+// accesses, else 2, else 1 (2-byte pieces have no asynchronous copy and are
+// loaded where they are used); NV of them, so that a row takes 256 threads or
+// fewer where it can (more rows in flight, fewer warps in a reduction).
 #include <type_traits>
 
 #include "mx4.cuh"
@@ -29,6 +30,7 @@ struct NormArgs {
     int64_t rows, y_stride, res_stride, gate_stride;
     int cols, gate_kind;
     float scale, eps;
+    int ahead;
 };
 
 template <typename T>
@@ -67,6 +69,16 @@ struct Piece {
 #pragma unroll
         for (int i = 0; i < kN; ++i) reinterpret_cast<Pack<T, kPer> *>(at)[i] = p[i];
     }
+    // the piece to shared memory, asynchronously
+    static __device__ __forceinline__ void copy(unsigned char *dst, const T *at) {
+        constexpr int kBytes = kPer * sizeof(T);
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(
+                             (uint32_t)__cvta_generic_to_shared(dst + i * kBytes)),
+                         "l"(at + i * kPer), "n"(kBytes < 4 ? 4 : kBytes)
+                         : "memory");
+    }
     __device__ __forceinline__ float get(int i) const { return to_f<T>(p[i / kPer].v[i % kPer]); }
     __device__ __forceinline__ void set(int i, float v) { p[i / kPer].v[i % kPer] = from_f<T>(v); }
 };
@@ -84,8 +96,13 @@ __device__ __forceinline__ float block_sum(float v, float *buf) {
     return s;
 }
 
+constexpr int kRowsAhead = 2;  // 1 where the memory of two rows is more than an SM has
+
 template <typename T, typename R, typename W, int VEC, int NV, int THREADS>
 __global__ void __launch_bounds__(THREADS) block_norm_kernel(const NormArgs a) {
+    constexpr bool kAsync = VEC * sizeof(T) >= 4;
+    constexpr int kPieceT = VEC * sizeof(T), kPieceR = VEC * sizeof(R);
+    extern __shared__ __align__(16) unsigned char rows[];  // [ahead][y, residual][NV][threads]
     __shared__ float sums[2][32];
     const int units = a.cols / VEC;
     const T *y = reinterpret_cast<const T *>(a.y);
@@ -95,16 +112,47 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(const NormArgs a) {
     T *normed = reinterpret_cast<T *>(a.normed);
     R *res_out = reinterpret_cast<R *>(a.residual_out);
     const float inv_cols = 1.f / (float)a.cols;
+    const int slot_bytes = NV * blockDim.x * (kPieceT + kPieceR);
+    unsigned char *my_y = rows + threadIdx.x * kPieceT, *my_r = rows + NV * blockDim.x * kPieceT + threadIdx.x * kPieceR;
+    auto copy_row = [&](int64_t row, int slot) {
+        if (row < a.rows)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = threadIdx.x + i * blockDim.x;
+                if (c >= units) break;
+                Piece<T, VEC>::copy(my_y + slot * slot_bytes + i * blockDim.x * kPieceT, y + row * a.y_stride + c * VEC);
+                Piece<R, VEC>::copy(my_r + slot * slot_bytes + i * blockDim.x * kPieceR,
+                                    res + row * a.res_stride + c * VEC);
+            }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if (kAsync)
+        for (int i = 0; i < a.ahead; ++i) copy_row(blockIdx.x + (int64_t)i * gridDim.x, i);
+    int slot = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         Piece<T, VEC> py[NV];
         Piece<R, VEC> pr[NV];
+        if (kAsync) {
+            if (a.ahead == kRowsAhead)
+                asm volatile("cp.async.wait_group %0;" ::"n"(kRowsAhead - 1) : "memory");
+            else
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+        }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = threadIdx.x + i * blockDim.x;
-            if (c < units) {
+            if (c >= units) continue;
+            if (kAsync) {
+                py[i].load(reinterpret_cast<const T *>(my_y + slot * slot_bytes + i * blockDim.x * kPieceT));
+                pr[i].load(reinterpret_cast<const R *>(my_r + slot * slot_bytes + i * blockDim.x * kPieceR));
+            } else {
                 py[i].load(y + row * a.y_stride + c * VEC);
                 pr[i].load(res + row * a.res_stride + c * VEC);
             }
+        }
+        if (kAsync) {
+            copy_row(row + (int64_t)a.ahead * gridDim.x, slot);
+            slot = slot + 1 == a.ahead ? 0 : slot + 1;
         }
         const float token_gate =
             a.gate_kind == WISP_GATE_TOKEN ? a.scale * to_f<T>(gate[row * a.gate_stride]) : a.scale;
@@ -162,16 +210,33 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(const NormArgs a) {
         }
         if (!post) __syncthreads();  // sums[1] of this row is read before the next row's sum goes there
     }
+    if (kAsync) asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 template <typename T, typename R, typename W, int VEC, int NV, int THREADS>
-int launch(const NormArgs &a, cudaStream_t stream) {
+int launch(NormArgs a, cudaStream_t stream) {
+    constexpr bool kAsync = VEC * sizeof(T) >= 4;
     const int units = a.cols / VEC;
     const int threads = ((units + NV - 1) / NV + 31) / 32 * 32;
+    const size_t row_bytes = (size_t)NV * threads * VEC * (sizeof(T) + sizeof(R));
+    a.ahead = row_bytes * kRowsAhead <= 200 * 1024 ? kRowsAhead : 1;
+    const size_t smem = kAsync ? a.ahead * row_bytes : 0;
     auto kernel = block_norm_kernel<T, R, W, VEC, NV, THREADS>;
-    // more CTAs than an SM holds: the next row starts when one ends
-    const int64_t most = 148 * 64;
-    kernel<<<(unsigned)(a.rows < most ? a.rows : most), threads, 0, stream>>>(a);
+    int dev = 0, sms = 0, per = 0;
+    WISP_CUDA_TRY(cudaGetDevice(&dev));
+    if (a.rows > 148) {
+        WISP_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+        if (smem > 48 * 1024)
+            WISP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        WISP_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, smem));
+        // without copies ahead, the next row starts when a CTA ends
+        if (!kAsync) per *= 8;
+    } else if (smem > 48 * 1024) {
+        WISP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    }
+    const int64_t most = (int64_t)sms * per;
+    const unsigned grid = (unsigned)(a.rows <= 148 || a.rows < most ? a.rows : most);
+    kernel<<<grid, threads, smem, stream>>>(a);
     WISP_CUDA_TRY(cudaGetLastError());
     return WISP_OK;
 }
@@ -236,7 +301,7 @@ extern "C" int wisp_block_norm(const void *y, int64_t y_stride, const void *resi
     if (rows > 1 && (y_stride < 0 || residual_stride < 0 || gate_stride < 0))
         return set_error("wisp_block_norm: negative stride"), WISP_ERR_INVALID;
     const NormArgs a{y,    residual,        pre_weight, post_weight, gate, normed, residual_out, rows, y_stride,
-                     residual_stride, gate_stride, cols,       gate_kind,   scale, eps};
+                     residual_stride, gate_stride, cols,       gate_kind,   scale, eps, 0};
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (dtype == WISP_BF16) return dispatch_types<__nv_bfloat16>(a, residual_dtype, weight_dtype, s);
     if (dtype == WISP_FP16) return dispatch_types<__half>(a, residual_dtype, weight_dtype, s);

@@ -14,7 +14,7 @@ import functools
 import torch
 
 from . import _lib
-from ._device import DTYPES, need_cuda, need_out, on, same_device, stream_of
+from ._device import DTYPES, cuda_index, launch, need_out, same_device
 
 BLOCK = 32
 
@@ -59,6 +59,13 @@ class Mx4Tensor:
         return f"Mx4Tensor(shape={tuple(self.shape)}, device={self.device})"
 
 
+def _new(codes: torch.Tensor, scales: torch.Tensor) -> Mx4Tensor:
+    """An Mx4Tensor of tensors made here: nothing to check."""
+    t = Mx4Tensor.__new__(Mx4Tensor)
+    t.codes, t.scales = codes, scales
+    return t
+
+
 def mx4_quantize(x: torch.Tensor, out: Mx4Tensor | None = None) -> Mx4Tensor:
     """``x [..., K]`` (bf16, fp16 or fp32) to MXFP4 (``wisp_mx4_quantize``).
 
@@ -66,49 +73,46 @@ def mx4_quantize(x: torch.Tensor, out: Mx4Tensor | None = None) -> Mx4Tensor:
     to the nearest E2M1 value, ties to even, saturating at 6.  A block with an infinity or a NaN reads back as NaN; a
     block of zeros has scale byte 0.  Rows may lie apart (``x`` two-dimensional, its last axis contiguous and every
     row on a 16-byte boundary); anything else is made contiguous first."""
-    dev = need_cuda("x", x)
+    index = cuda_index("x", x)
     dt = DTYPES.get(x.dtype)
     if dt is None:
         raise TypeError(f"x must be bf16, fp16 or fp32; got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % BLOCK:
-        raise ValueError(f"the last axis of x must be a multiple of {BLOCK}; got shape {tuple(x.shape)}")
-    cols = x.shape[-1]
-    size = x.element_size()
-    if x.is_contiguous():
-        stride = cols
-    elif x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= cols and x.stride(0) * size % 16 == 0:
-        stride = x.stride(0)
-    else:
-        x, stride = x.contiguous(), cols
-    if x.data_ptr() % 16:
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] == 0 or shape[-1] % BLOCK:
+        raise ValueError(f"the last axis of x must be a multiple of {BLOCK}; got shape {tuple(shape)}")
+    cols = stride = shape[-1]
+    if not x.is_contiguous():
+        if len(shape) == 2 and x.stride(1) == 1 and x.stride(0) >= cols and x.stride(0) * x.element_size() % 16 == 0:
+            stride = x.stride(0)
+        else:
+            x = x.contiguous()
+    ptr = x.data_ptr()
+    if ptr % 16:
         x, stride = x.clone(memory_format=torch.contiguous_format), cols
-    lead = x.shape[:-1]
+        ptr = x.data_ptr()
+    lead = shape[:-1]
     if out is None:
-        out = Mx4Tensor.__new__(Mx4Tensor)
-        out.codes = torch.empty((*lead, cols // 2), dtype=torch.uint8, device=dev)
-        out.scales = torch.empty((*lead, cols // BLOCK), dtype=torch.uint8, device=dev)
+        out = _new(x.new_empty((*lead, cols // 2), dtype=torch.uint8), x.new_empty((*lead, cols // BLOCK), dtype=torch.uint8))
     else:
-        need_out("out.codes", out.codes, (*lead, cols // 2), torch.uint8, dev)
-        need_out("out.scales", out.scales, (*lead, cols // BLOCK), torch.uint8, dev)
-    with on(dev):
-        _lib.check(_lib.lib().wisp_mx4_quantize(x.data_ptr(), dt, x.numel() // cols, cols, stride,
-                                                out.codes.data_ptr(), out.scales.data_ptr(), stream_of(dev)),
-                   "mx4_quantize")
+        need_out("out.codes", out.codes, (*lead, cols // 2), torch.uint8, index)
+        need_out("out.scales", out.scales, (*lead, cols // BLOCK), torch.uint8, index)
+    launch("wisp_mx4_quantize", index, ptr, dt, x.numel() // cols, cols, stride, out.codes.data_ptr(),
+           out.scales.data_ptr())
     return out
 
 
 def mx4_dequantize(q: Mx4Tensor, dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
     """The values of ``q`` (``wisp_mx4_dequantize``) as bf16 or fp32 (exact) or fp16 (rounded once where it cannot
     hold them)."""
-    dev = need_cuda("q", q.codes)
+    codes = q.codes
+    index = cuda_index("q", codes)
     dt = DTYPES.get(dtype)
     if dt is None:
         raise TypeError(f"dtype must be bf16, fp16 or fp32; got {dtype}")
-    shape = (*q.codes.shape[:-1], 2 * q.codes.shape[-1])
-    out = torch.empty(shape, dtype=dtype, device=dev) if out is None else need_out("out", out, shape, dtype, dev)
-    with on(dev):
-        _lib.check(_lib.lib().wisp_mx4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), out.numel() // shape[-1],
-                                                  shape[-1], out.data_ptr(), dt, stream_of(dev)), "mx4_dequantize")
+    shape = (*codes.shape[:-1], 2 * codes.shape[-1])
+    out = codes.new_empty(shape, dtype=dtype) if out is None else need_out("out", out, shape, dtype, index)
+    launch("wisp_mx4_dequantize", index, codes.data_ptr(), q.scales.data_ptr(), out.numel() // shape[-1], shape[-1],
+           out.data_ptr(), dt)
     return out
 
 
@@ -120,7 +124,7 @@ def mx4_matmul(a: Mx4Tensor, w: Mx4Tensor, offsets: torch.Tensor | None = None,
     on the device): rows ``offsets[g]`` to ``offsets[g + 1]`` times ``w[g]`` transposed, the products of MoE experts
     over rows sorted by expert.  Returns ``[M, N]`` bf16 (fp32 accumulation, one rounding).  Rows behind the last
     offset are left as they are in ``out`` (undefined in a new tensor)."""
-    dev = need_cuda("a", a.codes)
+    index = cuda_index("a", a.codes)
     if a.codes.dim() != 2 or w.codes.dim() not in (2, 3) or w.codes.shape[-1] != a.codes.shape[1]:
         raise ValueError(f"a is [M, K], w [N, K] or [G, N, K]; got {tuple(a.shape)} and {tuple(w.shape)}")
     rows, half = a.codes.shape
@@ -134,21 +138,18 @@ def mx4_matmul(a: Mx4Tensor, w: Mx4Tensor, offsets: torch.Tensor | None = None,
         op = offsets.data_ptr()
     elif groups != 1:
         raise ValueError(f"{groups} groups need offsets")
-    same_device(dev, w=w, offsets=offsets)
-    out = (torch.empty((rows, n), dtype=torch.bfloat16, device=dev) if out is None
-           else need_out("out", out, (rows, n), torch.bfloat16, dev))
-    with on(dev):
-        _lib.check(_lib.lib().wisp_mx4_matmul(
-            a.codes.data_ptr(), a.scales.data_ptr(), rows, w.codes.data_ptr(), w.scales.data_ptr(), groups, n, 2 * half,
-            op, out.data_ptr(), stream_of(dev)), "mx4_matmul")
+    same_device(index, w=w.codes, offsets=offsets)
+    out = (a.codes.new_empty((rows, n), dtype=torch.bfloat16) if out is None
+           else need_out("out", out, (rows, n), torch.bfloat16, index))
+    launch("wisp_mx4_matmul", index, a.codes.data_ptr(), a.scales.data_ptr(), rows, w.codes.data_ptr(),
+           w.scales.data_ptr(), groups, n, 2 * half, op, out.data_ptr())
     return out
 
 
 def mx4_synchronize(device: torch.device | None = None) -> None:
     """Wait for the device's current stream and raise if a bounded wait inside an :func:`mx4_matmul` ran out."""
-    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    with on(dev):
-        _lib.check(_lib.lib().wisp_mx4_sync(stream_of(dev)), "mx4_synchronize")
+    index = None if device is None else torch.device(device).index
+    launch("wisp_mx4_sync", torch.cuda.current_device() if index is None else index)
 
 
 MOE_MAX_TOKENS = 64
@@ -174,7 +175,7 @@ def mx4_moe(x: torch.Tensor, w13: Mx4Tensor, w2: Mx4Tensor, top_k: int | None = 
     ``topk_ids [T, k]`` (int32 or int64).  ``expert_map [E]`` (int32) gives each expert's slot, the row of ``w13`` and
     ``w2`` it lies in (a paged layer's ``expert_map_device``); without it the slot is the id.  Ids outside ``[0, E)``
     and experts without a slot contribute nothing.  Returns ``[T, H]`` bf16."""
-    dev = need_cuda("x", x)
+    index = cuda_index("x", x)
     if x.dtype != torch.bfloat16:
         raise TypeError(f"mx4_moe computes from bf16 activations; got {x.dtype}")
     if x.dim() != 2 or w13.codes.dim() != 3 or w2.codes.dim() != 3:
@@ -186,7 +187,7 @@ def mx4_moe(x: torch.Tensor, w13: Mx4Tensor, w2: Mx4Tensor, top_k: int | None = 
     if tokens > MOE_MAX_TOKENS:
         raise ValueError(f"mx4_moe takes at most {MOE_MAX_TOKENS} tokens a call; got {tokens} (mx4_quantize and "
                          "mx4_matmul serve longer ones)")
-    same_device(dev, w13=w13, w2=w2, router=router, topk_weights=topk_weights, topk_ids=topk_ids,
+    same_device(index, w13=w13.codes, w2=w2.codes, router=router, topk_weights=topk_weights, topk_ids=topk_ids,
                 expert_map=expert_map)
     experts = slots if expert_map is None else expert_map.numel()
     if expert_map is not None and (expert_map.dtype != torch.int32 or not expert_map.is_contiguous()):
@@ -213,16 +214,14 @@ def mx4_moe(x: torch.Tensor, w13: Mx4Tensor, w2: Mx4Tensor, top_k: int | None = 
         ip, wp, ids64 = topk_ids.data_ptr(), topk_weights.data_ptr(), int(topk_ids.dtype == torch.int64)
     if x.stride(1) != 1 or (tokens > 1 and (x.stride(0) < hidden or x.stride(0) % 8)) or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
-    out = (torch.empty((tokens, hidden), dtype=torch.bfloat16, device=dev) if out is None
-           else need_out("out", out, (tokens, hidden), torch.bfloat16, dev))
+    out = (x.new_empty((tokens, hidden)) if out is None
+           else need_out("out", out, (tokens, hidden), torch.bfloat16, index))
     need = _moe_workspace(tokens, experts, top_k, hidden, inter2 // 2)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with on(dev):
-        _lib.check(_lib.lib().wisp_mx4_moe(
-            x.data_ptr(), x.stride(0), rp, ip, ids64, wp, None if expert_map is None else expert_map.data_ptr(),
-            w13.codes.data_ptr(), w13.scales.data_ptr(), w2.codes.data_ptr(), w2.scales.data_ptr(), slots, tokens,
-            experts, top_k, hidden, inter2 // 2, int(renormalize), ws.data_ptr(), need, out.data_ptr(),
-            stream_of(dev)), "mx4_moe")
+    ws = x.new_empty(need, dtype=torch.uint8)
+    launch("wisp_mx4_moe", index, x.data_ptr(), x.stride(0), rp, ip, ids64, wp,
+           None if expert_map is None else expert_map.data_ptr(), w13.codes.data_ptr(), w13.scales.data_ptr(),
+           w2.codes.data_ptr(), w2.scales.data_ptr(), slots, tokens, experts, top_k, hidden, inter2 // 2,
+           int(renormalize), ws.data_ptr(), need, out.data_ptr())
     return out
 
 

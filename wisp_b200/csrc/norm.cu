@@ -15,8 +15,12 @@
 // The weights, which every row shares, stay in L1.  A thread's pieces of a row
 // are VEC values wide: 8 where the width and every address allow 16-byte
 // accesses, else 2, else 1 (2-byte pieces have no asynchronous copy and are
-// loaded where they are used); NV of them, so that a row takes 256 threads or
-// fewer where it can (more rows in flight, fewer warps in a reduction).
+// loaded where they are used); NV of them, so that a row takes 256 threads
+// where it can (more rows in flight, fewer warps in a reduction).  Threads and
+// pieces are constants of the kernel, which makes every address of a row one
+// register and a constant: with 2-value pieces the instructions, not the
+// memory, set the time (8191 rows of 2050: 80 us with the number of threads a
+// variable, 935 instructions a warp and row).
 #include <type_traits>
 
 #include "mx4.cuh"
@@ -85,49 +89,58 @@ struct Piece {
 
 // Sum over the block, the same in every thread.  Two buffers in turn: a
 // thread that is already at the next sum does not overwrite this one.
+template <int WARPS>
 __device__ __forceinline__ float block_sum(float v, float *buf) {
     v = warp_sum(v);
-    const int warps = (blockDim.x + 31) >> 5;
-    if (warps == 1) return v;
+    if (WARPS == 1) return v;
     if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
     __syncthreads();
     float s = 0.f;
-    for (int w = 0; w < warps; ++w) s += buf[w];
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) s += buf[w];
     return s;
 }
 
 constexpr int kRowsAhead = 2;  // 1 where the memory of two rows is more than an SM has
 
-template <typename T, typename R, typename W, int VEC, int NV, int THREADS>
+template <typename T, typename R, typename W, int VEC, int THREADS, int NV>
 __global__ void __launch_bounds__(THREADS) block_norm_kernel(const NormArgs a) {
     constexpr bool kAsync = VEC * sizeof(T) >= 4;
     constexpr int kPieceT = VEC * sizeof(T), kPieceR = VEC * sizeof(R);
     extern __shared__ __align__(16) unsigned char rows[];  // [ahead][y, residual][NV][threads]
     __shared__ float sums[2][32];
-    const int units = a.cols / VEC;
-    const T *y = reinterpret_cast<const T *>(a.y);
-    const R *res = reinterpret_cast<const R *>(a.residual);
-    const W *pre = reinterpret_cast<const W *>(a.pre), *post = reinterpret_cast<const W *>(a.post);
-    const T *gate = reinterpret_cast<const T *>(a.gate);
-    T *normed = reinterpret_cast<T *>(a.normed);
-    R *res_out = reinterpret_cast<R *>(a.residual_out);
+    constexpr int kStep = THREADS * VEC;  // values between a thread's pieces
+    constexpr int kSlotBytes = NV * THREADS * (kPieceT + kPieceR);
+    const int col = threadIdx.x * VEC, mine = a.cols - col;  // piece i is in the row where mine > i * kStep
+    const T *y = reinterpret_cast<const T *>(a.y) + col;
+    const R *res = reinterpret_cast<const R *>(a.residual) + col;
+    const W *pre = reinterpret_cast<const W *>(a.pre) + col, *post = reinterpret_cast<const W *>(a.post) + col;
+    const T *gate = reinterpret_cast<const T *>(a.gate) + (a.gate_kind >= WISP_GATE_CHANNEL ? col : 0);
+    T *normed = reinterpret_cast<T *>(a.normed) + col;
+    R *res_out = reinterpret_cast<R *>(a.residual_out) + col;
+    const bool has_post = a.post != nullptr;
     const float inv_cols = 1.f / (float)a.cols;
-    const int slot_bytes = NV * blockDim.x * (kPieceT + kPieceR);
-    unsigned char *my_y = rows + threadIdx.x * kPieceT, *my_r = rows + NV * blockDim.x * kPieceT + threadIdx.x * kPieceR;
+    unsigned char *my_y = rows + threadIdx.x * kPieceT, *my_r = rows + NV * THREADS * kPieceT + threadIdx.x * kPieceR;
     auto copy_row = [&](int64_t row, int slot) {
-        if (row < a.rows)
+        if (row < a.rows) {
+            const T *py = y + row * a.y_stride;
+            const R *pr = res + row * a.res_stride;
+            unsigned char *sy = my_y + slot * kSlotBytes, *sr = my_r + slot * kSlotBytes;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = threadIdx.x + i * blockDim.x;
-                if (c >= units) break;
-                Piece<T, VEC>::copy(my_y + slot * slot_bytes + i * blockDim.x * kPieceT, y + row * a.y_stride + c * VEC);
-                Piece<R, VEC>::copy(my_r + slot * slot_bytes + i * blockDim.x * kPieceR,
-                                    res + row * a.res_stride + c * VEC);
-            }
+            for (int i = 0; i < NV; ++i)
+                if (mine > i * kStep) {
+                    Piece<T, VEC>::copy(sy + i * THREADS * kPieceT, py + i * kStep);
+                    Piece<R, VEC>::copy(sr + i * THREADS * kPieceR, pr + i * kStep);
+                }
+        }
         asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto token_gate_of = [&](int64_t row) {
+        return a.gate_kind == WISP_GATE_TOKEN && row < a.rows ? a.scale * to_f<T>(gate[row * a.gate_stride]) : a.scale;
     };
     if (kAsync)
         for (int i = 0; i < a.ahead; ++i) copy_row(blockIdx.x + (int64_t)i * gridDim.x, i);
+    float next_gate = token_gate_of(blockIdx.x);
     int slot = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         Piece<T, VEC> py[NV];
@@ -138,52 +151,51 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(const NormArgs a) {
             else
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
+        {
+            const T *sy = kAsync ? reinterpret_cast<const T *>(my_y + slot * kSlotBytes) : y + row * a.y_stride;
+            const R *sr = kAsync ? reinterpret_cast<const R *>(my_r + slot * kSlotBytes) : res + row * a.res_stride;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = threadIdx.x + i * blockDim.x;
-            if (c >= units) continue;
-            if (kAsync) {
-                py[i].load(reinterpret_cast<const T *>(my_y + slot * slot_bytes + i * blockDim.x * kPieceT));
-                pr[i].load(reinterpret_cast<const R *>(my_r + slot * slot_bytes + i * blockDim.x * kPieceR));
-            } else {
-                py[i].load(y + row * a.y_stride + c * VEC);
-                pr[i].load(res + row * a.res_stride + c * VEC);
-            }
+            for (int i = 0; i < NV; ++i)
+                if (mine > i * kStep) {
+                    py[i].load(sy + i * kStep);
+                    pr[i].load(sr + i * kStep);
+                }
         }
         if (kAsync) {
             copy_row(row + (int64_t)a.ahead * gridDim.x, slot);
             slot = slot + 1 == a.ahead ? 0 : slot + 1;
         }
-        const float token_gate =
-            a.gate_kind == WISP_GATE_TOKEN ? a.scale * to_f<T>(gate[row * a.gate_stride]) : a.scale;
+        const float token_gate = next_gate;
+        next_gate = token_gate_of(row + gridDim.x);
         float rms = 1.f;
-        if (post) {
+        if (has_post) {
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (threadIdx.x + i * blockDim.x < units)
+                if (mine > i * kStep)
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) sum += py[i].get(j) * py[i].get(j);
-            rms = rsqrtf(block_sum(sum, sums[0]) * inv_cols + a.eps);
+            rms = rsqrtf(block_sum<THREADS / 32>(sum, sums[0]) * inv_cols + a.eps);
         }
         float r[NV][VEC];
         float sum = 0.f;
+        R *ro_row = res_out + row * a.cols;
+        const T *gate_row = gate + (a.gate_kind == WISP_GATE_FULL ? row * a.gate_stride : 0);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = threadIdx.x + i * blockDim.x;
-            if (c >= units) continue;
+            if (mine <= i * kStep) continue;
             float z[VEC];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) z[j] = py[i].get(j);
-            if (post) {
+            if (has_post) {
                 Piece<W, VEC> w;
-                w.load(post + c * VEC);
+                w.load(post + i * kStep);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) z[j] *= rms * w.get(j);
             }
             if (a.gate_kind >= WISP_GATE_CHANNEL) {
                 Piece<T, VEC> g;
-                g.load(gate + (a.gate_kind == WISP_GATE_FULL ? row * a.gate_stride : 0) + c * VEC);
+                g.load(gate_row + i * kStep);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) z[j] *= g.get(j);
             }
@@ -194,41 +206,39 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(const NormArgs a) {
                 sum += r[i][j] * r[i][j];
                 ro.set(j, r[i][j]);
             }
-            ro.store(res_out + row * a.cols + c * VEC);
+            ro.store(ro_row + i * kStep);
         }
-        rms = rsqrtf(block_sum(sum, sums[1]) * inv_cols + a.eps);
+        rms = rsqrtf(block_sum<THREADS / 32>(sum, sums[1]) * inv_cols + a.eps);
+        T *no_row = normed + row * a.cols;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = threadIdx.x + i * blockDim.x;
-            if (c >= units) continue;
+            if (mine <= i * kStep) continue;
             Piece<W, VEC> w;
-            w.load(pre + c * VEC);
+            w.load(pre + i * kStep);
             Piece<T, VEC> no;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) no.set(j, r[i][j] * rms * w.get(j));
-            no.store(normed + row * a.cols + c * VEC);
+            no.store(no_row + i * kStep);
         }
-        if (!post) __syncthreads();  // sums[1] of this row is read before the next row's sum goes there
+        if (!has_post) __syncthreads();  // sums[1] of this row is read before the next row's sum goes there
     }
     if (kAsync) asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <typename T, typename R, typename W, int VEC, int NV, int THREADS>
+template <typename T, typename R, typename W, int VEC, int THREADS, int NV>
 int launch(NormArgs a, cudaStream_t stream) {
     constexpr bool kAsync = VEC * sizeof(T) >= 4;
-    const int units = a.cols / VEC;
-    const int threads = ((units + NV - 1) / NV + 31) / 32 * 32;
-    const size_t row_bytes = (size_t)NV * threads * VEC * (sizeof(T) + sizeof(R));
+    const size_t row_bytes = (size_t)NV * THREADS * VEC * (sizeof(T) + sizeof(R));
     a.ahead = row_bytes * kRowsAhead <= 200 * 1024 ? kRowsAhead : 1;
     const size_t smem = kAsync ? a.ahead * row_bytes : 0;
-    auto kernel = block_norm_kernel<T, R, W, VEC, NV, THREADS>;
+    auto kernel = block_norm_kernel<T, R, W, VEC, THREADS, NV>;
     int dev = 0, sms = 0, per = 0;
     WISP_CUDA_TRY(cudaGetDevice(&dev));
     if (a.rows > 148) {
         WISP_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
         if (smem > 48 * 1024)
             WISP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        WISP_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, smem));
+        WISP_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, THREADS, smem));
         // without copies ahead, the next row starts when a CTA ends
         if (!kAsync) per *= 8;
     } else if (smem > 48 * 1024) {
@@ -236,7 +246,7 @@ int launch(NormArgs a, cudaStream_t stream) {
     }
     const int64_t most = (int64_t)sms * per;
     const unsigned grid = (unsigned)(a.rows <= 148 || a.rows < most ? a.rows : most);
-    kernel<<<grid, threads, smem, stream>>>(a);
+    kernel<<<grid, THREADS, smem, stream>>>(a);
     WISP_CUDA_TRY(cudaGetLastError());
     return WISP_OK;
 }
@@ -255,19 +265,24 @@ int dispatch(const NormArgs &a, cudaStream_t stream) {
                 ok(a.gate, a.gate_kind == WISP_GATE_FULL ? a.gate_stride : 0, sizeof(T))) &&
                ok(a.normed, a.cols, sizeof(T)) && ok(a.residual_out, a.cols, sizeof(R));
     };
+    const int cols = a.cols;
     if (fits(8)) {
-        if (a.cols <= 8 * 256) return launch<T, R, W, 8, 1, 256>(a, stream);
-        if (a.cols <= 8 * 512) return launch<T, R, W, 8, 2, 256>(a, stream);
-        return launch<T, R, W, 8, 2, 1024>(a, stream);
+        if (cols <= 8 * 64) return launch<T, R, W, 8, 64, 1>(a, stream);
+        if (cols <= 8 * 256) return launch<T, R, W, 8, 256, 1>(a, stream);
+        if (cols <= 8 * 512) return launch<T, R, W, 8, 256, 2>(a, stream);
+        return launch<T, R, W, 8, 1024, 2>(a, stream);
     }
     if (fits(2)) {
-        if (a.cols <= 2 * 512) return launch<T, R, W, 2, 2, 256>(a, stream);
-        if (a.cols <= 2 * 2048) return launch<T, R, W, 2, 8, 256>(a, stream);
-        return launch<T, R, W, 2, 8, 1024>(a, stream);
+        if (cols <= 2 * 256) return launch<T, R, W, 2, 64, 4>(a, stream);
+        if (cols <= 2 * 768) return launch<T, R, W, 2, 256, 3>(a, stream);
+        if (cols <= 2 * 1280) return launch<T, R, W, 2, 256, 5>(a, stream);
+        if (cols <= 2 * 2048) return launch<T, R, W, 2, 256, 8>(a, stream);
+        return launch<T, R, W, 2, 1024, 8>(a, stream);
     }
-    if (a.cols <= 1024) return launch<T, R, W, 1, 4, 256>(a, stream);
-    if (a.cols <= 4096) return launch<T, R, W, 1, 16, 256>(a, stream);
-    return launch<T, R, W, 1, 16, 1024>(a, stream);
+    if (cols <= 512) return launch<T, R, W, 1, 64, 8>(a, stream);
+    if (cols <= 2048) return launch<T, R, W, 1, 256, 8>(a, stream);
+    if (cols <= 4096) return launch<T, R, W, 1, 256, 16>(a, stream);
+    return launch<T, R, W, 1, 1024, 16>(a, stream);
 }
 
 template <typename T>

@@ -62,7 +62,7 @@ def test_matches_oracle(rows, cols, post, gate):
 
 @pytest.mark.parametrize("dtype,rdtype,wdtype", [(BF, FP, BF), (BF, BF, FP), (BF, FP, FP), (HF, HF, HF), (HF, FP, FP),
                                                  (HF, HF, FP), (HF, FP, HF), (FP, FP, FP)])
-@pytest.mark.parametrize("cols", [2048, 2050, 4099])
+@pytest.mark.parametrize("cols", [2048, 2050, 4096, 4094, 4099, 16384])
 def test_types(dtype, rdtype, wdtype, cols):
     run(*inputs(9, cols, dtype, rdtype, wdtype, True, "full"))
 

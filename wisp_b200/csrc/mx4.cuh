@@ -46,15 +46,11 @@ __device__ __forceinline__ uint32_t f32x8_to_e2m1(const float (&v)[8]) {
     return r;
 }
 
-// Eight consecutive values, widened to fp32 (exact) / rounded once from fp32.
+// Eight consecutive values, rounded once from fp32.
 template <typename T>
 struct Vec8;
 template <>
 struct Vec8<float> {
-    static __device__ __forceinline__ void load(const float *p, float (&v)[8]) {
-        const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    }
     static __device__ __forceinline__ void store(float *p, const float (&v)[8]) {
         reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
         reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -62,11 +58,6 @@ struct Vec8<float> {
 };
 template <>
 struct Vec8<__nv_bfloat16> {
-    static __device__ __forceinline__ void load(const __nv_bfloat16 *p, float (&v)[8]) {
-        const uint4 a = ld_cached16(p);
-        v[0] = bf16lo(a.x), v[1] = bf16hi(a.x), v[2] = bf16lo(a.y), v[3] = bf16hi(a.y);
-        v[4] = bf16lo(a.z), v[5] = bf16hi(a.z), v[6] = bf16lo(a.w), v[7] = bf16hi(a.w);
-    }
     static __device__ __forceinline__ void store(__nv_bfloat16 *p, const float (&v)[8]) {
         uint4 a;
         __nv_bfloat162 h[4];
@@ -78,16 +69,6 @@ struct Vec8<__nv_bfloat16> {
 };
 template <>
 struct Vec8<__half> {
-    static __device__ __forceinline__ void load(const __half *p, float (&v)[8]) {
-        const uint4 a = ld_cached16(p);
-        __half2 h[4];
-        memcpy(h, &a, 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(h[i]);
-            v[2 * i] = f.x, v[2 * i + 1] = f.y;
-        }
-    }
     static __device__ __forceinline__ void store(__half *p, const float (&v)[8]) {
         uint4 a;
         __half2 h[4];

@@ -11,7 +11,9 @@
 // Bound by HBM: 2.53 bytes a bf16 value each way.  Four threads share a
 // block: each holds 8 values (one 16-byte load of 16-bit types), the maximum
 // takes two shuffles, and the codes leave as one 32-bit store a thread, so a
-// warp's loads and stores are whole lines.
+// warp's loads and stores are whole lines.  The values stay as loaded until
+// they are rounded: widened at once they took twice the registers, and the
+// loads in flight of half as many threads.
 #include "mx4.cuh"
 
 namespace wisp {
@@ -21,48 +23,103 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;  // 8-value pieces of a thread: loads in flight
 
-__device__ __forceinline__ uint32_t quantize_piece(const float (&v)[8], uint32_t &byte) {
-    // |x| compared as integers: NaN above infinity above every number
-    uint32_t m = 0;
+// Eight values as they were loaded; the largest magnitude as fp32 bits with
+// NaN above infinity above every number.  16-bit types compare two values an
+// instruction and are widened only when they are rounded.
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<float> {
+    uint4 a, b;
+    __device__ __forceinline__ void load(const float *p) {
+        a = ld_stream16(p), b = ld_stream16(p + 4);
+    }
+    __device__ __forceinline__ void zero() { a = b = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ uint32_t block_max() const {
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-    const uint32_t field = m >> 23;
-    byte = field == 255 ? 255 : field > 2 ? field - 2 : 0;
-    if (byte == 255) return 0;
-    const float inv = __uint_as_float((254 - byte) << 23);  // 2^(127 - byte) = 2^-s
-    float q[8];
+        for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+        return max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+    }
+    __device__ __forceinline__ void widen(float (&v)[8]) const {
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = v[i] * inv;
-    return f32x8_to_e2m1(q);
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+    }
+};
+template <typename T2>
+__device__ __forceinline__ T2 as2(uint32_t w) {
+    T2 r;
+    memcpy(&r, &w, 4);
+    return r;
 }
+template <typename T, typename T2>
+struct Raw8x16 {
+    uint4 a;
+    __device__ __forceinline__ void load(const T *p) { a = ld_stream16(p); }
+    __device__ __forceinline__ void zero() { a = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ T2 pair_max() const {
+        T2 m = __hmax2_nan(__hmax2_nan(__habs2(as2<T2>(a.x)), __habs2(as2<T2>(a.y))),
+                           __hmax2_nan(__habs2(as2<T2>(a.z)), __habs2(as2<T2>(a.w))));
+        m = __hmax2_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+        return __hmax2_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+    }
+};
+template <>
+struct Raw8<__nv_bfloat16> : Raw8x16<__nv_bfloat16, __nv_bfloat162> {
+    __device__ __forceinline__ uint32_t block_max() const {
+        const __nv_bfloat162 m = pair_max();
+        return __float_as_uint(__bfloat162float(__hmax_nan(m.x, m.y)));
+    }
+    __device__ __forceinline__ void widen(float (&v)[8]) const {
+        v[0] = bf16lo(a.x), v[1] = bf16hi(a.x), v[2] = bf16lo(a.y), v[3] = bf16hi(a.y);
+        v[4] = bf16lo(a.z), v[5] = bf16hi(a.z), v[6] = bf16lo(a.w), v[7] = bf16hi(a.w);
+    }
+};
+template <>
+struct Raw8<__half> : Raw8x16<__half, __half2> {
+    __device__ __forceinline__ uint32_t block_max() const {
+        const __half2 m = pair_max();
+        return __float_as_uint(__half2float(__hmax_nan(m.x, m.y)));
+    }
+    __device__ __forceinline__ void widen(float (&v)[8]) const {
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(as2<__half2>(w[i]));
+            v[2 * i] = f.x, v[2 * i + 1] = f.y;
+        }
+    }
+};
 
 // Piece p of the matrix: columns 8 (p % (cols / 8)) .. of row p / (cols / 8).
-template <typename T>
+template <typename T, bool CONTIGUOUS>
 __global__ void __launch_bounds__(kThreads)
     quantize_kernel(const T *x, int64_t pieces, int64_t cols, int64_t row_stride, uint32_t *codes, uint8_t *scales) {
     const int64_t first = (int64_t)blockIdx.x * kThreads * kUnroll + threadIdx.x;
-    float v[kUnroll][8];
+    Raw8<T> v[kUnroll];
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
         const int64_t p = first + i * kThreads;
-        if (p < pieces) {
-            int64_t at = p * 8;
-            if (row_stride != cols) at = at / cols * row_stride + at % cols;
-            Vec8<T>::load(x + at, v[i]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-        }
+        if (p < pieces)
+            v[i].load(x + (CONTIGUOUS ? p * 8 : p * 8 / cols * row_stride + p * 8 % cols));
+        else
+            v[i].zero();
     }
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
         const int64_t p = first + i * kThreads;
-        uint32_t byte;
-        const uint32_t c = quantize_piece(v[i], byte);
+        const uint32_t field = v[i].block_max() >> 23;
+        const uint32_t byte = field == 255 ? 255 : field > 2 ? field - 2 : 0;
+        const float inv = __uint_as_float((254 - byte) << 23);  // 2^(127 - byte) = 2^-s
+        float f[8];
+        v[i].widen(f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] *= inv;
         if (p < pieces) {
-            codes[p] = c;
+            codes[p] = byte == 255 ? 0 : f32x8_to_e2m1(f);
             if ((p & 3) == 0) scales[p >> 2] = (uint8_t)byte;
         }
     }
@@ -127,12 +184,20 @@ extern "C" int wisp_mx4_quantize(const void *x, int32_t dtype, int64_t rows, int
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     uint32_t *c = reinterpret_cast<uint32_t *>(codes);
     uint8_t *b = reinterpret_cast<uint8_t *>(scales);
+    const auto run = [&](auto zero) {
+        using T = decltype(zero);
+        const T *in = reinterpret_cast<const T *>(x);
+        if (row_stride == cols)
+            quantize_kernel<T, true><<<grid, kThreads, 0, s>>>(in, pieces, cols, row_stride, c, b);
+        else
+            quantize_kernel<T, false><<<grid, kThreads, 0, s>>>(in, pieces, cols, row_stride, c, b);
+    };
     if (dtype == WISP_BF16)
-        quantize_kernel<<<grid, kThreads, 0, s>>>(reinterpret_cast<const __nv_bfloat16 *>(x), pieces, cols, row_stride, c, b);
+        run(__nv_bfloat16());
     else if (dtype == WISP_FP16)
-        quantize_kernel<<<grid, kThreads, 0, s>>>(reinterpret_cast<const __half *>(x), pieces, cols, row_stride, c, b);
+        run(__half());
     else
-        quantize_kernel<<<grid, kThreads, 0, s>>>(reinterpret_cast<const float *>(x), pieces, cols, row_stride, c, b);
+        run(float());
     WISP_CUDA_TRY(cudaGetLastError());
     return WISP_OK;
 }

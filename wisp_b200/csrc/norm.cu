@@ -236,12 +236,12 @@ int launch(NormArgs a, cudaStream_t stream) {
     WISP_CUDA_TRY(cudaGetDevice(&dev));
     if (a.rows > 148) {
         WISP_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-        if (smem > 48 * 1024)
+        if (smem > 47 * 1024)
             WISP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         WISP_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, THREADS, smem));
         // without copies ahead, the next row starts when a CTA ends
         if (!kAsync) per *= 8;
-    } else if (smem > 48 * 1024) {
+    } else if (smem > 47 * 1024) {
         WISP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     }
     const int64_t most = (int64_t)sms * per;

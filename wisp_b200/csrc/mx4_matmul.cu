@@ -12,12 +12,12 @@
 // stage have to fit 512 columns of tensor memory; of the widths that do, a
 // wider tile reads A less often.
 //
-// Ten warps: TMA producer (5 stages of 256 values of K: 16 KB of A, 24 KB of
-// W), MMA issuer, 4 epilogue warps, 4 warps that bring the scale bytes.  These
+// 14 warps: TMA producer (5 stages of 256 values of K: 16 KB of A, 24 KB of
+// W), MMA issuer, 4 epilogue warps, 8 warps that bring the scale bytes.  These
 // lie row by row in memory (the layout of the checkpoint, which paging copies
 // as it is), 8 bytes of a row a stage, and go to the scale atoms of shared
-// memory through registers, four stages ahead of their use; no TMA box can
-// make that arrangement.
+// memory through registers, ahead of their use; no TMA box can make that
+// arrangement.
 //
 // Bound by HBM for few rows a group (the weights are read once), for many by
 // L2: a stage brings 40 KB for 4 instructions of 96 cycles each.
@@ -39,9 +39,8 @@ constexpr int kSfCols = 24;                    // of a stage: two halves of 4 (A
 constexpr int kSfCol0 = 2 * kTileN;            // behind the two accumulators
 static_assert(kSfCol0 + kStages * kSfCols <= 512, "tensor memory");
 constexpr int kTmemCols = 512;
-constexpr int kThreads = 320;
 constexpr int kEpiWarp = 2, kSfWarp = 6;
-constexpr int kSfThreads = 128;
+constexpr int kThreads = (kSfWarp + kScaleGroups * kScaleGroupWarps) * 32;
 constexpr int kMaxGroups = 1024;
 
 struct MatmulArgs {
@@ -50,7 +49,7 @@ struct MatmulArgs {
     __nv_bfloat16 *out;
     int64_t rows;
     int *status;
-    int groups, N, blocks, a_align, w_align, vec_out;
+    int groups, N, blocks, align, vec_out;
 };
 
 struct Control {
@@ -157,20 +156,20 @@ __device__ void load_operands(Control &C, unsigned char *stages, const CUtensorM
         }
 }
 
+template <int WINDOW, int DEEP>
 __device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulArgs &a, int steps) {
-    constexpr int kDeep = 4;  // stages whose scale bytes are in registers
-    const int tid = threadIdx.x - kSfWarp * 32;
+    const int group = (threadIdx.x >> 5) - kSfWarp >= kScaleGroupWarps;
+    const int tid = threadIdx.x % (kScaleGroupWarps * 32);
     volatile int *abort = &C.abort;
     const int64_t wrows = (int64_t)a.groups * a.N;
     unsigned char *sf = stages + kABytes + kBBytes + atom_at(tid);
     RingPos<kStages> ring;
-    // the loads run kDeep steps ahead of the stores
+    // the loads run DEEP of the group's windows ahead of the stores
     Walk ahead(C, a);
     bool more = ahead.at(C, a);
     int kb = 0;
-    const uint8_t *pa = nullptr, *pw[2] = {};  // of step kb
+    const uint8_t *pa = nullptr, *pw[2] = {};  // rows of the tile
     auto point = [&] {
-        kb = 0;
         const int64_t ra = ahead.row0 + tid;
         pa = ra < a.rows ? a.a_scales + ra * a.blocks : nullptr;
 #pragma unroll
@@ -179,52 +178,61 @@ __device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulA
             pw[i] = tid + i * 128 < kTileN && rw < wrows ? a.w_scales + rw * a.blocks : nullptr;
         }
     };
-    // nothing here may wait for what it loads: the values are used kDeep steps later
-    auto load = [&](uint2 &x, uint2 (&y)[2], bool &valid) {
-        valid = more;
-        if (!more) return;
-        const int left = a.blocks - kb * kStepBlocks;
-        x = y[0] = y[1] = make_uint2(0, 0);
-        if (pa) {
-            x = load_scales(pa, left, a.a_align);
-            pa += kStepBlocks;
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (pw[i]) {
-                y[i] = load_scales(pw[i], left, a.w_align);
-                pw[i] += kStepBlocks;
-            }
-        if (++kb == steps) {
+    auto advance = [&](int windows) {
+        bool moved = false;
+        for (int i = 0; i < windows && more; ++i) {
+            kb += WINDOW;
+            if (kb < steps) continue;
+            kb = 0, moved = true;
             ahead.next();
             more = ahead.at(C, a);
-            if (more) point();
         }
+        if (moved && more) point();
+    };
+    struct Window {
+        uint2 a[WINDOW], w[2][WINDOW];
+        bool valid;
+    } buf[DEEP];
+    auto load = [&](Window &x) {
+        x.valid = more;
+        if (!more) return;
+        const int left = a.blocks - kb * kStepBlocks;
+#pragma unroll
+        for (int i = 0; i < WINDOW; ++i) x.a[i] = x.w[0][i] = x.w[1][i] = make_uint2(0, 0);
+        if (pa) load_window<WINDOW>(x.a, pa + kb * kStepBlocks, left, a.align);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (pw[i]) load_window<WINDOW>(x.w[i], pw[i] + kb * kStepBlocks, left, a.align);
+        advance(kScaleGroups);
     };
     if (more) point();
-    uint2 va[kDeep], vw[kDeep][2];
-    bool valid[kDeep];
+    advance(group);
+    ring.skip(group * WINDOW);
 #pragma unroll
-    for (int i = 0; i < kDeep; ++i) load(va[i], vw[i], valid[i]);
+    for (int i = 0; i < DEEP; ++i) load(buf[i]);
     while (true) {
 #pragma unroll
-        for (int i = 0; i < kDeep; ++i) {
-            if (!valid[i]) return;
-            if (!warp_wait(&C.empty[ring.slot], ring.turn ^ 1, abort, a.status)) return;
-            unsigned char *sfa = sf + ring.slot * kStageBytes, *sfw = sfa + kSfABytes;
-            *reinterpret_cast<uint32_t *>(sfa) = va[i].x;
-            *reinterpret_cast<uint32_t *>(sfa + kAtomBytes) = va[i].y;
-            *reinterpret_cast<uint32_t *>(sfw) = vw[i][0].x;
-            *reinterpret_cast<uint32_t *>(sfw + 2 * kAtomBytes) = vw[i][0].y;
-            if (tid < kTileN - 128) {
-                *reinterpret_cast<uint32_t *>(sfw + kAtomBytes) = vw[i][1].x;
-                *reinterpret_cast<uint32_t *>(sfw + 3 * kAtomBytes) = vw[i][1].y;
+        for (int i = 0; i < DEEP; ++i) {
+            if (!buf[i].valid) return;
+#pragma unroll
+            for (int j = 0; j < WINDOW; ++j) {
+                if (!warp_wait(&C.empty[ring.slot], ring.turn ^ 1, abort, a.status)) return;
+                unsigned char *sfa = sf + ring.slot * kStageBytes, *sfw = sfa + kSfABytes;
+                *reinterpret_cast<uint32_t *>(sfa) = buf[i].a[j].x;
+                *reinterpret_cast<uint32_t *>(sfa + kAtomBytes) = buf[i].a[j].y;
+                *reinterpret_cast<uint32_t *>(sfw) = buf[i].w[0][j].x;
+                *reinterpret_cast<uint32_t *>(sfw + 2 * kAtomBytes) = buf[i].w[0][j].y;
+                if (tid < kTileN - 128) {
+                    *reinterpret_cast<uint32_t *>(sfw + kAtomBytes) = buf[i].w[1][j].x;
+                    *reinterpret_cast<uint32_t *>(sfw + 3 * kAtomBytes) = buf[i].w[1][j].y;
+                }
+                fence_async_shared();
+                __syncwarp();
+                if ((tid & 31) == 0) mbar_arrive(&C.sf_full[ring.slot]);
+                ring.next();
             }
-            fence_async_shared();
-            __syncwarp();
-            if ((tid & 31) == 0) mbar_arrive(&C.sf_full[ring.slot]);
-            ring.next();
-            load(va[i], vw[i], valid[i]);
+            ring.skip((kScaleGroups - 1) * WINDOW);
+            load(buf[i]);
         }
     }
 }
@@ -316,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&C.full[s], 1);
-            mbar_init(&C.sf_full[s], kSfThreads / 32);
+            mbar_init(&C.sf_full[s], kScaleGroupWarps);
             mbar_init(&C.empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -340,8 +348,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (elect_one()) umma_commit(&C.mma_done);
     } else if (warp < kSfWarp) {
         store_tiles(C, a);
+    } else if (a.align == kWideAlign) {
+        load_all_scales<kWideWindow, 2>(C, stages, a, steps);
     } else {
-        load_all_scales(C, stages, a, steps);
+        load_all_scales<1, 4>(C, stages, a, steps);
     }
     __syncwarp();
     tc_fence_before();
@@ -407,7 +417,8 @@ extern "C" int wisp_mx4_matmul(const void *a_codes, const void *a_scales, int64_
     a.out = reinterpret_cast<__nv_bfloat16 *>(out);
     a.rows = rows, a.groups = groups, a.N = n, a.blocks = k / kBlock;
     if (const int rc = status_word(&a.status)) return rc;
-    a.a_align = scale_align(a_scales, a.blocks), a.w_align = scale_align(w_scales, a.blocks);
+    const int aa = scale_align(a_scales, a.blocks), wa = scale_align(w_scales, a.blocks);
+    a.align = aa < wa ? aa : wa;
     a.vec_out = n % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
     int dev = 0, sms = 0;
     WISP_CUDA_TRY(cudaGetDevice(&dev));

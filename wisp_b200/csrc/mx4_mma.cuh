@@ -71,6 +71,10 @@ struct RingPos {
     __device__ __forceinline__ void next() {
         if (++slot == STAGES) slot = 0, turn ^= 1;
     }
+    __device__ __forceinline__ void skip(int n) {  // n <= STAGES
+        slot += n;
+        if (slot >= STAGES) slot -= STAGES, turn ^= 1;
+    }
 };
 // Scale atom: 32 rows of 16 bytes, groups of 8 rows 128 bytes apart, no swizzle.
 __device__ __forceinline__ uint64_t smem_desc_atom(uint32_t saddr) {
@@ -110,27 +114,71 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
     return __all_sync(0xFFFFFFFFu, wait_or_abort(bar, parity, abort, status));
 }
 
-// The eight scale bytes of a row in a stage, of which `left` are the row's (the
-// others: 0).  `align`: what the rows' scale bytes are aligned to.
-__device__ __forceinline__ uint2 load_scales(const uint8_t *p, int left, int align) {
-    if (align >= 8) return __ldg(reinterpret_cast<const uint2 *>(p));
-    uint2 v = make_uint2(0, 0);
+// The scale bytes come in windows of WINDOW stages.  The rows of a tile lie in
+// as many lines of the cache, so a load instruction of 32 rows costs 32 lookups
+// whatever it brings: where the rows are 32-byte aligned, a window is four
+// stages and one 256-bit load of a row; else one stage and a load of 8 bytes
+// or less.  Two groups of four warps take the windows in turn, so that one
+// stores while the other loads.  (One group with 8-byte loads needed 1000
+// cycles a stage, twice what the products of a stage take.)
+constexpr int kWideWindow = 4;
+constexpr int kWideAlign = kWideWindow * kStepBlocks;
+constexpr int kScaleGroups = 2, kScaleGroupWarps = 4;
+
+// The first `left` of eight scale bytes; what lies behind a row's last block is
+// not a scale.
+__device__ __forceinline__ uint2 first_bytes(uint2 v, int left) {
+    if (left < 8) {
+        const uint64_t keep = (1ull << (8 * left)) - 1;
+        v.x &= (uint32_t)keep, v.y &= (uint32_t)(keep >> 32);
+    }
+    return v;
+}
+// A window's scale bytes of a row; `left` of them are the row's (the others:
+// 0, or what lies there for values that first_bytes() will see).  `align`:
+// what the rows are aligned to.  NC: through the read-only path.  Nothing here
+// waits for what it loads.
+template <int WINDOW, bool NC = true>
+__device__ __forceinline__ void load_window(uint2 (&v)[WINDOW], const uint8_t *p, int left, int align) {
+    if (WINDOW == kWideWindow) {
+        uint32_t r[8];
+        if (NC)
+            asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                         : "l"(p));
+        else
+            asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                         : "l"(p)
+                         : "memory");
+#pragma unroll
+        for (int i = 0; i < WINDOW; ++i) v[i] = make_uint2(r[2 * i], r[2 * i + 1]);
+        return;
+    }
+    if (!NC) {
+        v[0] = __ldcg(reinterpret_cast<const uint2 *>(p));
+        return;
+    }
+    if (align >= 8) {
+        v[0] = __ldg(reinterpret_cast<const uint2 *>(p));
+        return;
+    }
+    v[0] = make_uint2(0, 0);
     if (align >= 4) {
-        v.x = __ldg(reinterpret_cast<const uint32_t *>(p));
-        if (left > 4) v.y = __ldg(reinterpret_cast<const uint32_t *>(p) + 1);
-        return v;
+        v[0].x = __ldg(reinterpret_cast<const uint32_t *>(p));
+        if (left > 4) v[0].y = __ldg(reinterpret_cast<const uint32_t *>(p) + 1);
+        return;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if (i < left) v.x |= (uint32_t)__ldg(p + i) << (8 * i);
-        if (i + 4 < left) v.y |= (uint32_t)__ldg(p + i + 4) << (8 * i);
+        if (i < left) v[0].x |= (uint32_t)__ldg(p + i) << (8 * i);
+        if (i + 4 < left) v[0].y |= (uint32_t)__ldg(p + i + 4) << (8 * i);
     }
-    return v;
 }
 // What a matrix's rows of scale bytes are aligned to.
 __host__ __device__ inline int scale_align(const void *scales, int blocks) {
     const uintptr_t p = reinterpret_cast<uintptr_t>(scales) | (uintptr_t)blocks;
-    return p % 8 == 0 ? 8 : p % 4 == 0 ? 4 : 1;
+    return p % kWideAlign == 0 ? kWideAlign : p % 8 == 0 ? 8 : p % 4 == 0 ? 4 : 1;
 }
 
 }  // namespace mx4

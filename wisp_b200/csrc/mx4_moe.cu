@@ -22,7 +22,7 @@
 // hundred instructions that 128 columns of 16 rows take.)
 //
 // Bound by HBM: a few tokens use every byte of a routed expert once.  A
-// cooperative launch of one CTA of ten warps per SM runs
+// cooperative launch of one CTA of 14 warps per SM runs
 //   R  router products (a warp per expert row and token group), x to terms
 //   S  (after a grid barrier, every CTA for itself) top-k and the lists of
 //      each expert's tokens in groups of at most 16
@@ -36,8 +36,8 @@
 //      atomics, the same bits every run
 // In G and D a warp each feeds a ring of 5 stages of 256 values of K (weights
 // by TMA, the terms by bulk copies of 1 KB a token, laid out by their writers
-// as the swizzle wants them) and issues the products, four bring the scale
-// bytes to shared memory four stages ahead, four read the accumulators.
+// as the swizzle wants them) and issues the products, eight bring the scale
+// bytes (mx4_mma.cuh), four read the accumulators.
 #include <cooperative_groups.h>
 
 #include "mx4_mma.cuh"
@@ -48,15 +48,14 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kWarps = 10;
+constexpr int kEpiWarp = 2, kSfWarp = 6;       // four warps and two groups of four; 0: copies, 1: products
+constexpr int kWarps = kSfWarp + kScaleGroups * kScaleGroupWarps;
 constexpr int kThreads = kWarps * 32;
-constexpr int kEpiWarp = 2, kSfWarp = 6;       // four warps each; 0: copies, 1: products
 constexpr int kTerms = 6;                      // terms of an activation
 constexpr int kRows = 8;                       // rows of a token in the small operand
 constexpr int kGroup = 16;                     // tokens of a tile
 constexpr int kStages = 5;
 constexpr int kTermBytes = kRows * 128;        // terms of a token in a stage
-constexpr int kScaleBytes = kRows * kStepBlocks;
 constexpr int kABytes = 128 * 128, kBBytes = kGroup * kTermBytes;
 constexpr int kStageBytes = kABytes + kBBytes + 4 * kAtomBytes;
 constexpr int kAccCols = kGroup * kRows;       // of an accumulator; two of them
@@ -80,7 +79,7 @@ struct MoeArgs {
     const uint8_t *s13, *s2;
     __nv_bfloat16 *out;
     float *logits;                // [T][E]
-    uint8_t *xq, *xs;             // terms of x: [T][steps][kTermBytes], scales [T][steps][kScaleBytes]
+    uint8_t *xq, *xs;             // terms of x: [T][steps][kTermBytes], scales [T][kRows][steps * 8]
     uint8_t *aq, *as;             // terms of silu(g) u: the same for each pair
     float *y;                     // [split][T * k][H]
     int *status;
@@ -113,8 +112,8 @@ struct Control {
 // ---- phase R ------------------------------------------------------------------
 // One block of 32 values, one a lane, as terms: codes to `codes` (16 bytes of
 // row 0, rows 128 bytes apart, 16-byte pieces swizzled by the row) and scale
-// bytes to `scales` (rows kStepBlocks apart).
-__device__ __forceinline__ void write_terms(float v, uint8_t *codes, uint8_t *scales, int piece, int lane) {
+// bytes to `scales` (rows `stride` apart).
+__device__ __forceinline__ void write_terms(float v, uint8_t *codes, uint8_t *scales, int stride, int piece, int lane) {
     for (int q = 0; q < kTerms; ++q) {
         const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v) & 0x7FFFFFFFu);
         const int e = (int)(m >> 23);
@@ -134,7 +133,7 @@ __device__ __forceinline__ void write_terms(float v, uint8_t *codes, uint8_t *sc
         w |= __shfl_down_sync(0xFFFFFFFFu, w, 4) << 16;
         if ((lane & 7) == 0)
             *reinterpret_cast<uint32_t *>(codes + q * 128 + ((piece ^ q) << 4) + (lane >> 3) * 4) = w;
-        if (lane == 0) scales[q * kStepBlocks] = (uint8_t)byte;
+        if (lane == 0) scales[q * stride] = (uint8_t)byte;
     }
 }
 
@@ -143,8 +142,9 @@ __device__ void convert_tokens(const MoeArgs &a, int gw, int nw, int lane) {
     for (int u = gw; u < a.T * blocks; u += nw) {
         const int t = u / blocks, b = u - t * blocks, kb = b / kStepBlocks, piece = b % kStepBlocks;
         const float v = __bfloat162float(a.x[t * a.x_stride + b * kBlock + lane]);
-        write_terms(v, a.xq + ((size_t)t * steps + kb) * kTermBytes,
-                    a.xs + ((size_t)t * steps + kb) * kScaleBytes + piece, piece, lane);
+        const int stride = steps * kStepBlocks;
+        write_terms(v, a.xq + ((size_t)t * steps + kb) * kTermBytes, a.xs + (size_t)t * kRows * stride + b, stride, piece,
+                    lane);
     }
 }
 
@@ -440,78 +440,93 @@ __device__ int copy_early(Control &C, unsigned char *stages, const Phase &ph, co
     return early;
 }
 
-// The first `left` of eight scale bytes; what lies behind a row's last block is
-// not a scale.
-__device__ __forceinline__ uint2 first_bytes(uint2 v, int left) {
-    if (left < 8) {
-        const uint64_t keep = (1ull << (8 * left)) - 1;
-        v.x &= (uint32_t)keep, v.y &= (uint32_t)(keep >> 32);
-    }
-    return v;
-}
-
+template <int WINDOW, int DEEP>
 __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, const Lists &L, Cursor &cur, int *status) {
-    constexpr int kDeep = 4;  // stages whose scale bytes are in registers
-    const int tid = threadIdx.x - kSfWarp * 32;
+    const int group = (threadIdx.x >> 5) - kSfWarp >= kScaleGroupWarps;
+    const int tid = threadIdx.x - (kSfWarp + group * kScaleGroupWarps) * 32;
     volatile int *abort = &C.abort;
     unsigned char *sf = stages + kABytes + kBBytes + atom_at(tid);
-    // the loads run kDeep steps ahead of the stores
+    // the loads run DEEP of the group's windows ahead of the stores
     Walk ahead(ph);
     bool more = ahead.at(ph, L, C);
     int kb = 0;
-    const uint8_t *pw = nullptr, *pb = nullptr;  // of step kb
+    const uint8_t *pw = nullptr, *pb = nullptr;  // rows of the tile
     auto point = [&] {
-        kb = ahead.kb0;
         const int64_t row = ahead.row + (tid < 64 ? tid : ph.second + tid - 64);
-        pw = row < ph.w_rows ? ph.w_scales + row * ph.blocks + kb * kStepBlocks : nullptr;
+        pw = row < ph.w_rows ? ph.w_scales + row * ph.blocks : nullptr;
         const int i = tid / kRows, q = tid % kRows;
         pb = i < ahead.n && q < kTerms
-                 ? ph.b_scales + ((size_t)(L.pair[ahead.off + i] / ph.token_div) * ph.steps + kb) * kScaleBytes +
-                       q * kStepBlocks
+                 ? ph.b_scales + ((size_t)(L.pair[ahead.off + i] / ph.token_div) * kRows + q) * (ph.steps * kStepBlocks)
                  : nullptr;
     };
-    // nothing here may wait for what it loads: the values are used kDeep steps later
-    auto load = [&](uint2 &x, uint2 &y, int &left) {
-        left = more ? ph.blocks - kb * kStepBlocks : 0;
-        if (!more) return;
-        x = y = make_uint2(0, 0);
-        if (pw) {
-            x = load_scales(pw, left, ph.align);
-            pw += kStepBlocks;
-        }
-        if (pb) {  // (written by this kernel: not through the read-only path)
-            y = __ldcg(reinterpret_cast<const uint2 *>(pb));
-            pb += kScaleBytes;
-        }
-        if (++kb == ahead.kb1) {
+    auto advance = [&](int windows) {
+        bool moved = false;
+        for (int i = 0; i < windows && more; ++i) {
+            kb += WINDOW;
+            if (kb < ahead.kb1) continue;
+            moved = true;
             ahead.next();
             more = ahead.at(ph, L, C);
-            if (more) point();
+            kb = ahead.kb0;
         }
+        if (moved && more) point();
     };
-    if (more) point();
-    uint2 vw[kDeep], vb[kDeep];
-    int left[kDeep];
+    struct Window {
+        uint2 w[WINDOW], b[WINDOW];
+        int left;  // scale bytes of a row from here on, 0: no window
+    } buf[DEEP];
+    auto load = [&](Window &x) {
+        x.left = more ? ph.blocks - kb * kStepBlocks : 0;
+        if (!more) return;
 #pragma unroll
-    for (int i = 0; i < kDeep; ++i) load(vw[i], vb[i], left[i]);
+        for (int i = 0; i < WINDOW; ++i) x.w[i] = x.b[i] = make_uint2(0, 0);
+        if (pw) load_window<WINDOW>(x.w, pw + kb * kStepBlocks, x.left, ph.align);
+        if (pb) load_window<WINDOW, false>(x.b, pb + kb * kStepBlocks, x.left, ph.align);  // written by this kernel
+        advance(kScaleGroups);
+    };
+    if (more) {
+        point();
+        kb = ahead.kb0;
+    }
+    advance(group);
+    RingPos<kStages> ring = cur.ring;
+    ring.skip(group * WINDOW);
+#pragma unroll
+    for (int i = 0; i < DEEP; ++i) load(buf[i]);
     while (true) {
 #pragma unroll
-        for (int i = 0; i < kDeep; ++i) {
-            if (left[i] <= 0) return;
-            if (!warp_wait(&C.empty[cur.ring.slot], cur.ring.turn ^ 1, abort, status)) return;
-            unsigned char *at = sf + cur.ring.slot * kStageBytes;
-            const uint2 terms = first_bytes(vb[i], left[i]);
-            *reinterpret_cast<uint32_t *>(at) = vw[i].x;
-            *reinterpret_cast<uint32_t *>(at + kAtomBytes) = vw[i].y;
-            *reinterpret_cast<uint32_t *>(at + 2 * kAtomBytes) = terms.x;
-            *reinterpret_cast<uint32_t *>(at + 3 * kAtomBytes) = terms.y;
-            fence_async_shared();
-            __syncwarp();
-            if ((tid & 31) == 0) mbar_arrive(&C.sf_full[cur.ring.slot]);
-            cur.ring.next();
-            load(vw[i], vb[i], left[i]);
+        for (int i = 0; i < DEEP; ++i) {
+            if (buf[i].left <= 0) return;
+#pragma unroll
+            for (int j = 0; j < WINDOW; ++j) {
+                if (!warp_wait(&C.empty[ring.slot], ring.turn ^ 1, abort, status)) return;
+                unsigned char *at = sf + ring.slot * kStageBytes;
+                const uint2 terms = first_bytes(buf[i].b[j], buf[i].left - j * kStepBlocks);
+                *reinterpret_cast<uint32_t *>(at) = buf[i].w[j].x;
+                *reinterpret_cast<uint32_t *>(at + kAtomBytes) = buf[i].w[j].y;
+                *reinterpret_cast<uint32_t *>(at + 2 * kAtomBytes) = terms.x;
+                *reinterpret_cast<uint32_t *>(at + 3 * kAtomBytes) = terms.y;
+                fence_async_shared();
+                __syncwarp();
+                if ((tid & 31) == 0) mbar_arrive(&C.sf_full[ring.slot]);
+                ring.next();
+            }
+            ring.skip((kScaleGroups - 1) * WINDOW);
+            load(buf[i]);
         }
     }
+}
+// Every group has to come to the phase's last ring position, whichever windows
+// were its own.
+__device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, const Lists &L, Cursor &cur, int *status) {
+    if (ph.align == kWideAlign)
+        run_scales<kWideWindow, 2>(C, stages, ph, L, cur, status);
+    else
+        run_scales<1, 4>(C, stages, ph, L, cur, status);
+    int total = 0;
+    for (Walk t(ph); t.at(ph, L, C); t.next()) total += t.kb1 - t.kb0;
+    for (; total >= kStages; total -= kStages) cur.ring.skip(kStages);
+    cur.ring.skip(total);
 }
 
 // The whole warp walks, one lane issues.
@@ -593,8 +608,9 @@ __device__ void run_gate_up(Control &C, const Phase &ph, const Lists &L, Cursor 
             for (int i = quarter >> 1; i < tile.n; i += 2) {
                 const float g = ex[i * 128 + (quarter & 1) * 32 + lane], u = ex[i * 128 + 64 + (quarter & 1) * 32 + lane];
                 const int p = L.pair[tile.off + i], kb = j0 / kStepK, piece = j0 / kBlock % kStepBlocks;
+                const int stride = steps_out * kStepBlocks;
                 write_terms(g / (1.f + __expf(-g)) * u, a.aq + ((size_t)p * steps_out + kb) * kTermBytes,
-                            a.as + ((size_t)p * steps_out + kb) * kScaleBytes + piece, piece, lane);
+                            a.as + (size_t)p * kRows * stride + j0 / kBlock, stride, piece, lane);
             }
         epilogue_barrier();
     }
@@ -651,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&C.full[s], 1);
-            mbar_init(&C.sf_full[s], 4);
+            mbar_init(&C.sf_full[s], kScaleGroupWarps);
             mbar_init(&C.empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -709,10 +725,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     down.map = &map2, down.w_scales = a.s2, down.b_codes = a.aq, down.b_scales = a.as;
     down.blocks = a.I / kBlock, down.steps = (down.blocks + kStepBlocks - 1) / kStepBlocks, down.align = a.s2_align;
     down.groups = L.n, down.m_tiles = (a.H + 127) / 128, down.rows_m = 128;
-    down.split = choose_split(L.n * down.m_tiles, down.steps, a.max_split);
+    down.split = choose_split(L.n * down.m_tiles, down.align == kWideAlign ? down.steps / kWideWindow : down.steps,
+                              a.max_split);
     down.slot_rows = a.H, down.second = 64, down.w_rows = (int64_t)a.slots * a.H, down.token_div = 1;
 
-    if (tid <= down.split) C.cut[tid] = tid * down.steps / down.split;
+    // pieces of D begin at whole windows of scale bytes
+    const int cut = tid * down.steps / max(down.split, 1);
+    if (tid <= down.split) C.cut[tid] = down.align == kWideAlign ? cut / kWideWindow * kWideWindow : cut;
     __syncthreads();
 
     // G
@@ -785,9 +804,9 @@ struct Workspace {
         const size_t up = (H + kStepK - 1) / kStepK, down = (I + kStepK - 1) / kStepK, P = (size_t)T * k;
         logits = take((size_t)T * E * 4);
         xq = take(T * up * kTermBytes);
-        xs = take(T * up * kScaleBytes);
+        xs = take(T * up * kRows * kStepBlocks);
         aq = take(P * down * kTermBytes);
-        as = take(P * down * kScaleBytes);
+        as = take(P * down * kRows * kStepBlocks);
         split = (int)(down < kMaxSplit ? down : kMaxSplit);
         y = take((size_t)split * P * H * 4);
         bytes = at;

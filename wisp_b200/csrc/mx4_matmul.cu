@@ -12,7 +12,7 @@
 // stage have to fit 512 columns of tensor memory; of the widths that do, a
 // wider tile reads A less often.
 //
-// 14 warps: TMA producer (5 stages of 256 values of K: 16 KB of A, 24 KB of
+// 14 warps: TMA producer (4 stages of 256 values of K: 16 KB of A, 24 KB of
 // W), MMA issuer, 4 epilogue warps, 8 warps that bring the scale bytes.  These
 // lie row by row in memory (the layout of the checkpoint, which paging copies
 // as it is), 8 bytes of a row a stage, and go to the scale atoms of shared
@@ -31,7 +31,7 @@ namespace {
 __device__ int g_status = 0;
 
 constexpr int kTileM = 128, kTileN = 192;
-constexpr int kStages = 5;
+constexpr int kStages = 4;
 constexpr int kABytes = kTileM * 128, kBBytes = kTileN * 128;
 constexpr int kSfABytes = 2 * kAtomBytes, kSfBBytes = 4 * kAtomBytes;  // [two halves of K][row atoms]
 constexpr int kStageBytes = kABytes + kBBytes + kSfABytes + kSfBBytes;
@@ -42,6 +42,7 @@ constexpr int kTmemCols = 512;
 constexpr int kEpiWarp = 2, kSfWarp = 6;
 constexpr int kThreads = (kSfWarp + kScaleGroups * kScaleGroupWarps) * 32;
 constexpr int kMaxGroups = 1024;
+constexpr int kOutBytes = 32 * 128;           // staging of an epilogue warp: 32 rows of 64 columns
 
 struct MatmulArgs {
     const int32_t *offsets;  // [groups + 1], or nullptr: one group of all rows
@@ -158,6 +159,7 @@ __device__ void load_operands(Control &C, unsigned char *stages, const CUtensorM
 
 template <int WINDOW, int DEEP>
 __device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulArgs &a, int steps) {
+    static_assert(kStages > WINDOW, "a parity wait has to know its phase");
     const int group = (threadIdx.x >> 5) - kSfWarp >= kScaleGroupWarps;
     const int tid = threadIdx.x % (kScaleGroupWarps * 32);
     volatile int *abort = &C.abort;
@@ -237,6 +239,9 @@ __device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulA
     }
 }
 
+// The whole warp walks, one lane issues.  While the unit works off three of a
+// stage's four products the warp waits for the next stage: the waits take as
+// long as two products even when there is nothing to wait for.
 __device__ void issue_products(Control &C, unsigned char *stages, const MatmulArgs &a, int steps) {
     volatile int *abort = &C.abort;
     const uint32_t base = s_addr(stages), tmem = C.tmem_base;
@@ -245,20 +250,28 @@ __device__ void issue_products(Control &C, unsigned char *stages, const MatmulAr
     RingPos<kStages> ring;
     RingPos<2> accs;
     int consumed = 0;
+    bool ready = false;  // whether the stage at `ring` has been waited for
+    auto wait_stage = [&](const RingPos<kStages> &at) {
+        return warp_wait(&C.full[at.slot], at.turn, abort, a.status) &&
+               warp_wait(&C.sf_full[at.slot], at.turn, abort, a.status);
+    };
     for (Walk t(C, a); t.at(C, a); t.next(), accs.next()) {
         if (!warp_wait(&C.acc_empty[accs.slot], accs.turn ^ 1, abort, a.status)) return;
         tc_fence_after();
         const uint32_t acc = tmem + accs.slot * kTileN;
-        for (int kb = 0; kb < steps; ++kb, ring.next()) {
-            const int s = ring.slot;
-            if (!warp_wait(&C.full[s], ring.turn, abort, a.status) ||
-                !warp_wait(&C.sf_full[s], ring.turn, abort, a.status))
-                return;
+        const bool last_tile = t.t + (int)gridDim.x >= t.tiles;
+        for (int kb = 0; kb < steps; ++kb) {
+            if (!ready && !wait_stage(ring)) return;
             tc_fence_after();
+            const int s = ring.slot;
             // addresses are in units of 16 bytes; 64 values are 32 bytes further along K
             const uint64_t step = (uint64_t)(s * (kStageBytes >> 4));
             const uint64_t da = a0 + step, db = b0 + step, ds = sf0 + step;
             const uint32_t cols = tmem + kSfCol0 + s * kSfCols;
+            auto product = [&](int kk) {
+                umma_mxf4(acc, da + kk * 2, db + kk * 2, idesc_mxf4(kTileM, kTileN, (kk & 1) * 2), cols + (kk >> 1) * 12,
+                          cols + (kk >> 1) * 12 + 4, kb | kk);
+            };
             if (elect_one()) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -266,47 +279,73 @@ __device__ void issue_products(Control &C, unsigned char *stages, const MatmulAr
                     copy_atom(cols + h * 12 + 4, ds + ((kSfABytes + h * 2 * kAtomBytes) >> 4));
                     copy_atom(cols + h * 12 + 8, ds + ((kSfABytes + (h * 2 + 1) * kAtomBytes) >> 4));
                 }
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                    umma_mxf4(acc, da + kk * 2, db + kk * 2, idesc_mxf4(kTileM, kTileN, (kk & 1) * 2),
-                              cols + (kk >> 1) * 12, cols + (kk >> 1) * 12 + 4, kb | kk);
+                product(0);
+                product(1);
+                product(2);
+            }
+            ring.next();
+            const bool more = kb + 1 < steps || !last_tile;
+            const bool ok = !more || wait_stage(ring);
+            ready = more;
+            if (elect_one()) {
+                product(3);
                 umma_commit(&C.empty[s]);
                 C.consumed = ++consumed;
             }
+            if (!ok) return;
         }
         if (elect_one()) umma_commit(&C.acc_full[accs.slot]);
     }
 }
 
-__device__ void store_tiles(Control &C, const MatmulArgs &a) {
+// Epilogue warps: 64 columns at a time through shared memory (16-byte pieces
+// swizzled by the row), so that a store instruction writes 128 bytes of four
+// rows and not 16 bytes of 32.
+__device__ void store_tiles(Control &C, unsigned char *staging, const MatmulArgs &a) {
     volatile int *abort = &C.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3;
+    unsigned char *mine = staging + (warp - kEpiWarp) * kOutBytes;
     RingPos<2> accs;
     for (Walk t(C, a); t.at(C, a); t.next(), accs.next()) {
         if (!warp_wait(&C.acc_full[accs.slot], accs.turn, abort, a.status)) return;
         tc_fence_after();
-        const int r = quarter * 32 + lane;
-        __nv_bfloat16 *row = a.out + ((int64_t)t.row0 + r) * a.N + t.n0;
-        const int cols = min(kTileN, a.N - t.n0);
+        const int rows = t.rows - quarter * 32, cols = min(kTileN, a.N - t.n0);
+        __nv_bfloat16 *out = a.out + ((int64_t)t.row0 + quarter * 32) * a.N + t.n0;
+        const uint32_t taddr = C.tmem_base + accs.slot * kTileN + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
-        for (int c0 = 0; c0 < kTileN; c0 += 32) {
-            uint32_t v[32];
-            gemm::tmem_ld32(C.tmem_base + accs.slot * kTileN + ((uint32_t)(quarter * 32) << 16) + c0, v);
-            if (r >= t.rows || c0 >= cols) continue;
-            if (a.vec_out) {
+        for (int c0 = 0; c0 < cols && rows > 0; c0 += 64) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t v[32];
+                gemm::tmem_ld32(taddr + c0 + h * 32, v);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if (c0 + j * 8 >= cols) break;
                     float f[8];
 #pragma unroll
                     for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(v[j * 8 + x]);
-                    Vec8<__nv_bfloat16>::store(row + c0 + j * 8, f);
+                    Vec8<__nv_bfloat16>::store(
+                        reinterpret_cast<__nv_bfloat16 *>(mine + lane * 128 + (((h * 4 + j) ^ (lane & 7)) << 4)), f);
                 }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (c0 + j < cols) row[c0 + j] = __float2bfloat16_rn(__uint_as_float(v[j]));
             }
+            __syncwarp();
+            const int c = c0 + (lane & 7) * 8;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + (lane >> 3);
+                const uint4 v = *reinterpret_cast<const uint4 *>(mine + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+                if (r >= rows || c >= cols) continue;
+                __nv_bfloat16 *at = out + (int64_t)r * a.N + c;
+                if (a.vec_out) {
+                    *reinterpret_cast<uint4 *>(at) = v;
+                } else {
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int x = 0; x < 8; ++x)
+                        if (c + x < cols)
+                            at[x] = __ushort_as_bfloat16((unsigned short)(x & 1 ? w[x / 2] >> 16 : w[x / 2]));
+                }
+            }
+            __syncwarp();
         }
         tc_fence_before();
         __syncwarp();
@@ -319,7 +358,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const MatmulArgs a) {
     extern __shared__ unsigned char raw[];
     unsigned char *stages = raw + ((1024u - (s_addr(raw) & 1023u)) & 1023u);
-    Control &C = *reinterpret_cast<Control *>(stages + kStages * kStageBytes);
+    unsigned char *staging = stages + kStages * kStageBytes;
+    Control &C = *reinterpret_cast<Control *>(staging + 4 * kOutBytes);
     const int tid = threadIdx.x, warp = tid >> 5;
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -347,9 +387,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (elect_one()) umma_commit(&C.mma_done);
     } else if (warp < kSfWarp) {
-        store_tiles(C, a);
+        store_tiles(C, staging, a);
     } else if (a.align == kWideAlign) {
-        load_all_scales<kWideWindow, 2>(C, stages, a, steps);
+        load_all_scales<kWideWindow, 3>(C, stages, a, steps);
     } else {
         load_all_scales<1, 4>(C, stages, a, steps);
     }
@@ -369,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 int *g_words[64] = {};  // address of g_status on each device
 
-constexpr int kSmemBytes = kStages * kStageBytes + 1024 + sizeof(Control);
+constexpr int kSmemBytes = kStages * kStageBytes + 4 * kOutBytes + 1024 + sizeof(Control);
 static_assert(kSmemBytes <= 232448, "shared memory");
 
 }  // namespace

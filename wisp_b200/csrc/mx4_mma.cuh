@@ -30,7 +30,7 @@ using gemm::umma_commit;
 constexpr int kStepK = 256;                 // values of K in a stage: 128 bytes a row
 constexpr int kStepBlocks = kStepK / kBlock;  // scale bytes of a row in a stage
 constexpr int kAtomBytes = 512;             // scales of 128 rows x 128 values
-constexpr uint32_t kTries = 1u << 26;       // limit of one wait
+constexpr uint32_t kTries = 1u << 22;       // limit of one wait
 
 // Device word of the kernels' sticky status on the current device (mx4_matmul.cu).
 int status_word(int **word);
@@ -94,8 +94,8 @@ __device__ __forceinline__ int atom_at(int r) { return (r & 31) * 16 + (r >> 5) 
 
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Bounded wait: kTries attempts (a second or more; reading a timer in the loop
-// would delay every wait that does not succeed at once).
+// Bounded wait: kTries attempts, each of which suspends the thread for a while
+// (seconds in all; no wait here is longer than a few memory latencies).
 __device__ __forceinline__ bool wait_tries(uint64_t *bar, uint32_t parity, const volatile int *abort) {
     for (uint32_t i = 1; !mbar_try(bar, parity); ++i)
         if (i % 256 == 0 && (*abort || i >= kTries)) return false;
@@ -116,12 +116,19 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
 
 // The scale bytes come in windows of WINDOW stages.  The rows of a tile lie in
 // as many lines of the cache, so a load instruction of 32 rows costs 32 lookups
-// whatever it brings: where the rows are 32-byte aligned, a window is four
-// stages and one 256-bit load of a row; else one stage and a load of 8 bytes
+// whatever it brings: where the rows are 16-byte aligned, a window is two
+// stages and one 16-byte load of a row; else one stage and a load of 8 bytes
 // or less.  Two groups of four warps take the windows in turn, so that one
 // stores while the other loads.  (One group with 8-byte loads needed 1000
 // cycles a stage, twice what the products of a stage take.)
-constexpr int kWideWindow = 4;
+//
+// A group passes over the other one's windows without waiting for their slots.
+// A parity wait tells a phase from the one before it, not from the one before
+// that, so when the group waits for stage k - STAGES to be released it has to
+// know that stage k - 2 STAGES was.  Its own stage before k is k - 1 - WINDOW
+// at the earliest, for which it saw k - 1 - WINDOW - STAGES released, and stages
+// are released in order: STAGES > WINDOW is enough.
+constexpr int kWideWindow = 2;
 constexpr int kWideAlign = kWideWindow * kStepBlocks;
 constexpr int kScaleGroups = 2, kScaleGroupWarps = 4;
 
@@ -141,18 +148,8 @@ __device__ __forceinline__ uint2 first_bytes(uint2 v, int left) {
 template <int WINDOW, bool NC = true>
 __device__ __forceinline__ void load_window(uint2 (&v)[WINDOW], const uint8_t *p, int left, int align) {
     if (WINDOW == kWideWindow) {
-        uint32_t r[8];
-        if (NC)
-            asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                         : "l"(p));
-        else
-            asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                         : "l"(p)
-                         : "memory");
-#pragma unroll
-        for (int i = 0; i < WINDOW; ++i) v[i] = make_uint2(r[2 * i], r[2 * i + 1]);
+        const uint4 r = NC ? __ldg(reinterpret_cast<const uint4 *>(p)) : ld_cg16(p);
+        v[0] = make_uint2(r.x, r.y), v[WINDOW - 1] = make_uint2(r.z, r.w);
         return;
     }
     if (!NC) {

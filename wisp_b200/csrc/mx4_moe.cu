@@ -442,6 +442,7 @@ __device__ int copy_early(Control &C, unsigned char *stages, const Phase &ph, co
 
 template <int WINDOW, int DEEP>
 __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, const Lists &L, Cursor &cur, int *status) {
+    static_assert(kStages > WINDOW, "a parity wait has to know its phase");
     const int group = (threadIdx.x >> 5) - kSfWarp >= kScaleGroupWarps;
     const int tid = threadIdx.x - (kSfWarp + group * kScaleGroupWarps) * 32;
     volatile int *abort = &C.abort;
@@ -520,7 +521,7 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
 // were its own.
 __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, const Lists &L, Cursor &cur, int *status) {
     if (ph.align == kWideAlign)
-        run_scales<kWideWindow, 2>(C, stages, ph, L, cur, status);
+        run_scales<kWideWindow, 3>(C, stages, ph, L, cur, status);
     else
         run_scales<1, 4>(C, stages, ph, L, cur, status);
     int total = 0;

@@ -84,6 +84,7 @@ struct MoeArgs {
     float *y;                     // [split][T * k][H]
     int *status;
     int T, E, k, H, I, slots, ids64, renormalize, s13_align, s2_align, max_split;
+    uint32_t inv_k;               // p / k = p * inv_k >> 16 for every pair p
 };
 
 // What the lists are built from; lies where the ring will be.
@@ -91,7 +92,7 @@ struct Scratch {
     int ids[kMaxPairs];              // expert of pair t * k + j, -1: none
     uint32_t tokens[kMaxExperts][2];  // the tokens routed to an expert, a bit each
     int begin[kMaxExperts];          // where its pairs begin, -1: no slot
-    int scan[kWarps];
+    int scan[2][kWarps];
 };
 struct Lists {
     float w[kMaxPairs];                // routing weight of a pair
@@ -195,50 +196,66 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
     return key == 1 ? NAN : __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
-// Top-k of token t by (logit descending, id ascending), softmax weights.  A
-// lane keeps its best key; only the lane that wins a round looks for its next.
-template <int PER_LANE>
-__device__ void route_token(const MoeArgs &a, Lists &L, Scratch &S, int t, int lane) {
-    const float *logits = a.logits + (size_t)t * a.E;
-    uint32_t key[PER_LANE], best = 0;
-    int at = 0, my_id = -1;
-    uint32_t mine = 0;
+// Top-k of tokens t, t + kWarps, .. (N of them, those behind the last are
+// left out) by (logit descending, id ascending), softmax weights.  Every CTA
+// does this for itself, so its latency counts: a round is two reductions of
+// the warp (the largest key, the lowest id that has it) without a branch, and
+// a warp's tokens go through their rounds together.
+template <int PER_LANE, int N>
+__device__ void route_tokens(const MoeArgs &a, Lists &L, Scratch &S, int t0, int lane) {
+    uint32_t key[N][PER_LANE], mine[N] = {};
+    int my_id[N] = {};
 #pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) {
-        const int e = i * 32 + lane;
-        key[i] = e < a.E ? key_of(__ldcg(logits + e)) : 0;
-        if (key[i] > best) best = key[i], at = i;
+    for (int n = 0; n < N; ++n) {
+        const float *logits = a.logits + (size_t)min(t0 + n * kWarps, a.T - 1) * a.E;
+#pragma unroll
+        for (int i = 0; i < PER_LANE; ++i) {
+            const int e = i * 32 + lane;
+            key[n][i] = e < a.E ? key_of(__ldcg(logits + e)) : 0;
+        }
     }
     for (int j = 0; j < a.k; ++j) {
-        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
-        unsigned who = __ballot_sync(0xFFFFFFFFu, best == top);
-        if (who & (who - 1)) {  // equal logits: the lowest id
-            const uint32_t low = __reduce_min_sync(0xFFFFFFFFu, best == top ? (uint32_t)(at * 32 + lane) : 0x7FFFFFFFu);
-            who = 1u << (low & 31);
-        }
-        const int winner = __ffs(who) - 1, id = __shfl_sync(0xFFFFFFFFu, at, winner) * 32 + winner;
-        if (lane == j) mine = top, my_id = id;
-        if (lane == winner) {
-            const int gone = at;
-            best = 0;
 #pragma unroll
-            for (int i = 0; i < PER_LANE; ++i) {
-                if (i == gone) key[i] = 0;
-                if (key[i] > best) best = key[i], at = i;
-            }
+        for (int n = 0; n < N; ++n) {
+            uint32_t best = 0;
+            int id = 0;
+#pragma unroll
+            for (int i = 0; i < PER_LANE; ++i)
+                if (key[n][i] > best) best = key[n][i], id = i * 32 + lane;
+            const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
+            id = (int)__reduce_min_sync(0xFFFFFFFFu, best == top ? (uint32_t)id : 0x7FFFFFFFu);
+#pragma unroll
+            for (int i = 0; i < PER_LANE; ++i) key[n][i] = i * 32 + lane == id ? 0 : key[n][i];
+            mine[n] = lane == j ? top : mine[n];
+            my_id[n] = lane == j ? id : my_id[n];
         }
     }
-    const float l = logit_of(mine), mx = __shfl_sync(0xFFFFFFFFu, l, 0);
-    float p = 0.f, all = 0.f;
-    if (lane < a.k) p = all = expf(l - mx);
-    if (!a.renormalize) {
-        all = 0.f;
-        for (int e = lane; e < a.E; e += 32) all += expf(__ldcg(logits + e) - mx);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int t = t0 + n * kWarps;
+        if (t >= a.T) break;
+        const float l = logit_of(mine[n]), mx = __shfl_sync(0xFFFFFFFFu, l, 0);
+        float p = 0.f, all = 0.f;
+        if (lane < a.k) p = all = expf(l - mx);
+        if (!a.renormalize) {
+            all = 0.f;
+            for (int e = lane; e < a.E; e += 32) all += expf(__ldcg(a.logits + (size_t)t * a.E + e) - mx);
+        }
+        const float sum = warp_sum(all);
+        if (lane < a.k) {
+            S.ids[t * a.k + lane] = my_id[n];
+            L.w[t * a.k + lane] = p / sum;
+        }
     }
-    const float sum = warp_sum(all);
-    if (lane < a.k) {
-        S.ids[t * a.k + lane] = my_id;
-        L.w[t * a.k + lane] = p / sum;
+}
+// All tokens of this warp, two at a time.
+template <int PER_LANE>
+__device__ void route_all(const MoeArgs &a, Lists &L, Scratch &S, int warp, int lane) {
+    for (int t = warp; t < a.T; t += 2 * kWarps) {
+        if (t + kWarps < a.T)
+            route_tokens<PER_LANE, 2>(a, L, S, t, lane);
+        else
+            route_tokens<PER_LANE, 1>(a, L, S, t, lane);
     }
 }
 
@@ -265,48 +282,37 @@ __device__ void given_token(const MoeArgs &a, Lists &L, Scratch &S, int t) {
 // expert's set of tokens, a bit each, gives count and rank whatever the order
 // in which the bits were set.
 __device__ void build_lists(const MoeArgs &a, Lists &L, Scratch &S) {
-    constexpr int kPer = (kMaxExperts + kThreads - 1) / kThreads;
     const int P = a.T * a.k, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     for (int p = tid; p < P; p += kThreads) {
-        const int e = S.ids[p], t = p / a.k;
+        const int e = S.ids[p], t = (int)(p * a.inv_k >> 16);
         if (e >= 0) atomicOr(&S.tokens[e][t >> 5], 1u << (t & 31));
     }
     __syncthreads();
-    int count[kPer], slot[kPer], own = 0;  // pairs in the low half of `own`, groups in the high half
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int e = tid * kPer + i;
-        count[i] = e < a.E ? __popc(S.tokens[e][0]) + __popc(S.tokens[e][1]) : 0;
-        if (!count[i]) continue;
-        slot[i] = a.expert_map ? a.expert_map[e] : e;
-        if (slot[i] < 0 || slot[i] >= a.slots) count[i] = 0;
-        own += count[i] + ((count[i] + kGroup - 1) / kGroup << 16);
-    }
-    int run = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xFFFFFFFFu, run, o);
-        if (lane >= o) run += v;
-    }
-    if (lane == 31) S.scan[warp] = run;
-    __syncthreads();
-    int before = run - own, total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        const int v = S.scan[w];
-        if (w < warp) before += v;
-        total += v;
-    }
-    int pos = before & 0xFFFF, g = before >> 16;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int e = tid * kPer + i;
-        if (e < a.E) S.begin[e] = count[i] ? pos : -1;
-        for (int done = 0; done < count[i]; done += kGroup, ++g) {
-            L.slots[g] = slot[i];
-            L.off[g] = (unsigned short)(pos + done);
+    int total = 0;  // of the rounds so far: pairs in the low half, groups in the high half
+    for (int e0 = 0, round = 0; e0 < a.E; e0 += kThreads, ++round) {
+        const int e = e0 + tid;
+        int slot = 0, count = e < a.E ? __popc(S.tokens[e][0]) + __popc(S.tokens[e][1]) : 0;
+        if (count) {
+            slot = a.expert_map ? a.expert_map[e] : e;
+            if (slot < 0 || slot >= a.slots) count = 0;
         }
-        pos += count[i];
+        const int own = count + ((count + kGroup - 1) / kGroup << 16);
+        int run = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xFFFFFFFFu, run, o);
+            if (lane >= o) run += v;
+        }
+        if (lane == 31) S.scan[round & 1][warp] = run;
+        __syncthreads();
+        const int sum = lane < kWarps ? S.scan[round & 1][lane] : 0;
+        const int at = total + run - own + __reduce_add_sync(0xFFFFFFFFu, lane < warp ? sum : 0);
+        total += __reduce_add_sync(0xFFFFFFFFu, sum);
+        if (e < a.E) S.begin[e] = count ? at & 0xFFFF : -1;
+        for (int done = 0, g = at >> 16; done < count; done += kGroup, ++g) {
+            L.slots[g] = slot;
+            L.off[g] = (unsigned short)((at & 0xFFFF) + done);
+        }
     }
     if (tid == 0) {
         L.n = total >> 16;
@@ -314,7 +320,7 @@ __device__ void build_lists(const MoeArgs &a, Lists &L, Scratch &S) {
     }
     __syncthreads();
     for (int p = tid; p < P; p += kThreads) {
-        const int e = S.ids[p], at = e >= 0 ? S.begin[e] : -1, t = p / a.k;
+        const int e = S.ids[p], at = e >= 0 ? S.begin[e] : -1, t = (int)(p * a.inv_k >> 16);
         L.has[p] = at >= 0;
         if (at < 0) continue;
         const uint32_t before = (1u << (t & 31)) - 1;
@@ -701,14 +707,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // S
     if (a.router) {
-        for (int t = warp; t < a.T; t += kWarps) {
-            if (a.E <= 128)
-                route_token<4>(a, L, S, t, lane);
-            else if (a.E <= 256)
-                route_token<8>(a, L, S, t, lane);
-            else
-                route_token<32>(a, L, S, t, lane);
-        }
+        if (a.E <= 128)
+            route_all<4>(a, L, S, warp, lane);
+        else if (a.E <= 256)
+            route_all<8>(a, L, S, warp, lane);
+        else
+            for (int t = warp; t < a.T; t += kWarps) route_tokens<kMaxExperts / 32, 1>(a, L, S, t, lane);
     } else if (tid < a.T) {
         given_token(a, L, S, tid);
     }
@@ -774,12 +778,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = blockIdx.x * kThreads + tid; i < a.T * (a.H / 4); i += gridDim.x * kThreads) {
         const int t = i / (a.H / 4), h = (i - t * (a.H / 4)) * 4;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int j = 0; j < a.k; ++j) {
-            const int p = t * a.k + j;
-            if (!L.has[p]) continue;
-            for (int s = 0; s < down.split; ++s) {
-                const float4 v = __ldcg(reinterpret_cast<const float4 *>(a.y + ((size_t)s * P + p) * a.H + h));
-                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        for (int s = 0; s < down.split; ++s) {
+            const float *y = a.y + ((size_t)s * P + t * a.k) * a.H + h;
+            for (int j0 = 0; j0 < a.k; j0 += 8) {  // eight loads in flight
+                float4 v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    v[j] = j0 + j < a.k && L.has[t * a.k + j0 + j]
+                               ? __ldcg(reinterpret_cast<const float4 *>(y + (size_t)(j0 + j) * a.H))
+                               : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum.x += v[j].x, sum.y += v[j].y, sum.z += v[j].z, sum.w += v[j].w;
             }
         }
         __nv_bfloat162 o[2] = {__floats2bfloat162_rn(sum.x, sum.y), __floats2bfloat162_rn(sum.z, sum.w)};
@@ -889,7 +898,7 @@ extern "C" int wisp_mx4_moe(const void *x, int64_t x_stride, const void *router,
     if (const int rc = gemm::make_byte_map(&m13, w13_codes, (uint64_t)num_slots * 2 * inter, hidden / 2, 64)) return rc;
     if (const int rc = gemm::make_byte_map(&m2, w2_codes, (uint64_t)num_slots * hidden, inter / 2, 64)) return rc;
     a.T = num_tokens, a.E = num_experts, a.k = top_k, a.H = hidden, a.I = inter, a.slots = num_slots;
-    a.ids64 = ids_int64, a.renormalize = renormalize;
+    a.ids64 = ids_int64, a.renormalize = renormalize, a.inv_k = 65536 / top_k + 1;
     int dev = 0, sms = 0;
     WISP_CUDA_TRY(cudaGetDevice(&dev));
     WISP_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));

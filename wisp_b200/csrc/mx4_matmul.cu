@@ -42,6 +42,8 @@ constexpr int kTmemCols = 512;
 constexpr int kEpiWarp = 2, kSfWarp = 6;
 constexpr int kThreads = (kSfWarp + kScaleGroups * kScaleGroupWarps) * 32;
 constexpr int kMaxGroups = 1024;
+constexpr int kWindow = 2, kWindowsAhead = 3;  // stages of a window of scale bytes; windows in registers
+static_assert(kStages > kWindow, "a parity wait has to know its phase");
 constexpr int kOutBytes = 32 * 128;           // staging of an epilogue warp: 32 rows of 64 columns
 
 struct MatmulArgs {
@@ -157,9 +159,7 @@ __device__ void load_operands(Control &C, unsigned char *stages, const CUtensorM
         }
 }
 
-template <int WINDOW, int DEEP>
 __device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulArgs &a, int steps) {
-    static_assert(kStages > WINDOW, "a parity wait has to know its phase");
     const int group = (threadIdx.x >> 5) - kSfWarp >= kScaleGroupWarps;
     const int tid = threadIdx.x % (kScaleGroupWarps * 32);
     volatile int *abort = &C.abort;
@@ -180,44 +180,49 @@ __device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulA
             pw[i] = tid + i * 128 < kTileN && rw < wrows ? a.w_scales + rw * a.blocks : nullptr;
         }
     };
-    auto advance = [&](int windows) {
-        bool moved = false;
-        for (int i = 0; i < windows && more; ++i) {
-            kb += WINDOW;
-            if (kb < steps) continue;
-            kb = 0, moved = true;
-            ahead.next();
-            more = ahead.at(C, a);
-        }
-        if (moved && more) point();
+    auto count = [&] { return more ? min(kWindow, steps - kb) : 0; };
+    // to the next window, which may be of another tile
+    auto advance = [&] {
+        kb += kWindow;
+        if (kb < steps || !more) return false;
+        kb = 0;
+        ahead.next();
+        more = ahead.at(C, a);
+        return more;
     };
     struct Window {
-        uint2 a[WINDOW], w[2][WINDOW];
-        bool valid;
-    } buf[DEEP];
+        uint2 a[kWindow], w[2][kWindow];
+        int count, skip;  // stages of the window, and of the other group's window behind it
+    } buf[kWindowsAhead];
     auto load = [&](Window &x) {
-        x.valid = more;
+        x.count = count();
         if (!more) return;
         const int left = a.blocks - kb * kStepBlocks;
 #pragma unroll
-        for (int i = 0; i < WINDOW; ++i) x.a[i] = x.w[0][i] = x.w[1][i] = make_uint2(0, 0);
-        if (pa) load_window<WINDOW>(x.a, pa + kb * kStepBlocks, left, a.align);
+        for (int i = 0; i < kWindow; ++i) x.a[i] = x.w[0][i] = x.w[1][i] = make_uint2(0, 0);
+        if (pa) load_window<kWindow>(x.a, pa + kb * kStepBlocks, x.count, left, a.align);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            if (pw[i]) load_window<WINDOW>(x.w[i], pw[i] + kb * kStepBlocks, left, a.align);
-        advance(kScaleGroups);
+            if (pw[i]) load_window<kWindow>(x.w[i], pw[i] + kb * kStepBlocks, x.count, left, a.align);
+        bool moved = advance();
+        x.skip = count();
+        moved |= advance();
+        if (moved && more) point();
     };
+    if (group == 1) {
+        ring.skip(count());
+        advance();
+    }
     if (more) point();
-    advance(group);
-    ring.skip(group * WINDOW);
 #pragma unroll
-    for (int i = 0; i < DEEP; ++i) load(buf[i]);
+    for (int i = 0; i < kWindowsAhead; ++i) load(buf[i]);
     while (true) {
 #pragma unroll
-        for (int i = 0; i < DEEP; ++i) {
-            if (!buf[i].valid) return;
+        for (int i = 0; i < kWindowsAhead; ++i) {
+            if (!buf[i].count) return;
 #pragma unroll
-            for (int j = 0; j < WINDOW; ++j) {
+            for (int j = 0; j < kWindow; ++j) {
+                if (j >= buf[i].count) break;
                 if (!warp_wait(&C.empty[ring.slot], ring.turn ^ 1, abort, a.status)) return;
                 unsigned char *sfa = sf + ring.slot * kStageBytes, *sfw = sfa + kSfABytes;
                 *reinterpret_cast<uint32_t *>(sfa) = buf[i].a[j].x;
@@ -233,7 +238,7 @@ __device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulA
                 if ((tid & 31) == 0) mbar_arrive(&C.sf_full[ring.slot]);
                 ring.next();
             }
-            ring.skip((kScaleGroups - 1) * WINDOW);
+            ring.skip(buf[i].skip);
             load(buf[i]);
         }
     }
@@ -388,10 +393,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (elect_one()) umma_commit(&C.mma_done);
     } else if (warp < kSfWarp) {
         store_tiles(C, staging, a);
-    } else if (a.align == kWideAlign) {
-        load_all_scales<kWideWindow, 3>(C, stages, a, steps);
     } else {
-        load_all_scales<1, 4>(C, stages, a, steps);
+        load_all_scales(C, stages, a, steps);
     }
     __syncwarp();
     tc_fence_before();

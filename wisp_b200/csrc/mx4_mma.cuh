@@ -114,13 +114,14 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
     return __all_sync(0xFFFFFFFFu, wait_or_abort(bar, parity, abort, status));
 }
 
-// The scale bytes come in windows of WINDOW stages.  The rows of a tile lie in
-// as many lines of the cache, so a load instruction of 32 rows costs 32 lookups
-// whatever it brings: where the rows are 16-byte aligned, a window is two
-// stages and one 16-byte load of a row; else one stage and a load of 8 bytes
-// or less.  Two groups of four warps take the windows in turn, so that one
-// stores while the other loads.  (One group with 8-byte loads needed 1000
-// cycles a stage, twice what the products of a stage take.)
+// The scale bytes come in windows of up to WINDOW stages of a tile, each taken
+// by one of two groups of four warps in turn, so that one stores while the
+// other loads.  The rows of a tile lie in as many lines of the cache, so a load
+// instruction of 32 rows costs 32 lookups whatever it brings: 16 bytes (two
+// stages) a row and instruction where the rows' alignment allows it.  What a
+// new tile costs a thread (its rows' addresses) comes once in a window.  (One
+// group that loaded 8 bytes a stage needed 1000 cycles a stage, twice what the
+// products of a stage take.)
 //
 // A group passes over the other one's windows without waiting for their slots.
 // A parity wait tells a phase from the one before it, not from the one before
@@ -128,8 +129,6 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
 // know that stage k - 2 STAGES was.  Its own stage before k is k - 1 - WINDOW
 // at the earliest, for which it saw k - 1 - WINDOW - STAGES released, and stages
 // are released in order: STAGES > WINDOW is enough.
-constexpr int kWideWindow = 2;
-constexpr int kWideAlign = kWideWindow * kStepBlocks;
 constexpr int kScaleGroups = 2, kScaleGroupWarps = 4;
 
 // The first `left` of eight scale bytes; what lies behind a row's last block is
@@ -141,41 +140,49 @@ __device__ __forceinline__ uint2 first_bytes(uint2 v, int left) {
     }
     return v;
 }
-// A window's scale bytes of a row; `left` of them are the row's (the others:
-// 0, or what lies there for values that first_bytes() will see).  `align`:
-// what the rows are aligned to.  NC: through the read-only path.  Nothing here
-// waits for what it loads.
+// A window's scale bytes of a row, `count` stages of them from p on; `left` of
+// them are the row's (what comes for the others is not defined where the rows
+// are aligned to 8 bytes, else 0).  `align`: what p is aligned to.  NC: through
+// the read-only path.  Nothing here waits for what it loads.
 template <int WINDOW, bool NC = true>
-__device__ __forceinline__ void load_window(uint2 (&v)[WINDOW], const uint8_t *p, int left, int align) {
-    if (WINDOW == kWideWindow) {
-        const uint4 r = NC ? __ldg(reinterpret_cast<const uint4 *>(p)) : ld_cg16(p);
-        v[0] = make_uint2(r.x, r.y), v[WINDOW - 1] = make_uint2(r.z, r.w);
-        return;
-    }
-    if (!NC) {
-        v[0] = __ldcg(reinterpret_cast<const uint2 *>(p));
-        return;
-    }
-    if (align >= 8) {
-        v[0] = __ldg(reinterpret_cast<const uint2 *>(p));
-        return;
-    }
-    v[0] = make_uint2(0, 0);
-    if (align >= 4) {
-        v[0].x = __ldg(reinterpret_cast<const uint32_t *>(p));
-        if (left > 4) v[0].y = __ldg(reinterpret_cast<const uint32_t *>(p) + 1);
-        return;
-    }
+__device__ __forceinline__ void load_window(uint2 (&v)[WINDOW], const uint8_t *p, int count, int left, int align) {
+    static_assert(WINDOW % 2 == 0, "pairs of stages");
+    if (align >= 16) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (i < left) v[0].x |= (uint32_t)__ldg(p + i) << (8 * i);
-        if (i + 4 < left) v[0].y |= (uint32_t)__ldg(p + i + 4) << (8 * i);
+        for (int i = 0; i < WINDOW; i += 2)
+            if (i < count) {
+                const uint4 r = NC ? __ldg(reinterpret_cast<const uint4 *>(p) + i / 2) : ld_cg16(p + i * kStepBlocks);
+                v[i] = make_uint2(r.x, r.y), v[i + 1] = make_uint2(r.z, r.w);
+            }
+    } else if (align >= 8) {
+#pragma unroll
+        for (int i = 0; i < WINDOW; ++i)
+            if (i < count)
+                v[i] = NC ? __ldg(reinterpret_cast<const uint2 *>(p) + i) : __ldcg(reinterpret_cast<const uint2 *>(p) + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < WINDOW; ++i) {
+            v[i] = make_uint2(0, 0);
+            if (i >= count) continue;
+            const uint8_t *q = p + i * kStepBlocks;
+            const int n = left - i * kStepBlocks;
+            if (align >= 4) {
+                v[i].x = __ldg(reinterpret_cast<const uint32_t *>(q));
+                if (n > 4) v[i].y = __ldg(reinterpret_cast<const uint32_t *>(q) + 1);
+                continue;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j < n) v[i].x |= (uint32_t)__ldg(q + j) << (8 * j);
+                if (j + 4 < n) v[i].y |= (uint32_t)__ldg(q + j + 4) << (8 * j);
+            }
+        }
     }
 }
 // What a matrix's rows of scale bytes are aligned to.
 __host__ __device__ inline int scale_align(const void *scales, int blocks) {
     const uintptr_t p = reinterpret_cast<uintptr_t>(scales) | (uintptr_t)blocks;
-    return p % kWideAlign == 0 ? kWideAlign : p % 8 == 0 ? 8 : p % 4 == 0 ? 4 : 1;
+    return p % 16 == 0 ? 16 : p % 8 == 0 ? 8 : p % 4 == 0 ? 4 : 1;
 }
 
 }  // namespace mx4

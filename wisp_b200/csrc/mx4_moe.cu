@@ -62,6 +62,8 @@ constexpr int kAccCols = kGroup * kRows;       // of an accumulator; two of them
 constexpr int kSfCol0 = 2 * kAccCols, kSfCols = 16;
 constexpr int kTmemCols = 512;
 static_assert(kSfCol0 + kStages * kSfCols <= kTmemCols, "tensor memory");
+constexpr int kWindow = 4, kWindowsAhead = 2;   // stages of a window of scale bytes; windows in registers
+static_assert(kStages > kWindow, "a parity wait has to know its phase");
 constexpr int kMaxTokens = 64;
 constexpr int kMaxTopK = 16;
 constexpr int kMaxPairs = kMaxTokens * kMaxTopK;
@@ -340,7 +342,8 @@ struct Phase {
     const CUtensorMap *map;
     const uint8_t *w_scales, *b_codes, *b_scales;
     int64_t w_rows;  // rows of the weight matrix
-    int groups, m_tiles, split, rows_m, slot_rows, second, blocks, steps, align, token_div;
+    int groups, m_tiles, split, rows_m, slot_rows, second, blocks, steps, align, term_align;
+    uint32_t inv_div;  // pair * inv_div >> 16: which terms are the pair's
 };
 // A CTA's walk over the tiles.  (Roles that are one thread or warp feel every
 // instruction: no divisions here, nor remainders in the ring's positions.)
@@ -348,8 +351,8 @@ struct Walk {
     int per_group, dg, din;  // gridDim.x in groups and tiles
     int g, in;
     // the tile
-    int m0, kb0, kb1, off, n, piece;
-    int64_t row;
+    int m0 = 0, kb0 = 0, kb1 = 0, off = 0, n = 0, piece = 0;
+    int64_t row = 0;
     __device__ __forceinline__ Walk(const Phase &ph) {
         per_group = ph.m_tiles * ph.split;
         dg = gridDim.x / per_group, din = gridDim.x - dg * per_group;
@@ -403,7 +406,7 @@ __device__ void run_copies(Control &C, unsigned char *stages, const Phase &ph, c
     int issued = C.issued;
     for (Walk t(ph); t.at(ph, L, C); t.next()) {
         const uint8_t *terms =
-            lane < t.n ? ph.b_codes + ((size_t)(L.pair[t.off + lane] / ph.token_div) * ph.steps + t.kb0) * kTermBytes
+            lane < t.n ? ph.b_codes + ((size_t)(L.pair[t.off + lane] * ph.inv_div >> 16) * ph.steps + t.kb0) * kTermBytes
                        : nullptr;
         const uint32_t bytes = kABytes + t.n * kTermBytes;
         for (int kb = t.kb0; kb < t.kb1; ++kb, cur.ring.next()) {
@@ -446,66 +449,74 @@ __device__ int copy_early(Control &C, unsigned char *stages, const Phase &ph, co
     return early;
 }
 
-template <int WINDOW, int DEEP>
 __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, const Lists &L, Cursor &cur, int *status) {
-    static_assert(kStages > WINDOW, "a parity wait has to know its phase");
     const int group = (threadIdx.x >> 5) - kSfWarp >= kScaleGroupWarps;
     const int tid = threadIdx.x - (kSfWarp + group * kScaleGroupWarps) * 32;
     volatile int *abort = &C.abort;
     unsigned char *sf = stages + kABytes + kBBytes + atom_at(tid);
-    // the loads run DEEP of the group's windows ahead of the stores
+    // the loads run kWindowsAhead of the group's windows ahead of the stores
     Walk ahead(ph);
     bool more = ahead.at(ph, L, C);
-    int kb = 0;
+    int kb = ahead.kb0;
     const uint8_t *pw = nullptr, *pb = nullptr;  // rows of the tile
+    const int64_t my_row = tid < 64 ? tid : ph.second + tid - 64;
+    const int term_stride = ph.steps * kStepBlocks;
     auto point = [&] {
-        const int64_t row = ahead.row + (tid < 64 ? tid : ph.second + tid - 64);
+        const int64_t row = ahead.row + my_row;
         pw = row < ph.w_rows ? ph.w_scales + row * ph.blocks : nullptr;
         const int i = tid / kRows, q = tid % kRows;
         pb = i < ahead.n && q < kTerms
-                 ? ph.b_scales + ((size_t)(L.pair[ahead.off + i] / ph.token_div) * kRows + q) * (ph.steps * kStepBlocks)
+                 ? ph.b_scales + (size_t)((L.pair[ahead.off + i] * ph.inv_div >> 16) * kRows + q) * term_stride
                  : nullptr;
     };
-    auto advance = [&](int windows) {
-        bool moved = false;
-        for (int i = 0; i < windows && more; ++i) {
-            kb += WINDOW;
-            if (kb < ahead.kb1) continue;
-            moved = true;
-            ahead.next();
-            more = ahead.at(ph, L, C);
-            kb = ahead.kb0;
-        }
-        if (moved && more) point();
+    auto count = [&] { return more ? min(kWindow, ahead.kb1 - kb) : 0; };
+    // to the next window, which may be of another tile
+    auto advance = [&] {
+        kb += kWindow;
+        if (!more || kb < ahead.kb1) return false;
+        ahead.next();
+        more = ahead.at(ph, L, C);
+        kb = ahead.kb0;
+        return more;
     };
     struct Window {
-        uint2 w[WINDOW], b[WINDOW];
-        int left;  // scale bytes of a row from here on, 0: no window
-    } buf[DEEP];
+        uint2 w[kWindow], b[kWindow];
+        int count, skip;  // stages of the window, and of the other group's window behind it
+        int left;         // scale bytes of a row from here on
+    } buf[kWindowsAhead];
     auto load = [&](Window &x) {
-        x.left = more ? ph.blocks - kb * kStepBlocks : 0;
+        x.count = count();
         if (!more) return;
+        x.left = ph.blocks - kb * kStepBlocks;
 #pragma unroll
-        for (int i = 0; i < WINDOW; ++i) x.w[i] = x.b[i] = make_uint2(0, 0);
-        if (pw) load_window<WINDOW>(x.w, pw + kb * kStepBlocks, x.left, ph.align);
-        if (pb) load_window<WINDOW, false>(x.b, pb + kb * kStepBlocks, x.left, ph.align);  // written by this kernel
-        advance(kScaleGroups);
+        for (int i = 0; i < kWindow; ++i) x.w[i] = x.b[i] = make_uint2(0, 0);
+        if (pw) load_window<kWindow>(x.w, pw + kb * kStepBlocks, x.count, x.left, ph.align);
+        if (pb)  // written by this kernel
+            load_window<kWindow, false>(x.b, pb + kb * kStepBlocks, x.count, x.left, ph.term_align);
+        bool moved = advance();
+        x.skip = count();
+        moved |= advance();
+        if (moved && more) point();
     };
-    if (more) {
-        point();
-        kb = ahead.kb0;
-    }
-    advance(group);
     RingPos<kStages> ring = cur.ring;
-    ring.skip(group * WINDOW);
+    if (group == 1) {
+        ring.skip(count());
+        advance();
+    }
+    if (more) point();
 #pragma unroll
-    for (int i = 0; i < DEEP; ++i) load(buf[i]);
-    while (true) {
+    for (int i = 0; i < kWindowsAhead; ++i) load(buf[i]);
+    bool done = false;
+    while (!done) {
 #pragma unroll
-        for (int i = 0; i < DEEP; ++i) {
-            if (buf[i].left <= 0) return;
+        for (int i = 0; i < kWindowsAhead; ++i) {
+            if (done || !buf[i].count) {
+                done = true;
+                break;
+            }
 #pragma unroll
-            for (int j = 0; j < WINDOW; ++j) {
+            for (int j = 0; j < kWindow; ++j) {
+                if (j >= buf[i].count) break;
                 if (!warp_wait(&C.empty[ring.slot], ring.turn ^ 1, abort, status)) return;
                 unsigned char *at = sf + ring.slot * kStageBytes;
                 const uint2 terms = first_bytes(buf[i].b[j], buf[i].left - j * kStepBlocks);
@@ -518,22 +529,12 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
                 if ((tid & 31) == 0) mbar_arrive(&C.sf_full[ring.slot]);
                 ring.next();
             }
-            ring.skip((kScaleGroups - 1) * WINDOW);
+            ring.skip(buf[i].skip);
             load(buf[i]);
         }
     }
-}
-// Every group has to come to the phase's last ring position, whichever windows
-// were its own.
-__device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, const Lists &L, Cursor &cur, int *status) {
-    if (ph.align == kWideAlign)
-        run_scales<kWideWindow, 3>(C, stages, ph, L, cur, status);
-    else
-        run_scales<1, 4>(C, stages, ph, L, cur, status);
-    int total = 0;
-    for (Walk t(ph); t.at(ph, L, C); t.next()) total += t.kb1 - t.kb0;
-    for (; total >= kStages; total -= kStages) cur.ring.skip(kStages);
-    cur.ring.skip(total);
+    // both groups have come past the phase's last stage
+    cur.ring = ring;
 }
 
 // The whole warp walks, one lane issues.
@@ -652,7 +653,7 @@ __device__ void run_down(Control &C, const Phase &ph, const Lists &L, Cursor &cu
 // of tiles leaves less than a tenth of the SMs' time unused.
 __device__ __forceinline__ int choose_split(int tiles, int steps, int most) {
     int best = 1, best_use = 0;
-    for (int s = 1; s <= min(most, steps); ++s) {
+    for (int s = 1; s <= max(min(most, steps), 1); ++s) {
         const int n = tiles * s, use = 1000 * n / ((n + (int)gridDim.x - 1) / (int)gridDim.x * (int)gridDim.x);
         if (use > best_use) best = s, best_use = use;
         if (use >= 900) break;
@@ -726,17 +727,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     up.map = &map13, up.w_scales = a.s13, up.b_codes = a.xq, up.b_scales = a.xs;
     up.blocks = a.H / kBlock, up.steps = (up.blocks + kStepBlocks - 1) / kStepBlocks, up.align = a.s13_align;
     up.groups = L.n, up.m_tiles = (a.I + 63) / 64, up.split = 1, up.rows_m = 64;
-    up.slot_rows = 2 * a.I, up.second = a.I, up.w_rows = (int64_t)a.slots * 2 * a.I, up.token_div = a.k;
+    up.slot_rows = 2 * a.I, up.second = a.I, up.w_rows = (int64_t)a.slots * 2 * a.I, up.inv_div = a.inv_k;
     down.map = &map2, down.w_scales = a.s2, down.b_codes = a.aq, down.b_scales = a.as;
     down.blocks = a.I / kBlock, down.steps = (down.blocks + kStepBlocks - 1) / kStepBlocks, down.align = a.s2_align;
     down.groups = L.n, down.m_tiles = (a.H + 127) / 128, down.rows_m = 128;
-    down.split = choose_split(L.n * down.m_tiles, down.align == kWideAlign ? down.steps / kWideWindow : down.steps,
-                              a.max_split);
-    down.slot_rows = a.H, down.second = 64, down.w_rows = (int64_t)a.slots * a.H, down.token_div = 1;
+    down.split = choose_split(L.n * down.m_tiles, down.steps / 2, a.max_split);
+    down.slot_rows = a.H, down.second = 64, down.w_rows = (int64_t)a.slots * a.H, down.inv_div = 65536;
 
-    // pieces of D begin at whole windows of scale bytes
-    const int cut = tid * down.steps / max(down.split, 1);
-    if (tid <= down.split) C.cut[tid] = down.align == kWideAlign ? cut / kWideWindow * kWideWindow : cut;
+    // (pieces of D begin at whole 16-byte loads of scale bytes)
+    up.term_align = up.steps % 2 ? 8 : 16, down.term_align = down.steps % 2 ? 8 : 16;
+    const bool pairs = down.align >= 16 || down.term_align >= 16;
+    if (tid <= down.split) C.cut[tid] = tid * down.steps / down.split / (pairs ? 2 : 1) * (pairs ? 2 : 1);
     __syncthreads();
 
     // G

@@ -42,7 +42,7 @@ constexpr int kTmemCols = 512;
 constexpr int kEpiWarp = 2, kSfWarp = 6;
 constexpr int kThreads = (kSfWarp + kScaleGroups * kScaleGroupWarps) * 32;
 constexpr int kMaxGroups = 1024;
-constexpr int kWindow = 2, kWindowsAhead = 3;  // stages of a window of scale bytes; windows in registers
+constexpr int kWindow = 2, kWindowsAhead = 2;  // stages of a window of scale bytes; windows in registers
 static_assert(kStages > kWindow, "a parity wait has to know its phase");
 constexpr int kOutBytes = 32 * 128;           // staging of an epilogue warp: 32 rows of 64 columns
 

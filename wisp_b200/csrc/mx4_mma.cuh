@@ -102,11 +102,15 @@ __device__ __forceinline__ bool wait_tries(uint64_t *bar, uint32_t parity, const
     return true;
 }
 // The same; a wait that runs out sets the status and the CTA's abort word.
-__device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
+// (One copy of the loop for a kernel's many waits: see load_unaligned_scales.)
+static __device__ __noinline__ bool wait_long(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
     if (wait_tries(bar, parity, abort)) return true;
     *abort = 1;
     *reinterpret_cast<volatile int *>(status) = WISP_ERR_TIMEOUT;
     return false;
+}
+__device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
+    return mbar_try(bar, parity) || wait_long(bar, parity, abort, status);
 }
 
 // For a converged warp: all lanes wait, all go on or none does.
@@ -140,10 +144,29 @@ __device__ __forceinline__ uint2 first_bytes(uint2 v, int left) {
     }
     return v;
 }
+// The eight scale bytes of a row in a stage, of which `left` are the row's (the
+// others: 0), where the rows are not aligned to 8 bytes.  Not inlined: kernels
+// whose roles run at the same time share one instruction cache, and this is
+// the rare case (inlined and unrolled everywhere it made a kernel of 228 KB,
+// which spent as long on fetching instructions as on memory).
+static __device__ __noinline__ uint2 load_unaligned_scales(const uint8_t *p, int left, int align) {
+    uint2 v = make_uint2(0, 0);
+    if (align >= 4) {
+        v.x = __ldg(reinterpret_cast<const uint32_t *>(p));
+        if (left > 4) v.y = __ldg(reinterpret_cast<const uint32_t *>(p) + 1);
+        return v;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (j < left) v.x |= (uint32_t)__ldg(p + j) << (8 * j);
+        if (j + 4 < left) v.y |= (uint32_t)__ldg(p + j + 4) << (8 * j);
+    }
+    return v;
+}
 // A window's scale bytes of a row, `count` stages of them from p on; `left` of
 // them are the row's (what comes for the others is not defined where the rows
 // are aligned to 8 bytes, else 0).  `align`: what p is aligned to.  NC: through
-// the read-only path.  Nothing here waits for what it loads.
+// the read-only path.  With aligned rows nothing here waits for what it loads.
 template <int WINDOW, bool NC = true>
 __device__ __forceinline__ void load_window(uint2 (&v)[WINDOW], const uint8_t *p, int count, int left, int align) {
     static_assert(WINDOW % 2 == 0, "pairs of stages");
@@ -161,22 +184,8 @@ __device__ __forceinline__ void load_window(uint2 (&v)[WINDOW], const uint8_t *p
                 v[i] = NC ? __ldg(reinterpret_cast<const uint2 *>(p) + i) : __ldcg(reinterpret_cast<const uint2 *>(p) + i);
     } else {
 #pragma unroll
-        for (int i = 0; i < WINDOW; ++i) {
-            v[i] = make_uint2(0, 0);
-            if (i >= count) continue;
-            const uint8_t *q = p + i * kStepBlocks;
-            const int n = left - i * kStepBlocks;
-            if (align >= 4) {
-                v[i].x = __ldg(reinterpret_cast<const uint32_t *>(q));
-                if (n > 4) v[i].y = __ldg(reinterpret_cast<const uint32_t *>(q) + 1);
-                continue;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (j < n) v[i].x |= (uint32_t)__ldg(q + j) << (8 * j);
-                if (j + 4 < n) v[i].y |= (uint32_t)__ldg(q + j + 4) << (8 * j);
-            }
-        }
+        for (int i = 0; i < WINDOW; ++i)
+            if (i < count) v[i] = load_unaligned_scales(p + i * kStepBlocks, left - i * kStepBlocks, align);
     }
 }
 // What a matrix's rows of scale bytes are aligned to.

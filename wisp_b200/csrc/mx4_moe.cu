@@ -62,7 +62,7 @@ constexpr int kAccCols = kGroup * kRows;       // of an accumulator; two of them
 constexpr int kSfCol0 = 2 * kAccCols, kSfCols = 16;
 constexpr int kTmemCols = 512;
 static_assert(kSfCol0 + kStages * kSfCols <= kTmemCols, "tensor memory");
-constexpr int kWindow = 4, kWindowsAhead = 2;   // stages of a window of scale bytes; windows in registers
+constexpr int kWindow = 4;                     // stages of a window of scale bytes
 static_assert(kStages > kWindow, "a parity wait has to know its phase");
 constexpr int kMaxTokens = 64;
 constexpr int kMaxTopK = 16;
@@ -104,19 +104,13 @@ struct Lists {
     unsigned char has[kMaxPairs];      // whether the pair is in a group
     int n;                             // groups
 };
-struct Control {
-    uint64_t full[kStages], sf_full[kStages], empty[kStages];
-    uint64_t acc_full[2], acc_empty[2], mma_done;
-    uint32_t tmem_base;
-    int abort, issued, consumed;
-    int cut[kMaxSplit + 1];  // K steps at which the pieces of D begin
-};
 
 // ---- phase R ------------------------------------------------------------------
 // One block of 32 values, one a lane, as terms: codes to `codes` (16 bytes of
 // row 0, rows 128 bytes apart, 16-byte pieces swizzled by the row) and scale
 // bytes to `scales` (rows `stride` apart).
 __device__ __forceinline__ void write_terms(float v, uint8_t *codes, uint8_t *scales, int stride, int piece, int lane) {
+#pragma unroll 1
     for (int q = 0; q < kTerms; ++q) {
         const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v) & 0x7FFFFFFFu);
         const int e = (int)(m >> 23);
@@ -156,7 +150,7 @@ constexpr int kAhead = 8;  // 16-byte loads of a lane in flight
 // One expert's row times TOKENS tokens.
 template <int TOKENS>
 __device__ void route_products(const MoeArgs &a, int gw, int nw, int lane) {
-    constexpr int kDeep = TOKENS == 1 ? kAhead : TOKENS == 2 ? 4 : 2;
+    constexpr int kDeep = TOKENS == 1 ? kAhead : 2;
     const int groups = (a.T + TOKENS - 1) / TOKENS;
     for (int u = gw; u < a.E * groups; u += nw) {
         const int e = u % a.E, t0 = u / a.E * TOKENS;
@@ -198,6 +192,23 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
     return key == 1 ? NAN : __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
+// The weights of a token whose lane j holds its j-th logit's key and expert.
+__device__ void finish_token(const MoeArgs &a, Lists &L, Scratch &S, int t, int lane, uint32_t mine, int my_id) {
+    const float l = logit_of(mine), mx = __shfl_sync(0xFFFFFFFFu, l, 0);
+    float p = 0.f, all = 0.f;
+    if (lane < a.k) p = all = expf(l - mx);
+    if (!a.renormalize) {
+        all = 0.f;
+#pragma unroll 1
+        for (int e = lane; e < a.E; e += 32) all += expf(__ldcg(a.logits + (size_t)t * a.E + e) - mx);
+    }
+    const float sum = warp_sum(all);
+    if (lane < a.k) {
+        S.ids[t * a.k + lane] = my_id;
+        L.w[t * a.k + lane] = p / sum;
+    }
+}
+
 // Top-k of tokens t, t + kWarps, .. (N of them, those behind the last are
 // left out) by (logit descending, id ascending), softmax weights.  Every CTA
 // does this for itself, so its latency counts: a round is two reductions of
@@ -232,33 +243,34 @@ __device__ void route_tokens(const MoeArgs &a, Lists &L, Scratch &S, int t0, int
             my_id[n] = lane == j ? id : my_id[n];
         }
     }
-#pragma unroll
+#pragma unroll 1
     for (int n = 0; n < N; ++n) {
         const int t = t0 + n * kWarps;
         if (t >= a.T) break;
-        const float l = logit_of(mine[n]), mx = __shfl_sync(0xFFFFFFFFu, l, 0);
-        float p = 0.f, all = 0.f;
-        if (lane < a.k) p = all = expf(l - mx);
-        if (!a.renormalize) {
-            all = 0.f;
-            for (int e = lane; e < a.E; e += 32) all += expf(__ldcg(a.logits + (size_t)t * a.E + e) - mx);
-        }
-        const float sum = warp_sum(all);
-        if (lane < a.k) {
-            S.ids[t * a.k + lane] = my_id[n];
-            L.w[t * a.k + lane] = p / sum;
-        }
+        finish_token(a, L, S, t, lane, n ? mine[N - 1] : mine[0], n ? my_id[N - 1] : my_id[0]);
     }
 }
-// All tokens of this warp, two at a time.
-template <int PER_LANE>
-__device__ void route_all(const MoeArgs &a, Lists &L, Scratch &S, int warp, int lane) {
-    for (int t = warp; t < a.T; t += 2 * kWarps) {
-        if (t + kWarps < a.T)
-            route_tokens<PER_LANE, 2>(a, L, S, t, lane);
-        else
-            route_tokens<PER_LANE, 1>(a, L, S, t, lane);
+// The same for more experts than a lane has registers for: `keys` [E] in
+// shared memory, this warp's own.
+__device__ void route_token_shared(const MoeArgs &a, Lists &L, Scratch &S, uint32_t *keys, int t, int lane) {
+    const float *logits = a.logits + (size_t)t * a.E;
+    uint32_t mine = 0;
+    int my_id = 0;
+#pragma unroll 4
+    for (int e = lane; e < a.E; e += 32) keys[e] = key_of(__ldcg(logits + e));
+    for (int j = 0; j < a.k; ++j) {
+        uint32_t best = 0;
+        int id = 0;
+#pragma unroll 4
+        for (int e = lane; e < a.E; e += 32)
+            if (keys[e] > best) best = keys[e], id = e;
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
+        id = (int)__reduce_min_sync(0xFFFFFFFFu, best == top ? (uint32_t)id : 0x7FFFFFFFu);
+        if ((id & 31) == lane) keys[id] = 0;
+        mine = lane == j ? top : mine;
+        my_id = lane == j ? id : my_id;
     }
+    finish_token(a, L, S, t, lane, mine, my_id);
 }
 
 // The caller's routing of token t; an expert named twice is taken once, with
@@ -344,6 +356,14 @@ struct Phase {
     int64_t w_rows;  // rows of the weight matrix
     int groups, m_tiles, split, rows_m, slot_rows, second, blocks, steps, align, term_align;
     uint32_t inv_div;  // pair * inv_div >> 16: which terms are the pair's
+};
+struct Control {
+    uint64_t full[kStages], sf_full[kStages], empty[kStages];
+    uint64_t acc_full[2], acc_empty[2], mma_done;
+    uint32_t tmem_base;
+    int abort, issued, consumed;
+    Phase phase[2];  // G, D
+    int cut[kMaxSplit + 1];  // K steps at which the pieces of D begin
 };
 // A CTA's walk over the tiles.  (Roles that are one thread or warp feel every
 // instruction: no divisions here, nor remainders in the ring's positions.)
@@ -454,7 +474,7 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
     const int tid = threadIdx.x - (kSfWarp + group * kScaleGroupWarps) * 32;
     volatile int *abort = &C.abort;
     unsigned char *sf = stages + kABytes + kBBytes + atom_at(tid);
-    // the loads run kWindowsAhead of the group's windows ahead of the stores
+    // a window is loaded as soon as the one before it is stored; the other group's comes between them
     Walk ahead(ph);
     bool more = ahead.at(ph, L, C);
     int kb = ahead.kb0;
@@ -483,8 +503,8 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
         uint2 w[kWindow], b[kWindow];
         int count, skip;  // stages of the window, and of the other group's window behind it
         int left;         // scale bytes of a row from here on
-    } buf[kWindowsAhead];
-    auto load = [&](Window &x) {
+    } x;
+    auto load = [&] {
         x.count = count();
         if (!more) return;
         x.left = ph.blocks - kb * kStepBlocks;
@@ -504,34 +524,26 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
         advance();
     }
     if (more) point();
+    load();
+#pragma unroll 1
+    while (x.count) {
 #pragma unroll
-    for (int i = 0; i < kWindowsAhead; ++i) load(buf[i]);
-    bool done = false;
-    while (!done) {
-#pragma unroll
-        for (int i = 0; i < kWindowsAhead; ++i) {
-            if (done || !buf[i].count) {
-                done = true;
-                break;
-            }
-#pragma unroll
-            for (int j = 0; j < kWindow; ++j) {
-                if (j >= buf[i].count) break;
-                if (!warp_wait(&C.empty[ring.slot], ring.turn ^ 1, abort, status)) return;
-                unsigned char *at = sf + ring.slot * kStageBytes;
-                const uint2 terms = first_bytes(buf[i].b[j], buf[i].left - j * kStepBlocks);
-                *reinterpret_cast<uint32_t *>(at) = buf[i].w[j].x;
-                *reinterpret_cast<uint32_t *>(at + kAtomBytes) = buf[i].w[j].y;
-                *reinterpret_cast<uint32_t *>(at + 2 * kAtomBytes) = terms.x;
-                *reinterpret_cast<uint32_t *>(at + 3 * kAtomBytes) = terms.y;
-                fence_async_shared();
-                __syncwarp();
-                if ((tid & 31) == 0) mbar_arrive(&C.sf_full[ring.slot]);
-                ring.next();
-            }
-            ring.skip(buf[i].skip);
-            load(buf[i]);
+        for (int j = 0; j < kWindow; ++j) {
+            if (j >= x.count) break;
+            if (!warp_wait(&C.empty[ring.slot], ring.turn ^ 1, abort, status)) return;
+            unsigned char *at = sf + ring.slot * kStageBytes;
+            const uint2 terms = first_bytes(x.b[j], x.left - j * kStepBlocks);
+            *reinterpret_cast<uint32_t *>(at) = x.w[j].x;
+            *reinterpret_cast<uint32_t *>(at + kAtomBytes) = x.w[j].y;
+            *reinterpret_cast<uint32_t *>(at + 2 * kAtomBytes) = terms.x;
+            *reinterpret_cast<uint32_t *>(at + 3 * kAtomBytes) = terms.y;
+            fence_async_shared();
+            __syncwarp();
+            if ((tid & 31) == 0) mbar_arrive(&C.sf_full[ring.slot]);
+            ring.next();
         }
+        ring.skip(x.skip);
+        load();
     }
     // both groups have come past the phase's last stage
     cur.ring = ring;
@@ -692,11 +704,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // R: warps in turn over the SMs, so that few units spread
     const int gw = warp * gridDim.x + blockIdx.x;
     if (a.router) {
-        // as many warps at work as there are: the fewest tokens a unit with which no warp has two
         if (a.E * a.T <= nw)
             route_products<1>(a, gw, nw, lane);
-        else if (a.E * ((a.T + 1) / 2) <= nw)
-            route_products<2>(a, gw, nw, lane);
         else
             route_products<4>(a, gw, nw, lane);
     }
@@ -709,11 +718,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // S
     if (a.router) {
         if (a.E <= 128)
-            route_all<4>(a, L, S, warp, lane);
-        else if (a.E <= 256)
-            route_all<8>(a, L, S, warp, lane);
+            for (int t = warp; t < a.T; t += 2 * kWarps) route_tokens<4, 2>(a, L, S, t, lane);
         else
-            for (int t = warp; t < a.T; t += kWarps) route_tokens<kMaxExperts / 32, 1>(a, L, S, t, lane);
+            for (int t = warp; t < a.T; t += kWarps)
+                route_token_shared(a, L, S, reinterpret_cast<uint32_t *>(&S + 1) + warp * a.E, t, lane);
     } else if (tid < a.T) {
         given_token(a, L, S, tid);
     }
@@ -723,63 +731,59 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("fence.proxy.async;" ::: "memory");
     __syncthreads();
 
-    Phase up{}, down{};
-    up.map = &map13, up.w_scales = a.s13, up.b_codes = a.xq, up.b_scales = a.xs;
-    up.blocks = a.H / kBlock, up.steps = (up.blocks + kStepBlocks - 1) / kStepBlocks, up.align = a.s13_align;
-    up.groups = L.n, up.m_tiles = (a.I + 63) / 64, up.split = 1, up.rows_m = 64;
-    up.slot_rows = 2 * a.I, up.second = a.I, up.w_rows = (int64_t)a.slots * 2 * a.I, up.inv_div = a.inv_k;
-    down.map = &map2, down.w_scales = a.s2, down.b_codes = a.aq, down.b_scales = a.as;
-    down.blocks = a.I / kBlock, down.steps = (down.blocks + kStepBlocks - 1) / kStepBlocks, down.align = a.s2_align;
-    down.groups = L.n, down.m_tiles = (a.H + 127) / 128, down.rows_m = 128;
-    down.split = choose_split(L.n * down.m_tiles, down.steps / 2, a.max_split);
-    down.slot_rows = a.H, down.second = 64, down.w_rows = (int64_t)a.slots * a.H, down.inv_div = 65536;
-
-    // (pieces of D begin at whole 16-byte loads of scale bytes)
-    up.term_align = up.steps % 2 ? 8 : 16, down.term_align = down.steps % 2 ? 8 : 16;
-    const bool pairs = down.align >= 16 || down.term_align >= 16;
-    if (tid <= down.split) C.cut[tid] = tid * down.steps / down.split / (pairs ? 2 : 1) * (pairs ? 2 : 1);
+    if (tid == 0) {
+        Phase &up = C.phase[0], &down = C.phase[1];
+        up.map = &map13, up.w_scales = a.s13, up.b_codes = a.xq, up.b_scales = a.xs;
+        up.blocks = a.H / kBlock, up.steps = (up.blocks + kStepBlocks - 1) / kStepBlocks, up.align = a.s13_align;
+        up.groups = L.n, up.m_tiles = (a.I + 63) / 64, up.split = 1, up.rows_m = 64;
+        up.slot_rows = 2 * a.I, up.second = a.I, up.w_rows = (int64_t)a.slots * 2 * a.I, up.inv_div = a.inv_k;
+        down.map = &map2, down.w_scales = a.s2, down.b_codes = a.aq, down.b_scales = a.as;
+        down.blocks = a.I / kBlock, down.steps = (down.blocks + kStepBlocks - 1) / kStepBlocks, down.align = a.s2_align;
+        down.groups = L.n, down.m_tiles = (a.H + 127) / 128, down.rows_m = 128;
+        down.split = choose_split(L.n * down.m_tiles, down.steps / 2, a.max_split);
+        down.slot_rows = a.H, down.second = 64, down.w_rows = (int64_t)a.slots * a.H, down.inv_div = 65536;
+        // (pieces of D begin at whole 16-byte loads of scale bytes)
+        up.term_align = up.steps % 2 ? 8 : 16, down.term_align = down.steps % 2 ? 8 : 16;
+        const int unit = down.align >= 16 || down.term_align >= 16 ? 2 : 1;
+        for (int i = 0; i <= down.split; ++i) C.cut[i] = i * down.steps / down.split / unit * unit;
+    }
     __syncthreads();
 
-    // G
+    // G and D, by the same code
     Cursor cur;
     int early = 0;
-    if (warp == 0) {
-        run_copies(C, stages, up, L, cur, 0, a.status);
-        early = copy_early(C, stages, down, L, cur.ring, a.status);
-    } else if (warp == 1) {
-        run_products(C, stages, up, L, cur, a.status);
-    } else if (warp < kSfWarp) {
-        run_gate_up(C, up, L, cur, a, ex, down.steps);
-    } else {
-        run_scales(C, stages, up, L, cur, a.status);
-    }
-    __syncwarp();
-    asm volatile("fence.proxy.async;" ::: "memory");  // the terms are read by bulk copies
-    cg::this_grid().sync();
-    asm volatile("fence.proxy.async;" ::: "memory");
-
-    // D
-    if (warp == 0) {
-        run_copies(C, stages, down, L, cur, early, a.status);
-    } else if (warp == 1) {
-        run_products(C, stages, down, L, cur, a.status);
+#pragma unroll 1
+    for (int phase = 0; phase < 2; ++phase) {
+        const Phase ph = C.phase[phase];
+        if (warp == 0) {
+            run_copies(C, stages, ph, L, cur, early, a.status);
+            if (phase == 0) early = copy_early(C, stages, C.phase[1], L, cur.ring, a.status);
+        } else if (warp == 1) {
+            run_products(C, stages, ph, L, cur, a.status);
+            __syncwarp();
+            if (phase == 1 && elect_one()) umma_commit(&C.mma_done);
+        } else if (warp < kSfWarp) {
+            if (phase == 0)
+                run_gate_up(C, ph, L, cur, a, ex, C.phase[1].steps);
+            else
+                run_down(C, ph, L, cur, a);
+        } else {
+            run_scales(C, stages, ph, L, cur, a.status);
+        }
         __syncwarp();
-        if (elect_one()) umma_commit(&C.mma_done);
-    } else if (warp < kSfWarp) {
-        run_down(C, down, L, cur, a);
-    } else {
-        run_scales(C, stages, down, L, cur, a.status);
+        tc_fence_before();
+        asm volatile("fence.proxy.async;" ::: "memory");  // D's terms are read by bulk copies
+        cg::this_grid().sync();
+        asm volatile("fence.proxy.async;" ::: "memory");
+        tc_fence_after();
     }
-    __syncwarp();
-    tc_fence_before();
-    cg::this_grid().sync();
 
     // C
-    const int P = a.T * a.k;
+    const int P = a.T * a.k, split = C.phase[1].split;
     for (int i = blockIdx.x * kThreads + tid; i < a.T * (a.H / 4); i += gridDim.x * kThreads) {
         const int t = i / (a.H / 4), h = (i - t * (a.H / 4)) * 4;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < down.split; ++s) {
+        for (int s = 0; s < split; ++s) {
             const float *y = a.y + ((size_t)s * P + t * a.k) * a.H + h;
             for (int j0 = 0; j0 < a.k; j0 += 8) {  // eight loads in flight
                 float4 v[8];
@@ -825,7 +829,7 @@ struct Workspace {
 };
 constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kGroup * 128 * 4 + sizeof(Control) + sizeof(Lists);
 static_assert(kSmemBytes <= 232448, "shared memory");
-static_assert(sizeof(Scratch) <= kStages * kStageBytes, "the lists' scratch lies in the ring");
+static_assert(sizeof(Scratch) + kWarps * kMaxExperts * 4 <= kStages * kStageBytes, "the lists' scratch lies in the ring");
 
 int check_shape(int32_t T, int32_t E, int32_t k, int32_t H, int32_t I, int32_t slots) {
     if (T < 0 || T > kMaxTokens || E < 1 || E > kMaxExperts || k < 1 || k > kMaxTopK || k > E || slots < 1)

@@ -42,7 +42,7 @@ constexpr int kTmemCols = 512;
 constexpr int kEpiWarp = 2, kSfWarp = 6;
 constexpr int kThreads = (kSfWarp + kScaleGroups * kScaleGroupWarps) * 32;
 constexpr int kMaxGroups = 1024;
-constexpr int kWindow = 2, kWindowsAhead = 2;  // stages of a window of scale bytes; windows in registers
+constexpr int kWindow = 2;  // stages of a window of scale bytes
 static_assert(kStages > kWindow, "a parity wait has to know its phase");
 constexpr int kOutBytes = 32 * 128;           // staging of an epilogue warp: 32 rows of 64 columns
 
@@ -193,7 +193,7 @@ __device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulA
     struct Window {
         uint2 a[kWindow], w[2][kWindow];
         int count, skip;  // stages of the window, and of the other group's window behind it
-    } buf[kWindowsAhead];
+    } x, next;
     auto load = [&](Window &x) {
         x.count = count();
         if (!more) return;
@@ -214,33 +214,31 @@ __device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulA
         advance();
     }
     if (more) point();
-#pragma unroll
-    for (int i = 0; i < kWindowsAhead; ++i) load(buf[i]);
+    x.count = x.skip = 0;
+#pragma unroll 1
     while (true) {
+        load(next);  // ahead of what it waits for here
 #pragma unroll
-        for (int i = 0; i < kWindowsAhead; ++i) {
-            if (!buf[i].count) return;
-#pragma unroll
-            for (int j = 0; j < kWindow; ++j) {
-                if (j >= buf[i].count) break;
-                if (!warp_wait(&C.empty[ring.slot], ring.turn ^ 1, abort, a.status)) return;
-                unsigned char *sfa = sf + ring.slot * kStageBytes, *sfw = sfa + kSfABytes;
-                *reinterpret_cast<uint32_t *>(sfa) = buf[i].a[j].x;
-                *reinterpret_cast<uint32_t *>(sfa + kAtomBytes) = buf[i].a[j].y;
-                *reinterpret_cast<uint32_t *>(sfw) = buf[i].w[0][j].x;
-                *reinterpret_cast<uint32_t *>(sfw + 2 * kAtomBytes) = buf[i].w[0][j].y;
-                if (tid < kTileN - 128) {
-                    *reinterpret_cast<uint32_t *>(sfw + kAtomBytes) = buf[i].w[1][j].x;
-                    *reinterpret_cast<uint32_t *>(sfw + 3 * kAtomBytes) = buf[i].w[1][j].y;
-                }
-                fence_async_shared();
-                __syncwarp();
-                if ((tid & 31) == 0) mbar_arrive(&C.sf_full[ring.slot]);
-                ring.next();
+        for (int j = 0; j < kWindow; ++j) {
+            if (j >= x.count) break;
+            if (!warp_wait(&C.empty[ring.slot], ring.turn ^ 1, abort, a.status)) return;
+            unsigned char *sfa = sf + ring.slot * kStageBytes, *sfw = sfa + kSfABytes;
+            *reinterpret_cast<uint32_t *>(sfa) = x.a[j].x;
+            *reinterpret_cast<uint32_t *>(sfa + kAtomBytes) = x.a[j].y;
+            *reinterpret_cast<uint32_t *>(sfw) = x.w[0][j].x;
+            *reinterpret_cast<uint32_t *>(sfw + 2 * kAtomBytes) = x.w[0][j].y;
+            if (tid < kTileN - 128) {
+                *reinterpret_cast<uint32_t *>(sfw + kAtomBytes) = x.w[1][j].x;
+                *reinterpret_cast<uint32_t *>(sfw + 3 * kAtomBytes) = x.w[1][j].y;
             }
-            ring.skip(buf[i].skip);
-            load(buf[i]);
+            fence_async_shared();
+            __syncwarp();
+            if ((tid & 31) == 0) mbar_arrive(&C.sf_full[ring.slot]);
+            ring.next();
         }
+        ring.skip(x.skip);
+        if (!next.count) break;
+        x = next;
     }
 }
 

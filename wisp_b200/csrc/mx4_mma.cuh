@@ -144,24 +144,36 @@ __device__ __forceinline__ uint2 first_bytes(uint2 v, int left) {
     }
     return v;
 }
-// The eight scale bytes of a row in a stage, of which `left` are the row's (the
+// The scale bytes of a window of a row, of which `left` are the row's (the
 // others: 0), where the rows are not aligned to 8 bytes.  Not inlined: kernels
 // whose roles run at the same time share one instruction cache, and this is
 // the rare case (inlined and unrolled everywhere it made a kernel of 228 KB,
 // which spent as long on fetching instructions as on memory).
-static __device__ __noinline__ uint2 load_unaligned_scales(const uint8_t *p, int left, int align) {
-    uint2 v = make_uint2(0, 0);
-    if (align >= 4) {
-        v.x = __ldg(reinterpret_cast<const uint32_t *>(p));
-        if (left > 4) v.y = __ldg(reinterpret_cast<const uint32_t *>(p) + 1);
-        return v;
-    }
+template <int WINDOW>
+struct ScaleWindow {
+    uint2 v[WINDOW];
+};
+template <int WINDOW>
+__device__ __noinline__ ScaleWindow<WINDOW> load_unaligned_scales(const uint8_t *p, int count, int left, int align) {
+    ScaleWindow<WINDOW> r;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (j < left) v.x |= (uint32_t)__ldg(p + j) << (8 * j);
-        if (j + 4 < left) v.y |= (uint32_t)__ldg(p + j + 4) << (8 * j);
+    for (int i = 0; i < WINDOW; ++i) {
+        uint2 v = make_uint2(0, 0);
+        const int n = i < count ? left - i * kStepBlocks : 0;
+        const uint8_t *q = p + i * kStepBlocks;
+        if (align >= 4) {
+            if (n > 0) v.x = __ldg(reinterpret_cast<const uint32_t *>(q));
+            if (n > 4) v.y = __ldg(reinterpret_cast<const uint32_t *>(q) + 1);
+        } else {
+#pragma unroll 1
+            for (int j = 0; j < min(n, 8); ++j) {
+                const uint32_t b = (uint32_t)__ldg(q + j) << (8 * (j & 3));
+                v.x |= j < 4 ? b : 0, v.y |= j < 4 ? 0 : b;
+            }
+        }
+        r.v[i] = v;
     }
-    return v;
+    return r;
 }
 // A window's scale bytes of a row, `count` stages of them from p on; `left` of
 // them are the row's (what comes for the others is not defined where the rows
@@ -183,9 +195,9 @@ __device__ __forceinline__ void load_window(uint2 (&v)[WINDOW], const uint8_t *p
             if (i < count)
                 v[i] = NC ? __ldg(reinterpret_cast<const uint2 *>(p) + i) : __ldcg(reinterpret_cast<const uint2 *>(p) + i);
     } else {
+        const ScaleWindow<WINDOW> r = load_unaligned_scales<WINDOW>(p, count, left, align);
 #pragma unroll
-        for (int i = 0; i < WINDOW; ++i)
-            if (i < count) v[i] = load_unaligned_scales(p + i * kStepBlocks, left - i * kStepBlocks, align);
+        for (int i = 0; i < WINDOW; ++i) v[i] = r.v[i];
     }
 }
 // What a matrix's rows of scale bytes are aligned to.

@@ -524,9 +524,10 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
         advance();
     }
     if (more) point();
-    load();
 #pragma unroll 1
-    while (x.count) {
+    while (true) {
+        load();
+        if (!x.count) break;
 #pragma unroll
         for (int j = 0; j < kWindow; ++j) {
             if (j >= x.count) break;
@@ -543,7 +544,6 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
             ring.next();
         }
         ring.skip(x.skip);
-        load();
     }
     // both groups have come past the phase's last stage
     cur.ring = ring;

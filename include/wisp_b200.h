@@ -165,9 +165,13 @@ WISP_API int wisp_mx4_sync(void *stream);
  * [inter] in MXFP4; expert e lies in slot expert_map[e] (int32 [num_experts];
  * NULL: slot e).  An id outside [0, num_experts) and an expert whose slot is
  * outside [0, num_slots) contribute nothing; an expert a token names twice
- * counts once, with the sum of the weights.  fp32 arithmetic; silu(g) u is
- * rounded to bf16 and out once.  A token's result does not depend on the
- * slots.  T <= 64, top_k <= 16, num_experts <= 1024, hidden and inter
+ * counts once, with the sum of the weights.  slot_strides: bytes from slot to
+ * slot of w13's codes, w13's scales, w2's codes and w2's scales, each a whole
+ * number of its rows (NULL: the slots follow one another).  Activations take
+ * part as sums of six MXFP4 terms (at least 12 bits of a block's largest
+ * value), the rest is fp32, out is rounded once.  A token's result depends on
+ * nothing but its own row, weights and experts: not on the slots, nor on the
+ * other tokens of the call.  T <= 64, top_k <= 16, num_experts <= 1024, hidden and inter
  * multiples of 32 up to 32768 and 65536.  workspace:
  * wisp_mx4_moe_workspace() bytes, aligned to 16, any contents; calls that may
  * overlap on the GPU need one each.
@@ -177,7 +181,7 @@ WISP_API int wisp_mx4_moe_workspace(int32_t num_tokens, int32_t num_experts, int
 WISP_API int wisp_mx4_moe(const void *x, int64_t x_stride, const void *router, const void *topk_ids,
                           int32_t ids_int64, const float *topk_weights, const int32_t *expert_map,
                           const void *w13_codes, const void *w13_scales, const void *w2_codes, const void *w2_scales,
-                          int32_t num_slots, int32_t num_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,
+                          const int64_t *slot_strides, int32_t num_slots, int32_t num_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,
                           int32_t inter, int32_t renormalize, void *workspace, int64_t workspace_bytes, void *out,
                           void *stream);
 

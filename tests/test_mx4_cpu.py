@@ -71,6 +71,8 @@ def test_python_refusals():
         Mx4Tensor(codes[:1], scales)
     with pytest.raises(ValueError, match="contiguous"):
         Mx4Tensor(codes.t().contiguous().t(), scales)
+    blob = torch.zeros(3, 70, dtype=torch.uint8)         # a stack whose matrices lie apart
+    assert Mx4Tensor(blob[:, :64].view(3, 2, 32), torch.zeros(3, 2, 2, dtype=torch.uint8)).shape == (3, 2, 64)
     with pytest.raises(ValueError, match="CUDA"):
         block_norm(x, x, x[0])
 
@@ -101,8 +103,9 @@ def test_moe_refusals():
     f = _lib.lib().wisp_mx4_moe
 
     def call(T=1, E=4, k=2, H=64, I=32, slots=4, x=P, router=P, ids=None, w=None, emap=None, c13=P, ws=P,
-             nbytes=1 << 30, stride=64, out=P):
-        return f(x, stride, router, ids, 0, w, emap, c13, P, P, P, slots, T, E, k, H, I, 1, ws, nbytes, out, None)
+             nbytes=1 << 30, stride=64, out=P, strides=None):
+        strides = strides and (ctypes.c_int64 * 4)(*strides)
+        return f(x, stride, router, ids, 0, w, emap, c13, P, P, P, strides, slots, T, E, k, H, I, 1, ws, nbytes, out, None)
     refused(call(T=65), "64 tokens")
     refused(call(T=-1), "64 tokens")
     refused(call(E=1025), "1024 experts")
@@ -122,6 +125,9 @@ def test_moe_refusals():
     refused(call(c13=P + 8), "aligned")
     refused(call(out=P + 8), "aligned")
     refused(call(ws=P + 4), "aligned")
+    good = [64 * 32, 64 * 2, 64 * 16, 64]               # slots of H 64, I 32 that follow one another
+    for i, bad in ((0, 64 * 32 - 32), (0, 64 * 32 + 16), (1, 64), (2, 0), (3, 48)):
+        refused(call(strides=good[:i] + [bad] + good[i + 1:]), "whole rows")
     refused(call(slots=1 << 26, I=32), "rows")
     refused(call(T=2, stride=32), "overlap")
     refused(call(T=2, stride=68), "16-byte")

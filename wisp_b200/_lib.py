@@ -55,7 +55,7 @@ SIGNATURES = {
     "wisp_mx4_matmul": (ctypes.c_int, [_vp, _vp, _c_int64, _vp, _vp, _c_int32, _c_int32, _c_int32, _vp, _vp, _vp]),
     "wisp_mx4_sync": (ctypes.c_int, [_vp]),
     "wisp_mx4_moe_workspace": (ctypes.c_int, [_c_int32] * 5 + [_p64]),
-    "wisp_mx4_moe": (ctypes.c_int, [_vp, _c_int64, _vp, _vp, _c_int32, _vp, _vp, _vp, _vp, _vp, _vp] +
+    "wisp_mx4_moe": (ctypes.c_int, [_vp, _c_int64, _vp, _vp, _c_int32, _vp, _vp, _vp, _vp, _vp, _vp, _p64] +
                      [_c_int32] * 7 + [_vp, _c_int64, _vp, _vp]),
     "wisp_block_norm": (ctypes.c_int, [_vp, _c_int64, _vp, _c_int64, _vp, _vp, _vp, _c_int32, _c_int64, _c_int32,
                                        _c_int32, _c_int32, _c_int64, _c_int32, ctypes.c_float, ctypes.c_float,

@@ -30,8 +30,8 @@
 //      expert; the epilogue brings g and u of a value together through shared
 //      memory and writes silu(g) u as terms again
 //   D  (after a barrier; its first weights are on their way before it) down:
-//      tiles of 128 rows of the hidden size, the intermediate size in pieces
-//      where there are too few tiles to fill the SMs evenly; p_e y_e in fp32
+//      tiles of 128 rows of the hidden size, a large intermediate size in
+//      pieces; p_e y_e in fp32
 //   C  (after a barrier) the sum over a token's experts, in routing order: no
 //      atomics, the same bits every run
 // In G and D a warp each feeds a ring of 5 stages of 256 values of K (weights
@@ -39,6 +39,8 @@
 // as the swizzle wants them) and issues the products, eight bring the scale
 // bytes (mx4_mma.cuh), four read the accumulators.
 #include <cooperative_groups.h>
+
+#include <algorithm>
 
 #include "mx4_mma.cuh"
 
@@ -69,7 +71,7 @@ constexpr int kMaxTopK = 16;
 constexpr int kMaxPairs = kMaxTokens * kMaxTopK;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxGroups = kMaxPairs;          // no group is empty
-constexpr int kMaxSplit = 8;                   // pieces of the intermediate size in D
+constexpr int kMaxSplit = 16;                  // pieces of the intermediate size in D
 
 struct MoeArgs {
     const __nv_bfloat16 *x;
@@ -79,13 +81,14 @@ struct MoeArgs {
     const float *weights;
     const int32_t *expert_map;    // [E] slot of each expert, or nullptr: slot = expert
     const uint8_t *s13, *s2;
+    int w13_rows, s13_rows, w2_rows, s2_rows;  // rows from slot to slot: codes, scale bytes
     __nv_bfloat16 *out;
     float *logits;                // [T][E]
     uint8_t *xq, *xs;             // terms of x: [T][steps][kTermBytes], scales [T][kRows][steps * 8]
     uint8_t *aq, *as;             // terms of silu(g) u: the same for each pair
     float *y;                     // [split][T * k][H]
     int *status;
-    int T, E, k, H, I, slots, ids64, renormalize, s13_align, s2_align, max_split;
+    int T, E, k, H, I, slots, ids64, renormalize, s13_align, s2_align;
     uint32_t inv_k;               // p / k = p * inv_k >> 16 for every pair p
 };
 
@@ -347,14 +350,14 @@ __device__ void build_lists(const MoeArgs &a, Lists &L, Scratch &S) {
 
 // ---- phases G and D ---------------------------------------------------------------
 // The tiles of a phase, in the order group, piece of K, rows; a CTA takes every
-// gridDim.x-th.  Weight rows: the first 64 of a tile from slot * slot_rows +
-// m0 on, the second 64 from `second` rows further on.  K: `blocks` scale bytes
-// a row, `steps` steps of 256 values, in `split` pieces.
+// gridDim.x-th.  An expert's matrix has `rows` rows; slots lie slot_rows rows
+// of codes and scale_slot_rows rows of scale bytes apart.  The first 64 rows
+// of a tile are m0 .., the second 64 lie `second` rows further on.  K: `blocks`
+// scale bytes a row, `steps` steps of 256 values, in `split` pieces.
 struct Phase {
     const CUtensorMap *map;
     const uint8_t *w_scales, *b_codes, *b_scales;
-    int64_t w_rows;  // rows of the weight matrix
-    int groups, m_tiles, split, rows_m, slot_rows, second, blocks, steps, align, term_align;
+    int groups, m_tiles, split, rows_m, rows, slot_rows, scale_slot_rows, second, blocks, steps, align, term_align;
     uint32_t inv_div;  // pair * inv_div >> 16: which terms are the pair's
 };
 struct Control {
@@ -372,7 +375,7 @@ struct Walk {
     int g, in;
     // the tile
     int m0 = 0, kb0 = 0, kb1 = 0, off = 0, n = 0, piece = 0;
-    int64_t row = 0;
+    int row = 0, slot = 0;  // row of the weight matrix, slot
     __device__ __forceinline__ Walk(const Phase &ph) {
         per_group = ph.m_tiles * ph.split;
         dg = gridDim.x / per_group, din = gridDim.x - dg * per_group;
@@ -390,7 +393,8 @@ struct Walk {
         m0 = m * ph.rows_m;
         off = L.off[g];
         n = L.off[g + 1] - off;
-        row = (int64_t)L.slots[g] * ph.slot_rows + m0;
+        slot = L.slots[g];
+        row = slot * ph.slot_rows + m0;
         return true;
     }
     __device__ __forceinline__ void next() {
@@ -413,8 +417,8 @@ struct Cursor {
 };
 
 __device__ __forceinline__ void load_weights(unsigned char *st, const Phase &ph, const Walk &t, int kb, uint64_t *bar) {
-    tma_load_2d(st, ph.map, kb * 128, (int)t.row, bar);
-    tma_load_2d(st + kABytes / 2, ph.map, kb * 128, (int)t.row + ph.second, bar);
+    tma_load_2d(st, ph.map, kb * 128, t.row, bar);
+    tma_load_2d(st + kABytes / 2, ph.map, kb * 128, t.row + ph.second, bar);
 }
 
 // Copies of a phase's steps: the first lane brings the weights (those of the
@@ -479,11 +483,11 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
     bool more = ahead.at(ph, L, C);
     int kb = ahead.kb0;
     const uint8_t *pw = nullptr, *pb = nullptr;  // rows of the tile
-    const int64_t my_row = tid < 64 ? tid : ph.second + tid - 64;
+    const int my_row = tid < 64 ? tid : ph.second + tid - 64;
     const int term_stride = ph.steps * kStepBlocks;
     auto point = [&] {
-        const int64_t row = ahead.row + my_row;
-        pw = row < ph.w_rows ? ph.w_scales + row * ph.blocks : nullptr;
+        const int row = ahead.m0 + my_row;
+        pw = row < ph.rows ? ph.w_scales + ((int64_t)ahead.slot * ph.scale_slot_rows + row) * ph.blocks : nullptr;
         const int i = tid / kRows, q = tid % kRows;
         pb = i < ahead.n && q < kTerms
                  ? ph.b_scales + (size_t)((L.pair[ahead.off + i] * ph.inv_div >> 16) * kRows + q) * term_stride
@@ -661,17 +665,11 @@ __device__ void run_down(Control &C, const Phase &ph, const Lists &L, Cursor &cu
     }
 }
 
-// Pieces of the intermediate size in D: the fewest with which the last round
-// of tiles leaves less than a tenth of the SMs' time unused.
-__device__ __forceinline__ int choose_split(int tiles, int steps, int most) {
-    int best = 1, best_use = 0;
-    for (int s = 1; s <= max(min(most, steps), 1); ++s) {
-        const int n = tiles * s, use = 1000 * n / ((n + (int)gridDim.x - 1) / (int)gridDim.x * (int)gridDim.x);
-        if (use > best_use) best = s, best_use = use;
-        if (use >= 900) break;
-    }
-    return best;
-}
+// Pieces of the intermediate size in D.  They let a few experts' tiles fill the
+// SMs evenly (two experts of 4096 x 14336 are 64 tiles of 1 MB), and depend on
+// the sizes alone, so that a token's bits do not depend on the tokens beside it.
+__host__ __device__ constexpr int pieces_of(int steps) { return (steps + 15) / 16; }
+static_assert(pieces_of(65536 / kStepK) <= kMaxSplit, "largest intermediate size");
 
 __global__ void __launch_bounds__(kThreads, 1)
     moe_kernel(const __grid_constant__ CUtensorMap map13, const __grid_constant__ CUtensorMap map2, const MoeArgs a) {
@@ -736,12 +734,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         up.map = &map13, up.w_scales = a.s13, up.b_codes = a.xq, up.b_scales = a.xs;
         up.blocks = a.H / kBlock, up.steps = (up.blocks + kStepBlocks - 1) / kStepBlocks, up.align = a.s13_align;
         up.groups = L.n, up.m_tiles = (a.I + 63) / 64, up.split = 1, up.rows_m = 64;
-        up.slot_rows = 2 * a.I, up.second = a.I, up.w_rows = (int64_t)a.slots * 2 * a.I, up.inv_div = a.inv_k;
+        up.rows = 2 * a.I, up.slot_rows = a.w13_rows, up.scale_slot_rows = a.s13_rows, up.second = a.I;
+        up.inv_div = a.inv_k;
         down.map = &map2, down.w_scales = a.s2, down.b_codes = a.aq, down.b_scales = a.as;
         down.blocks = a.I / kBlock, down.steps = (down.blocks + kStepBlocks - 1) / kStepBlocks, down.align = a.s2_align;
         down.groups = L.n, down.m_tiles = (a.H + 127) / 128, down.rows_m = 128;
-        down.split = choose_split(L.n * down.m_tiles, down.steps / 2, a.max_split);
-        down.slot_rows = a.H, down.second = 64, down.w_rows = (int64_t)a.slots * a.H, down.inv_div = 65536;
+        down.split = pieces_of(down.steps);
+        down.rows = a.H, down.slot_rows = a.w2_rows, down.scale_slot_rows = a.s2_rows, down.second = 64;
+        down.inv_div = 65536;
         // (pieces of D begin at whole 16-byte loads of scale bytes)
         up.term_align = up.steps % 2 ? 8 : 16, down.term_align = down.steps % 2 ? 8 : 16;
         const int unit = down.align >= 16 || down.term_align >= 16 ? 2 : 1;
@@ -812,7 +812,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 struct Workspace {
     size_t logits, xq, xs, aq, as, y, bytes;
-    int split;  // pieces of D that y has room for
     Workspace(int T, int E, int k, int H, int I) {
         size_t at = 0;
         const auto take = [&](size_t n) { const size_t here = at; at += (n + 255) / 256 * 256; return here; };
@@ -822,8 +821,7 @@ struct Workspace {
         xs = take(T * up * kRows * kStepBlocks);
         aq = take(P * down * kTermBytes);
         as = take(P * down * kRows * kStepBlocks);
-        split = (int)(down < kMaxSplit ? down : kMaxSplit);
-        y = take((size_t)split * P * H * 4);
+        y = take((size_t)pieces_of((int)down) * P * H * 4);
         bytes = at;
     }
 };
@@ -838,8 +836,15 @@ int check_shape(int32_t T, int32_t E, int32_t k, int32_t H, int32_t I, int32_t s
     if (H < 32 || H % 32 || H > 32768 || I < 32 || I % 32 || I > 65536)
         return set_error("wisp_mx4_moe: hidden and intermediate sizes are multiples of 32, at most 32768 and 65536"),
                WISP_ERR_INVALID;
-    if ((int64_t)slots * 2 * I > INT32_MAX || (int64_t)slots * H > INT32_MAX)
-        return set_error("wisp_mx4_moe: too many weight rows"), WISP_ERR_INVALID;
+    return WISP_OK;
+}
+
+// Rows of `row_bytes` from slot to slot, from a stride in bytes.
+int slot_rows(int64_t stride, int64_t row_bytes, int64_t rows, int32_t slots, int *out) {
+    if (stride % row_bytes || stride / row_bytes < rows || stride / row_bytes * slots > INT32_MAX)
+        return set_error("wisp_mx4_moe: slots must be whole rows apart and not overlap, with at most 2^31 rows in all"),
+               WISP_ERR_INVALID;
+    *out = (int)(stride / row_bytes);
     return WISP_OK;
 }
 
@@ -861,7 +866,7 @@ extern "C" int wisp_mx4_moe_workspace(int32_t num_tokens, int32_t num_experts, i
 extern "C" int wisp_mx4_moe(const void *x, int64_t x_stride, const void *router, const void *topk_ids,
                             int32_t ids_int64, const float *topk_weights, const int32_t *expert_map,
                             const void *w13_codes, const void *w13_scales, const void *w2_codes, const void *w2_scales,
-                            int32_t num_slots, int32_t num_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,
+                            const int64_t *slot_strides, int32_t num_slots, int32_t num_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,
                             int32_t inter, int32_t renormalize, void *workspace, int64_t workspace_bytes, void *out,
                             void *stream) {
     if (const int rc = check_shape(num_tokens, num_experts, top_k, hidden, inter, num_slots)) return rc;
@@ -897,11 +902,21 @@ extern "C" int wisp_mx4_moe(const void *x, int64_t x_stride, const void *router,
     a.logits = reinterpret_cast<float *>(ws + w.logits);
     a.xq = ws + w.xq, a.xs = ws + w.xs, a.aq = ws + w.aq, a.as = ws + w.as;
     a.y = reinterpret_cast<float *>(ws + w.y);
-    a.max_split = w.split;
-    if (const int rc = status_word(&a.status)) return rc;
-    CUtensorMap m13, m2;
-    if (const int rc = gemm::make_byte_map(&m13, w13_codes, (uint64_t)num_slots * 2 * inter, hidden / 2, 64)) return rc;
-    if (const int rc = gemm::make_byte_map(&m2, w2_codes, (uint64_t)num_slots * hidden, inter / 2, 64)) return rc;
+    const int64_t hb = hidden / 2, ib = inter / 2;
+    const int64_t packed[4] = {2 * inter * hb, 2 * inter * (hb / 16), hidden * ib, hidden * (ib / 16)};
+    const int64_t *st = slot_strides ? slot_strides : packed;
+    int rc = slot_rows(st[0], hb, 2 * inter, num_slots, &a.w13_rows);
+    if (!rc) rc = slot_rows(st[1], hb / 16, 2 * inter, num_slots, &a.s13_rows);
+    if (!rc) rc = slot_rows(st[2], ib, hidden, num_slots, &a.w2_rows);
+    if (!rc) rc = slot_rows(st[3], ib / 16, hidden, num_slots, &a.s2_rows);
+    if (!rc) rc = status_word(&a.status);
+    CUtensorMap m13, m2;  // they end with the last slot's last row
+    if (!rc) rc = gemm::make_byte_map(&m13, w13_codes, (uint64_t)a.w13_rows * (num_slots - 1) + 2 * inter, hb, 64);
+    if (!rc) rc = gemm::make_byte_map(&m2, w2_codes, (uint64_t)a.w2_rows * (num_slots - 1) + hidden, ib, 64);
+    if (rc) return rc;
+    // a slot's scale bytes are aligned like the first slot's only where the stride keeps that
+    a.s13_align = std::min(a.s13_align, scale_align(nullptr, (int)(st[1] & 15)));
+    a.s2_align = std::min(a.s2_align, scale_align(nullptr, (int)(st[3] & 15)));
     a.T = num_tokens, a.E = num_experts, a.k = top_k, a.H = hidden, a.I = inter, a.slots = num_slots;
     a.ids64 = ids_int64, a.renormalize = renormalize, a.inv_k = 65536 / top_k + 1;
     int dev = 0, sms = 0;

@@ -11,6 +11,7 @@ and expert compute run in this package's sm_100a kernels.
 """
 from .fused_moe import WispMoEState, install_wisp_moe, is_installed
 from .fused_moe_fp8 import WispMoEStateFP8, install_wisp_fp8, is_fp8_installed
+from .fused_moe_mx4 import WispMoEStateMX4
 
 __all__ = ["install_wisp_moe", "is_installed", "WispMoEState", "install_wisp_fp8", "is_fp8_installed",
-           "WispMoEStateFP8"]
+           "WispMoEStateFP8", "WispMoEStateMX4"]

@@ -20,8 +20,9 @@ BLOCK = 32
 
 
 class Mx4Tensor:
-    """Codes and scales of a matrix ``[..., K]``, ``K`` a multiple of 32, both contiguous uint8 (scales may be given
-    as ``torch.float8_e8m0fnu``)."""
+    """Codes and scales of a matrix ``[..., K]``, ``K`` a multiple of 32, both uint8 (scales may be given as
+    ``torch.float8_e8m0fnu``) and contiguous; the matrices of a stack ``[S, N, K]`` may lie apart (slots that hold
+    other tensors too)."""
 
     __slots__ = ("codes", "scales")
 
@@ -36,8 +37,10 @@ class Mx4Tensor:
                              f"{tuple(scales.shape)}")
         if codes.device != scales.device:
             raise ValueError(f"codes are on {codes.device}, scales on {scales.device}")
-        if not (codes.is_contiguous() and scales.is_contiguous()):
-            raise ValueError("codes and scales must be contiguous")
+        for t in (codes, scales):
+            if not (t.is_contiguous() or (t.dim() == 3 and t.stride(2) == 1 and t.stride(1) == t.shape[2]
+                                          and t.stride(0) >= t.shape[1] * t.shape[2])):
+                raise ValueError("codes and scales must be contiguous, or a stack of contiguous matrices")
         self.codes, self.scales = codes, scales
 
     @property
@@ -106,6 +109,8 @@ def mx4_dequantize(q: Mx4Tensor, dtype: torch.dtype = torch.bfloat16, out: torch
     hold them)."""
     codes = q.codes
     index = cuda_index("q", codes)
+    if not (codes.is_contiguous() and q.scales.is_contiguous()):
+        raise ValueError("mx4_dequantize takes contiguous matrices")
     dt = DTYPES.get(dtype)
     if dt is None:
         raise TypeError(f"dtype must be bf16, fp16 or fp32; got {dtype}")
@@ -127,6 +132,8 @@ def mx4_matmul(a: Mx4Tensor, w: Mx4Tensor, offsets: torch.Tensor | None = None,
     index = cuda_index("a", a.codes)
     if a.codes.dim() != 2 or w.codes.dim() not in (2, 3) or w.codes.shape[-1] != a.codes.shape[1]:
         raise ValueError(f"a is [M, K], w [N, K] or [G, N, K]; got {tuple(a.shape)} and {tuple(w.shape)}")
+    if not (a.codes.is_contiguous() and w.codes.is_contiguous() and w.scales.is_contiguous()):
+        raise ValueError("mx4_matmul takes contiguous matrices")
     rows, half = a.codes.shape
     n = w.codes.shape[-2]
     groups = w.codes.shape[0] if w.codes.dim() == 3 else 1
@@ -214,13 +221,18 @@ def mx4_moe(x: torch.Tensor, w13: Mx4Tensor, w2: Mx4Tensor, top_k: int | None = 
         ip, wp, ids64 = topk_ids.data_ptr(), topk_weights.data_ptr(), int(topk_ids.dtype == torch.int64)
     if x.stride(1) != 1 or (tokens > 1 and (x.stride(0) < hidden or x.stride(0) % 8)) or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
+    strides = None
+    if not (w13.codes.is_contiguous() and w13.scales.is_contiguous() and w2.codes.is_contiguous()
+            and w2.scales.is_contiguous()):
+        strides = (ctypes.c_int64 * 4)(w13.codes.stride(0), w13.scales.stride(0), w2.codes.stride(0),
+                                       w2.scales.stride(0))
     out = (x.new_empty((tokens, hidden)) if out is None
            else need_out("out", out, (tokens, hidden), torch.bfloat16, index))
     need = _moe_workspace(tokens, experts, top_k, hidden, inter2 // 2)
     ws = x.new_empty(need, dtype=torch.uint8)
     launch("wisp_mx4_moe", index, x.data_ptr(), x.stride(0), rp, ip, ids64, wp,
            None if expert_map is None else expert_map.data_ptr(), w13.codes.data_ptr(), w13.scales.data_ptr(),
-           w2.codes.data_ptr(), w2.scales.data_ptr(), slots, tokens, experts, top_k, hidden, inter2 // 2,
+           w2.codes.data_ptr(), w2.scales.data_ptr(), strides, slots, tokens, experts, top_k, hidden, inter2 // 2,
            int(renormalize), ws.data_ptr(), need, out.data_ptr())
     return out
 

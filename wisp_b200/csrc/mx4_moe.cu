@@ -22,17 +22,17 @@
 // hundred instructions that 128 columns of 16 rows take.)
 //
 // Bound by HBM: a few tokens use every byte of a routed expert once.  A
-// cooperative launch of one CTA of 14 warps per SM runs
+// cooperative launch of one CTA of 16 warps per SM runs
 //   R  router products (a warp per expert row and token group), x to terms
 //   S  (after a grid barrier, every CTA for itself) top-k and the lists of
 //      each expert's tokens in groups of at most 16
 //   G  gate-up: tiles of 64 gate rows and the matching 64 up rows of a group's
 //      expert; the epilogue brings g and u of a value together through shared
 //      memory and writes silu(g) u as terms again
-//   D  (after a barrier; its first weights are on their way before it) down:
-//      tiles of 128 rows of the hidden size, a large intermediate size in
-//      pieces; p_e y_e in fp32
-//   C  (after a barrier) the sum over a token's experts, in routing order: no
+//   D  (a group's tiles once the group's tiles of G are counted; weights are on
+//      their way before) down: tiles of 128 rows of the hidden size, a large
+//      intermediate size in pieces; p_e y_e in fp32
+//   C  (after a second barrier) the sum over a token's experts, in routing order: no
 //      atomics, the same bits every run
 // In G and D a warp each feeds a ring of 5 stages of 256 values of K (weights
 // by TMA, the terms by bulk copies of 1 KB a token, laid out by their writers
@@ -51,7 +51,8 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kEpiWarp = 2, kSfWarp = 6;       // four warps and two groups of four; 0: copies, 1: products
-constexpr int kWarps = kSfWarp + kScaleGroups * kScaleGroupWarps;
+constexpr int kWarps = 16;                     // two of them in R, S and C only
+static_assert(kSfWarp + kScaleGroups * kScaleGroupWarps <= kWarps, "roles");
 constexpr int kThreads = kWarps * 32;
 constexpr int kTerms = 6;                      // terms of an activation
 constexpr int kRows = 8;                       // rows of a token in the small operand
@@ -87,6 +88,7 @@ struct MoeArgs {
     uint8_t *xq, *xs;             // terms of x: [T][steps][kTermBytes], scales [T][kRows][steps * 8]
     uint8_t *aq, *as;             // terms of silu(g) u: the same for each pair
     float *y;                     // [split][T * k][H]
+    uint32_t *done;               // [groups] tiles of G that are finished
     int *status;
     int T, E, k, H, I, slots, ids64, renormalize, s13_align, s2_align;
     uint32_t inv_k;               // p / k = p * inv_k >> 16 for every pair p
@@ -109,11 +111,25 @@ struct Lists {
 };
 
 // ---- phase R ------------------------------------------------------------------
+// 8 x 8 transpose of nibbles over 8 lanes: lane r's nibble c goes to lane c's
+// nibble r.
+__device__ __forceinline__ uint32_t transpose_nibbles(uint32_t w, int r) {
+    uint32_t o = __shfl_xor_sync(0xFFFFFFFFu, w, 4);
+    w = r & 4 ? (w & 0xFFFF0000u) | (o >> 16) : (w & 0x0000FFFFu) | (o << 16);
+    o = __shfl_xor_sync(0xFFFFFFFFu, w, 2);
+    w = r & 2 ? (w & 0xFF00FF00u) | ((o >> 8) & 0x00FF00FFu) : (w & 0x00FF00FFu) | ((o & 0x00FF00FFu) << 8);
+    o = __shfl_xor_sync(0xFFFFFFFFu, w, 1);
+    return r & 1 ? (w & 0xF0F0F0F0u) | ((o >> 4) & 0x0F0F0F0Fu) : (w & 0x0F0F0F0Fu) | ((o & 0x0F0F0F0Fu) << 4);
+}
+
 // One block of 32 values, one a lane, as terms: codes to `codes` (16 bytes of
 // row 0, rows 128 bytes apart, 16-byte pieces swizzled by the row) and scale
-// bytes to `scales` (rows `stride` apart).
+// bytes to `scales` (rows `stride` apart).  A term needs the one before it, so
+// only that chain is in the loop: a lane collects its six codes in a word and
+// the words are transposed together.
 __device__ __forceinline__ void write_terms(float v, uint8_t *codes, uint8_t *scales, int stride, int piece, int lane) {
-#pragma unroll 1
+    uint32_t word = 0, my_byte = 0;
+#pragma unroll
     for (int q = 0; q < kTerms; ++q) {
         const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v) & 0x7FFFFFFFu);
         const int e = (int)(m >> 23);
@@ -127,14 +143,13 @@ __device__ __forceinline__ void write_terms(float v, uint8_t *codes, uint8_t *sc
             : "f"(v * inv), "f"(0.f));
         const uint32_t h = e2m1x2_to_f16x2(c);
         v = fmaf(-__low2float(*reinterpret_cast<const __half2 *>(&h)), scale_value(byte), v);
-        uint32_t w = c & 15;
-        w |= __shfl_down_sync(0xFFFFFFFFu, w, 1) << 4;
-        w |= __shfl_down_sync(0xFFFFFFFFu, w, 2) << 8;
-        w |= __shfl_down_sync(0xFFFFFFFFu, w, 4) << 16;
-        if ((lane & 7) == 0)
-            *reinterpret_cast<uint32_t *>(codes + q * 128 + ((piece ^ q) << 4) + (lane >> 3) * 4) = w;
-        if (lane == 0) scales[q * stride] = (uint8_t)byte;
+        word |= c << (4 * q);
+        my_byte = lane == q ? (uint32_t)byte : my_byte;
     }
+    const int q = lane & 7;
+    word = transpose_nibbles(word, q);
+    if (q < kTerms) *reinterpret_cast<uint32_t *>(codes + q * 128 + ((piece ^ q) << 4) + (lane >> 3) * 4) = word;
+    if (lane < kTerms) scales[lane * stride] = (uint8_t)my_byte;
 }
 
 __device__ void convert_tokens(const MoeArgs &a, int gw, int nw, int lane) {
@@ -357,6 +372,8 @@ __device__ void build_lists(const MoeArgs &a, Lists &L, Scratch &S) {
 struct Phase {
     const CUtensorMap *map;
     const uint8_t *w_scales, *b_codes, *b_scales;
+    const uint32_t *done;  // where the terms are made by tiles of this launch: how many of a group's are finished
+    uint32_t done_tiles;   // and how many there are
     int groups, m_tiles, split, rows_m, rows, slot_rows, scale_slot_rows, second, blocks, steps, align, term_align;
     uint32_t inv_div;  // pair * inv_div >> 16: which terms are the pair's
 };
@@ -410,10 +427,31 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t b
                  : "memory");
 }
 
+// Waits (a converged warp, bounded) until the terms of a group are in memory,
+// and makes them visible to this thread's loads and copies.
+__device__ __forceinline__ bool wait_terms(const Phase &ph, int group, volatile int *abort, int *status) {
+    if (!ph.done) return true;
+    uint32_t n;
+    bool ok = false;
+#pragma unroll 1
+    for (uint32_t i = 1; !ok && i < kTries; ++i) {
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(ph.done + group) : "memory");
+        ok = n >= ph.done_tiles;
+        if (i % 256 == 0 && *abort) break;
+    }
+    asm volatile("fence.proxy.async;" ::: "memory");
+    if (!ok) {
+        *abort = 1;
+        *reinterpret_cast<volatile int *>(status) = WISP_ERR_TIMEOUT;
+    }
+    return __all_sync(0xFFFFFFFFu, ok);
+}
+
 // What of a role lives on from phase to phase.
 struct Cursor {
     RingPos<kStages> ring;
     RingPos<2> acc;
+    int first = 0;  // the scale group whose turn the next window is
 };
 
 __device__ __forceinline__ void load_weights(unsigned char *st, const Phase &ph, const Walk &t, int kb, uint64_t *bar) {
@@ -429,6 +467,8 @@ __device__ void run_copies(Control &C, unsigned char *stages, const Phase &ph, c
     const int lane = threadIdx.x & 31;
     int issued = C.issued;
     for (Walk t(ph); t.at(ph, L, C); t.next()) {
+        // (weights that need no terms are on their way: copy_early)
+        if (!wait_terms(ph, t.g, abort, status)) return;
         const uint8_t *terms =
             lane < t.n ? ph.b_codes + ((size_t)(L.pair[t.off + lane] * ph.inv_div >> 16) * ph.steps + t.kb0) * kTermBytes
                        : nullptr;
@@ -486,6 +526,10 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
     const int my_row = tid < 64 ? tid : ph.second + tid - 64;
     const int term_stride = ph.steps * kStepBlocks;
     auto point = [&] {
+        if (!wait_terms(ph, ahead.g, abort, status)) {
+            more = false;
+            return;
+        }
         const int row = ahead.m0 + my_row;
         pw = row < ph.rows ? ph.w_scales + ((int64_t)ahead.slot * ph.scale_slot_rows + row) * ph.blocks : nullptr;
         const int i = tid / kRows, q = tid % kRows;
@@ -523,7 +567,9 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
         if (moved && more) point();
     };
     RingPos<kStages> ring = cur.ring;
-    if (group == 1) {
+    int last = -1;  // the group that had the last window
+    if (group != cur.first && more) {
+        last = 1 - group;
         ring.skip(count());
         advance();
     }
@@ -532,6 +578,7 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
     while (true) {
         load();
         if (!x.count) break;
+        last = x.skip ? 1 - group : group;
 #pragma unroll
         for (int j = 0; j < kWindow; ++j) {
             if (j >= x.count) break;
@@ -549,8 +596,9 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
         }
         ring.skip(x.skip);
     }
-    // both groups have come past the phase's last stage
+    // both groups have come past the phase's last stage, and go on in turn
     cur.ring = ring;
+    if (last >= 0) cur.first = 1 - last;
 }
 
 // The whole warp walks, one lane issues.
@@ -636,7 +684,12 @@ __device__ void run_gate_up(Control &C, const Phase &ph, const Lists &L, Cursor 
                 write_terms(g / (1.f + __expf(-g)) * u, a.aq + ((size_t)p * steps_out + kb) * kTermBytes,
                             a.as + (size_t)p * kRows * stride + j0 / kBlock, stride, piece, lane);
             }
+        // the terms are read by copies and loads of other CTAs once the group's count says so; the barrier puts
+        // every warp's stores before the release, which costs one thread and not all of them a fence of the GPU
+        asm volatile("fence.proxy.async.global;" ::: "memory");
         epilogue_barrier();
+        if (quarter == 0 && lane == 0)
+            asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(a.done + tile.g) : "memory");
     }
 }
 
@@ -709,13 +762,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     convert_tokens(a, nw - 1 - gw, nw, lane);
     for (int i = tid; i < 2 * a.E; i += kThreads) (&S.tokens[0][0])[i] = 0;
+    for (int i = blockIdx.x * kThreads + tid; i < a.T * a.k; i += gridDim.x * kThreads) a.done[i] = 0;  // groups <= pairs
     asm volatile("fence.proxy.async;" ::: "memory");  // the terms are read by bulk copies
     cg::this_grid().sync();
     tc_fence_after();
 
     // S
     if (a.router) {
-        if (a.E <= 128)
+        if (a.E <= 128 && a.T <= kWarps) {
+            if (warp < a.T) route_tokens<4, 1>(a, L, S, warp, lane);
+        } else if (a.E <= 128)
             for (int t = warp; t < a.T; t += 2 * kWarps) route_tokens<4, 2>(a, L, S, t, lane);
         else
             for (int t = warp; t < a.T; t += kWarps)
@@ -735,13 +791,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         up.blocks = a.H / kBlock, up.steps = (up.blocks + kStepBlocks - 1) / kStepBlocks, up.align = a.s13_align;
         up.groups = L.n, up.m_tiles = (a.I + 63) / 64, up.split = 1, up.rows_m = 64;
         up.rows = 2 * a.I, up.slot_rows = a.w13_rows, up.scale_slot_rows = a.s13_rows, up.second = a.I;
-        up.inv_div = a.inv_k;
+        up.inv_div = a.inv_k, up.done = nullptr;
         down.map = &map2, down.w_scales = a.s2, down.b_codes = a.aq, down.b_scales = a.as;
         down.blocks = a.I / kBlock, down.steps = (down.blocks + kStepBlocks - 1) / kStepBlocks, down.align = a.s2_align;
         down.groups = L.n, down.m_tiles = (a.H + 127) / 128, down.rows_m = 128;
         down.split = pieces_of(down.steps);
         down.rows = a.H, down.slot_rows = a.w2_rows, down.scale_slot_rows = a.s2_rows, down.second = 64;
-        down.inv_div = 65536;
+        down.inv_div = 65536, down.done = a.done, down.done_tiles = up.m_tiles;
         // (pieces of D begin at whole 16-byte loads of scale bytes)
         up.term_align = up.steps % 2 ? 8 : 16, down.term_align = down.steps % 2 ? 8 : 16;
         const int unit = down.align >= 16 || down.term_align >= 16 ? 2 : 1;
@@ -749,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncthreads();
 
-    // G and D, by the same code
+    // G and D, by the same code and without a barrier between them: a tile of D waits for its group's tiles of G
     Cursor cur;
     int early = 0;
 #pragma unroll 1
@@ -767,16 +823,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 run_gate_up(C, ph, L, cur, a, ex, C.phase[1].steps);
             else
                 run_down(C, ph, L, cur, a);
-        } else {
+        } else if (warp < kSfWarp + kScaleGroups * kScaleGroupWarps) {
             run_scales(C, stages, ph, L, cur, a.status);
         }
         __syncwarp();
-        tc_fence_before();
-        asm volatile("fence.proxy.async;" ::: "memory");  // D's terms are read by bulk copies
-        cg::this_grid().sync();
-        asm volatile("fence.proxy.async;" ::: "memory");
-        tc_fence_after();
     }
+    tc_fence_before();
+    cg::this_grid().sync();
+    tc_fence_after();
 
     // C
     const int P = a.T * a.k, split = C.phase[1].split;
@@ -811,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 struct Workspace {
-    size_t logits, xq, xs, aq, as, y, bytes;
+    size_t logits, xq, xs, aq, as, y, done, bytes;
     Workspace(int T, int E, int k, int H, int I) {
         size_t at = 0;
         const auto take = [&](size_t n) { const size_t here = at; at += (n + 255) / 256 * 256; return here; };
@@ -822,6 +876,7 @@ struct Workspace {
         aq = take(P * down * kTermBytes);
         as = take(P * down * kRows * kStepBlocks);
         y = take((size_t)pieces_of((int)down) * P * H * 4);
+        done = take(P * 4);
         bytes = at;
     }
 };
@@ -902,6 +957,7 @@ extern "C" int wisp_mx4_moe(const void *x, int64_t x_stride, const void *router,
     a.logits = reinterpret_cast<float *>(ws + w.logits);
     a.xq = ws + w.xq, a.xs = ws + w.xs, a.aq = ws + w.aq, a.as = ws + w.as;
     a.y = reinterpret_cast<float *>(ws + w.y);
+    a.done = reinterpret_cast<uint32_t *>(ws + w.done);
     const int64_t hb = hidden / 2, ib = inter / 2;
     const int64_t packed[4] = {2 * inter * hb, 2 * inter * (hb / 16), hidden * ib, hidden * (ib / 16)};
     const int64_t *st = slot_strides ? slot_strides : packed;

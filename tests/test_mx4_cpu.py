@@ -58,7 +58,7 @@ def test_python_refusals():
     x = torch.zeros(2, 64)
     with pytest.raises(ValueError, match="CUDA"):
         mx4_quantize(x)
-    with pytest.raises(TypeError, match="tensor"):
+    with pytest.raises(TypeError, match="Tensor"):
         mx4_quantize([1.0])
     codes, scales = ref.quantize(x)
     with pytest.raises(ValueError, match="CUDA"):

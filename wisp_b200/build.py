@@ -1,4 +1,5 @@
-"""Build ``wisp_b200/lib/libwisp_b200.so`` from ``wisp_b200/csrc`` with nvcc.
+"""Build ``wisp_b200/lib/libwisp_b200.so`` from ``wisp_b200/csrc`` with nvcc, and the Python binding of the stateless
+operators (``wisp_b200/lib/_wisp_bind.so``, ``csrc/bind.cpp`` against torch's headers) with g++.
 
 sm_100a only (B200).  The library links the CUDA runtime statically and
 reaches no driver symbol at load time, so it also loads (for symbol checks)
@@ -21,6 +22,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libwisp_b200.so")
+BIND_SRC = os.path.join(CSRC, "bind.cpp")
+BIND = os.path.join(LIBDIR, "_wisp_bind.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -48,8 +51,32 @@ def _stale() -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def build_bind(force: bool = False) -> str:
+    """The Python binding; it finds ``libwisp_b200.so`` beside itself."""
+    header = os.path.join(INCLUDE, "wisp_b200.h")
+    if not force and os.path.exists(BIND) and all(os.path.getmtime(p) <= os.path.getmtime(BIND)
+                                                  for p in (BIND_SRC, header)):
+        return BIND
+    import sysconfig
+
+    import torch
+    tree = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    inc = [os.path.join(tree, "include"), os.path.join(tree, "include", "torch", "csrc", "api", "include"),
+           os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    tmp = BIND + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{p}" for p in inc], BIND_SRC,
+           "-o", tmp, f"-L{LIBDIR}", "-lwisp_b200", "-Wl,-rpath,$ORIGIN", f"-L{os.path.join(tree, 'lib')}", "-lc10",
+           "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, BIND)
+    return BIND
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not _stale():
+        build_bind()
         return LIB
     os.makedirs(LIBDIR, exist_ok=True)
     objdir = os.path.join(LIBDIR, "_obj")
@@ -73,6 +100,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     tmp = LIB + ".tmp"
     subprocess.run([nvcc, *ARCH, "-shared", "-cudart", "static", "-o", tmp, *objs], check=True)
     os.replace(tmp, LIB)
+    build_bind(force)
     return LIB
 
 

@@ -191,19 +191,23 @@ __device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulA
         return more;
     };
     struct Window {
-        uint2 a[kWindow], w[2][kWindow];
+        ScaleWords<kWindow> a, w[2];
+        uint32_t a_shift, w_shift[2];
         int count, skip;  // stages of the window, and of the other group's window behind it
+        int left;         // scale bytes of a row from here on
     } x, next;
     auto load = [&](Window &x) {
         x.count = count();
         if (!more) return;
-        const int left = a.blocks - kb * kStepBlocks;
+        x.left = a.blocks - kb * kStepBlocks;
+        x.a.zero(), x.w[0].zero(), x.w[1].zero();
+        if (pa) x.a.load(pa + kb * kStepBlocks, x.count, x.left, a.align);
+        x.a_shift = row_shift(pa);
 #pragma unroll
-        for (int i = 0; i < kWindow; ++i) x.a[i] = x.w[0][i] = x.w[1][i] = make_uint2(0, 0);
-        if (pa) load_window<kWindow>(x.a, pa + kb * kStepBlocks, x.count, left, a.align);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (pw[i]) load_window<kWindow>(x.w[i], pw[i] + kb * kStepBlocks, x.count, left, a.align);
+        for (int i = 0; i < 2; ++i) {
+            if (pw[i]) x.w[i].load(pw[i] + kb * kStepBlocks, x.count, x.left, a.align);
+            x.w_shift[i] = row_shift(pw[i]);
+        }
         bool moved = advance();
         x.skip = count();
         moved |= advance();
@@ -223,13 +227,16 @@ __device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulA
             if (j >= x.count) break;
             if (!warp_wait(&C.empty[ring.slot], ring.turn ^ 1, abort, a.status)) return;
             unsigned char *sfa = sf + ring.slot * kStageBytes, *sfw = sfa + kSfABytes;
-            *reinterpret_cast<uint32_t *>(sfa) = x.a[j].x;
-            *reinterpret_cast<uint32_t *>(sfa + kAtomBytes) = x.a[j].y;
-            *reinterpret_cast<uint32_t *>(sfw) = x.w[0][j].x;
-            *reinterpret_cast<uint32_t *>(sfw + 2 * kAtomBytes) = x.w[0][j].y;
+            uint2 v = x.a.stage(j, x.a_shift, x.left);
+            *reinterpret_cast<uint32_t *>(sfa) = v.x;
+            *reinterpret_cast<uint32_t *>(sfa + kAtomBytes) = v.y;
+            v = x.w[0].stage(j, x.w_shift[0], x.left);
+            *reinterpret_cast<uint32_t *>(sfw) = v.x;
+            *reinterpret_cast<uint32_t *>(sfw + 2 * kAtomBytes) = v.y;
             if (tid < kTileN - 128) {
-                *reinterpret_cast<uint32_t *>(sfw + kAtomBytes) = x.w[1][j].x;
-                *reinterpret_cast<uint32_t *>(sfw + 3 * kAtomBytes) = x.w[1][j].y;
+                v = x.w[1].stage(j, x.w_shift[1], x.left);
+                *reinterpret_cast<uint32_t *>(sfw + kAtomBytes) = v.x;
+                *reinterpret_cast<uint32_t *>(sfw + 3 * kAtomBytes) = v.y;
             }
             fence_async_shared();
             __syncwarp();

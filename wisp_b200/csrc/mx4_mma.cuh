@@ -102,7 +102,9 @@ __device__ __forceinline__ bool wait_tries(uint64_t *bar, uint32_t parity, const
     return true;
 }
 // The same; a wait that runs out sets the status and the CTA's abort word.
-// (One copy of the loop for a kernel's many waits: see load_unaligned_scales.)
+// (One copy of the loop for a kernel's many waits: roles that run at the same
+// time share one instruction cache.  A kernel of 228 KB, everything inlined and
+// unrolled, spent as long on fetching instructions as on memory.)
 static __device__ __noinline__ bool wait_long(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
     if (wait_tries(bar, parity, abort)) return true;
     *abort = 1;
@@ -144,61 +146,56 @@ __device__ __forceinline__ uint2 first_bytes(uint2 v, int left) {
     }
     return v;
 }
-// The scale bytes of a window of a row, of which `left` are the row's (the
-// others: 0), where the rows are not aligned to 8 bytes.  Not inlined: kernels
-// whose roles run at the same time share one instruction cache, and this is
-// the rare case (inlined and unrolled everywhere it made a kernel of 228 KB,
-// which spent as long on fetching instructions as on memory).
+// A window's scale bytes of a row as they were loaded: aligned words.
+// stage() shifts them into place where they are used, so that nothing waits for
+// a load where it is issued.
 template <int WINDOW>
-struct ScaleWindow {
-    uint2 v[WINDOW];
-};
-template <int WINDOW>
-__device__ __noinline__ ScaleWindow<WINDOW> load_unaligned_scales(const uint8_t *p, int count, int left, int align) {
-    ScaleWindow<WINDOW> r;
+struct ScaleWords {
+    uint32_t w[2 * WINDOW + 1];
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < WINDOW; ++i) {
-        uint2 v = make_uint2(0, 0);
-        const int n = i < count ? left - i * kStepBlocks : 0;
-        const uint8_t *q = p + i * kStepBlocks;
-        if (align >= 4) {
-            if (n > 0) v.x = __ldg(reinterpret_cast<const uint32_t *>(q));
-            if (n > 4) v.y = __ldg(reinterpret_cast<const uint32_t *>(q) + 1);
+        for (int i = 0; i <= 2 * WINDOW; ++i) w[i] = 0;
+    }
+    // The eight bytes of the window's j-th stage; `shift`: bits by which the row
+    // is out of its words, `left`: bytes of the row from the window's first on.
+    __device__ __forceinline__ uint2 stage(int j, uint32_t shift, int left) const {
+        const uint2 v = make_uint2(__funnelshift_r(w[2 * j], w[2 * j + 1], shift),
+                                   __funnelshift_r(w[2 * j + 1], w[2 * j + 2], shift));
+        return first_bytes(v, left - j * kStepBlocks);
+    }
+    // `count` stages from p on, `left` bytes of which are the row's.  `align`:
+    // what p is aligned to.  Rows of any alignment are read as the 32-bit words
+    // that hold a byte of theirs.  NC: through the read-only path.
+    template <bool NC = true>
+    __device__ __forceinline__ void load(const uint8_t *p, int count, int left, int align) {
+        static_assert(WINDOW % 2 == 0, "pairs of stages");
+        if (align >= 16) {
+#pragma unroll
+            for (int i = 0; i < WINDOW; i += 2)
+                if (i < count) {
+                    const uint4 r = NC ? __ldg(reinterpret_cast<const uint4 *>(p) + i / 2) : ld_cg16(p + i * kStepBlocks);
+                    w[2 * i] = r.x, w[2 * i + 1] = r.y, w[2 * i + 2] = r.z, w[2 * i + 3] = r.w;
+                }
+        } else if (align >= 8) {
+#pragma unroll
+            for (int i = 0; i < WINDOW; ++i)
+                if (i < count) {
+                    const uint2 r = NC ? __ldg(reinterpret_cast<const uint2 *>(p) + i)
+                                       : __ldcg(reinterpret_cast<const uint2 *>(p) + i);
+                    w[2 * i] = r.x, w[2 * i + 1] = r.y;
+                }
         } else {
-#pragma unroll 1
-            for (int j = 0; j < min(n, 8); ++j) {
-                const uint32_t b = (uint32_t)__ldg(q + j) << (8 * (j & 3));
-                v.x |= j < 4 ? b : 0, v.y |= j < 4 ? 0 : b;
-            }
+            const int off = (int)(reinterpret_cast<uintptr_t>(p) & 3), bytes = min(left, count * kStepBlocks) + off;
+            const uint32_t *q = reinterpret_cast<const uint32_t *>(p - off);
+#pragma unroll
+            for (int i = 0; i <= 2 * WINDOW; ++i)
+                if (4 * i < bytes) w[i] = __ldg(q + i);
         }
-        r.v[i] = v;
     }
-    return r;
-}
-// A window's scale bytes of a row, `count` stages of them from p on; `left` of
-// them are the row's (what comes for the others is not defined where the rows
-// are aligned to 8 bytes, else 0).  `align`: what p is aligned to.  NC: through
-// the read-only path.  With aligned rows nothing here waits for what it loads.
-template <int WINDOW, bool NC = true>
-__device__ __forceinline__ void load_window(uint2 (&v)[WINDOW], const uint8_t *p, int count, int left, int align) {
-    static_assert(WINDOW % 2 == 0, "pairs of stages");
-    if (align >= 16) {
-#pragma unroll
-        for (int i = 0; i < WINDOW; i += 2)
-            if (i < count) {
-                const uint4 r = NC ? __ldg(reinterpret_cast<const uint4 *>(p) + i / 2) : ld_cg16(p + i * kStepBlocks);
-                v[i] = make_uint2(r.x, r.y), v[i + 1] = make_uint2(r.z, r.w);
-            }
-    } else if (align >= 8) {
-#pragma unroll
-        for (int i = 0; i < WINDOW; ++i)
-            if (i < count)
-                v[i] = NC ? __ldg(reinterpret_cast<const uint2 *>(p) + i) : __ldcg(reinterpret_cast<const uint2 *>(p) + i);
-    } else {
-        const ScaleWindow<WINDOW> r = load_unaligned_scales<WINDOW>(p, count, left, align);
-#pragma unroll
-        for (int i = 0; i < WINDOW; ++i) v[i] = r.v[i];
-    }
+};
+// Bits by which a row of scale bytes is out of its words.
+__device__ __forceinline__ uint32_t row_shift(const uint8_t *p) {
+    return (uint32_t)(reinterpret_cast<uintptr_t>(p) & 3) * 8;
 }
 // What a matrix's rows of scale bytes are aligned to.
 __host__ __device__ inline int scale_align(const void *scales, int blocks) {

@@ -548,7 +548,8 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
         return more;
     };
     struct Window {
-        uint2 w[kWindow], b[kWindow];
+        ScaleWords<kWindow> w, b;
+        uint32_t w_shift;
         int count, skip;  // stages of the window, and of the other group's window behind it
         int left;         // scale bytes of a row from here on
     } x;
@@ -556,11 +557,10 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
         x.count = count();
         if (!more) return;
         x.left = ph.blocks - kb * kStepBlocks;
-#pragma unroll
-        for (int i = 0; i < kWindow; ++i) x.w[i] = x.b[i] = make_uint2(0, 0);
-        if (pw) load_window<kWindow>(x.w, pw + kb * kStepBlocks, x.count, x.left, ph.align);
-        if (pb)  // written by this kernel
-            load_window<kWindow, false>(x.b, pb + kb * kStepBlocks, x.count, x.left, ph.term_align);
+        x.w.zero(), x.b.zero();
+        if (pw) x.w.load(pw + kb * kStepBlocks, x.count, x.left, ph.align);
+        x.w_shift = row_shift(pw);
+        if (pb) x.b.load<false>(pb + kb * kStepBlocks, x.count, x.left, ph.term_align);  // written by this kernel
         bool moved = advance();
         x.skip = count();
         moved |= advance();
@@ -584,9 +584,9 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
             if (j >= x.count) break;
             if (!warp_wait(&C.empty[ring.slot], ring.turn ^ 1, abort, status)) return;
             unsigned char *at = sf + ring.slot * kStageBytes;
-            const uint2 terms = first_bytes(x.b[j], x.left - j * kStepBlocks);
-            *reinterpret_cast<uint32_t *>(at) = x.w[j].x;
-            *reinterpret_cast<uint32_t *>(at + kAtomBytes) = x.w[j].y;
+            const uint2 scales = x.w.stage(j, x.w_shift, x.left), terms = x.b.stage(j, 0, x.left);
+            *reinterpret_cast<uint32_t *>(at) = scales.x;
+            *reinterpret_cast<uint32_t *>(at + kAtomBytes) = scales.y;
             *reinterpret_cast<uint32_t *>(at + 2 * kAtomBytes) = terms.x;
             *reinterpret_cast<uint32_t *>(at + 3 * kAtomBytes) = terms.y;
             fence_async_shared();

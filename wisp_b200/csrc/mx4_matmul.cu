@@ -10,7 +10,8 @@
 // columns' weights in L2.  192 columns, because two accumulators (the epilogue
 // of a tile runs while the next one accumulates) and the scales of every ring
 // stage have to fit 512 columns of tensor memory; of the widths that do, a
-// wider tile reads A less often.
+// wider tile reads A less often.  Few tiles are 64 columns wide (Narrow).  The
+// steps along K are the same, and so are the bits.
 //
 // 14 warps: TMA producer (4 stages of 256 values of K: 16 KB of A, 24 KB of
 // W), MMA issuer, 4 epilogue warps, 8 warps that bring the scale bytes.  These
@@ -19,8 +20,10 @@
 // memory through registers, ahead of their use; no TMA box can make that
 // arrangement.
 //
-// Bound by HBM for few rows a group (the weights are read once), for many by
-// L2: a stage brings 40 KB for 4 instructions of 96 cycles each.
+// Bound by HBM for few rows a group (the weights are read once): EXPERTS.
+// For many it is the tensor cores and the power they may draw: WIDE.
+// For one small product it is latency: 11 us at 16 rows x 4096 x 4096 on 64
+// CTAs, of which a launch and the first loads are 6.
 #include "mx4_mma.cuh"
 
 namespace wisp {
@@ -30,21 +33,30 @@ namespace {
 
 __device__ int g_status = 0;
 
-constexpr int kTileM = 128, kTileN = 192;
-constexpr int kStages = 4;
-constexpr int kABytes = kTileM * 128, kBBytes = kTileN * 128;
-constexpr int kSfABytes = 2 * kAtomBytes, kSfBBytes = 4 * kAtomBytes;  // [two halves of K][row atoms]
-constexpr int kStageBytes = kABytes + kBBytes + kSfABytes + kSfBBytes;
-constexpr int kSfCols = 24;                    // of a stage: two halves of 4 (A) + 8 (W) columns
-constexpr int kSfCol0 = 2 * kTileN;            // behind the two accumulators
-static_assert(kSfCol0 + kStages * kSfCols <= 512, "tensor memory");
-constexpr int kTmemCols = 512;
+constexpr int kTileM = 128;
 constexpr int kEpiWarp = 2, kSfWarp = 6;
 constexpr int kThreads = (kSfWarp + kScaleGroups * kScaleGroupWarps) * 32;
 constexpr int kMaxGroups = 1024;
 constexpr int kWindow = 2;  // stages of a window of scale bytes
-static_assert(kStages > kWindow, "a parity wait has to know its phase");
-constexpr int kOutBytes = 32 * 128;           // staging of an epilogue warp: 32 rows of 64 columns
+constexpr int kTmemCols = 512;
+constexpr int kOutBytes = 32 * 128;  // staging of an epilogue warp: 32 rows of 64 columns
+
+// The sizes that follow from a tile's columns.
+template <int N, int STAGES>
+struct Shape {
+    static constexpr int kTileN = N, kStages = STAGES;
+    static constexpr int kABytes = kTileM * 128, kBBytes = kTileN * 128;
+    static constexpr int kWAtoms = (kTileN + 127) / 128;  // row atoms of W's scales
+    static constexpr int kSfABytes = 2 * kAtomBytes, kSfBBytes = 2 * kWAtoms * kAtomBytes;  // [two halves of K][row atoms]
+    static constexpr int kStageBytes = kABytes + kBBytes + kSfABytes + kSfBBytes;
+    static constexpr int kSfHalf = 4 + 4 * kWAtoms;  // columns of tensor memory: A's atom, W's
+    static constexpr int kSfCols = 2 * kSfHalf;      // of a stage
+    static constexpr int kSfCol0 = 2 * kTileN;       // behind the two accumulators
+    static constexpr int kCols = kTileN < 64 ? kTileN : 64;  // the epilogue's piece
+    static_assert(kSfCol0 + kStages * kSfCols <= kTmemCols, "tensor memory");
+    static_assert(kStages > kWindow, "a parity wait has to know its phase");
+    static_assert(kTileN % kCols == 0 && kTileN <= 256, "tile");
+};
 
 struct MatmulArgs {
     const int32_t *offsets;  // [groups + 1], or nullptr: one group of all rows
@@ -55,8 +67,9 @@ struct MatmulArgs {
     int groups, N, blocks, align, vec_out;
 };
 
+template <class S>
 struct Control {
-    uint64_t full[kStages], sf_full[kStages], empty[kStages];
+    uint64_t full[S::kStages], sf_full[S::kStages], empty[S::kStages];
     uint64_t acc_full[2], acc_empty[2], mma_done;
     uint32_t tmem_base;
     int abort, issued, consumed;
@@ -74,17 +87,18 @@ __device__ __forceinline__ void group_rows(const MatmulArgs &a, int g, int &begi
 
 // A CTA's walk over the tiles of all groups, gridDim.x apart; row tiles fastest
 // within a group.  For a converged warp: 32 groups are looked at together.
+template <class S>
 struct Walk {
     int t, tiles, ntiles_n, g = 0;
     // the tile: first row, rows of the group from there on, first column, its row of W
     int row0, rows, n0, wrow0;
-    __device__ __forceinline__ Walk(const Control &C, const MatmulArgs &a) {
-        ntiles_n = (a.N + kTileN - 1) / kTileN;
+    __device__ __forceinline__ Walk(const Control<S> &C, const MatmulArgs &a) {
+        ntiles_n = (a.N + S::kTileN - 1) / S::kTileN;
         tiles = C.first[a.groups] * ntiles_n;
         t = blockIdx.x;
     }
     // False behind the last tile.
-    __device__ __forceinline__ bool at(const Control &C, const MatmulArgs &a) {
+    __device__ __forceinline__ bool at(const Control<S> &C, const MatmulArgs &a) {
         if (t >= tiles) return false;
         const int lane = threadIdx.x & 31;
         while (true) {  // groups that end before this tile
@@ -99,7 +113,7 @@ struct Walk {
         group_rows(a, g, begin, end);
         row0 = begin + (in - n * mtiles) * kTileM;
         rows = end - row0;
-        n0 = n * kTileN;
+        n0 = n * S::kTileN;
         wrow0 = g * a.N + n0;
         return true;
     }
@@ -107,7 +121,8 @@ struct Walk {
 };
 
 // Row tiles of every group.
-__device__ void scan_groups(Control &C, const MatmulArgs &a) {
+template <class S>
+__device__ void scan_groups(Control<S> &C, const MatmulArgs &a) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kPer = (kMaxGroups + kThreads - 1) / kThreads;
     int count[kPer], own = 0;
@@ -141,33 +156,35 @@ __device__ void scan_groups(Control &C, const MatmulArgs &a) {
     __syncthreads();
 }
 
-__device__ void load_operands(Control &C, unsigned char *stages, const CUtensorMap *map_a, const CUtensorMap *map_w,
+template <class S>
+__device__ void load_operands(Control<S> &C, unsigned char *stages, const CUtensorMap *map_a, const CUtensorMap *map_w,
                               const MatmulArgs &a, int steps) {
     volatile int *abort = &C.abort;
-    RingPos<kStages> ring;
+    RingPos<S::kStages> ring;
     int issued = 0;
-    for (Walk t(C, a); t.at(C, a); t.next())
+    for (Walk<S> t(C, a); t.at(C, a); t.next())
         for (int kb = 0; kb < steps; ++kb, ring.next()) {
             if (!warp_wait(&C.empty[ring.slot], ring.turn ^ 1, abort, a.status)) return;
             if (elect_one()) {
-                unsigned char *st = stages + ring.slot * kStageBytes;
-                mbar_expect_tx(&C.full[ring.slot], kABytes + kBBytes);
+                unsigned char *st = stages + ring.slot * S::kStageBytes;
+                mbar_expect_tx(&C.full[ring.slot], S::kABytes + S::kBBytes);
                 tma_load_2d(st, map_a, kb * 128, t.row0, &C.full[ring.slot]);
-                tma_load_2d(st + kABytes, map_w, kb * 128, t.wrow0, &C.full[ring.slot]);
+                tma_load_2d(st + S::kABytes, map_w, kb * 128, t.wrow0, &C.full[ring.slot]);
                 C.issued = ++issued;
             }
         }
 }
 
-__device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulArgs &a, int steps) {
+template <class S>
+__device__ void load_all_scales(Control<S> &C, unsigned char *stages, const MatmulArgs &a, int steps) {
     const int group = (threadIdx.x >> 5) - kSfWarp >= kScaleGroupWarps;
     const int tid = threadIdx.x % (kScaleGroupWarps * 32);
     volatile int *abort = &C.abort;
     const int64_t wrows = (int64_t)a.groups * a.N;
-    unsigned char *sf = stages + kABytes + kBBytes + atom_at(tid);
-    RingPos<kStages> ring;
+    unsigned char *sf = stages + S::kABytes + S::kBBytes + atom_at(tid);
+    RingPos<S::kStages> ring;
     // the loads run DEEP of the group's windows ahead of the stores
-    Walk ahead(C, a);
+    Walk<S> ahead(C, a);
     bool more = ahead.at(C, a);
     int kb = 0;
     const uint8_t *pa = nullptr, *pw[2] = {};  // rows of the tile
@@ -177,7 +194,7 @@ __device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulA
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int64_t rw = (int64_t)ahead.wrow0 + tid + i * 128;
-            pw[i] = tid + i * 128 < kTileN && rw < wrows ? a.w_scales + rw * a.blocks : nullptr;
+            pw[i] = tid + i * 128 < S::kTileN && rw < wrows ? a.w_scales + rw * a.blocks : nullptr;
         }
     };
     auto count = [&] { return more ? min(kWindow, steps - kb) : 0; };
@@ -226,17 +243,17 @@ __device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulA
         for (int j = 0; j < kWindow; ++j) {
             if (j >= x.count) break;
             if (!warp_wait(&C.empty[ring.slot], ring.turn ^ 1, abort, a.status)) return;
-            unsigned char *sfa = sf + ring.slot * kStageBytes, *sfw = sfa + kSfABytes;
+            unsigned char *sfa = sf + ring.slot * S::kStageBytes, *sfw = sfa + S::kSfABytes;
             uint2 v = x.a.stage(j, x.a_shift, x.left);
             *reinterpret_cast<uint32_t *>(sfa) = v.x;
             *reinterpret_cast<uint32_t *>(sfa + kAtomBytes) = v.y;
             v = x.w[0].stage(j, x.w_shift[0], x.left);
             *reinterpret_cast<uint32_t *>(sfw) = v.x;
-            *reinterpret_cast<uint32_t *>(sfw + 2 * kAtomBytes) = v.y;
-            if (tid < kTileN - 128) {
+            *reinterpret_cast<uint32_t *>(sfw + S::kWAtoms * kAtomBytes) = v.y;
+            if (tid < S::kTileN - 128) {
                 v = x.w[1].stage(j, x.w_shift[1], x.left);
                 *reinterpret_cast<uint32_t *>(sfw + kAtomBytes) = v.x;
-                *reinterpret_cast<uint32_t *>(sfw + 3 * kAtomBytes) = v.y;
+                *reinterpret_cast<uint32_t *>(sfw + (S::kWAtoms + 1) * kAtomBytes) = v.y;
             }
             fence_async_shared();
             __syncwarp();
@@ -252,42 +269,45 @@ __device__ void load_all_scales(Control &C, unsigned char *stages, const MatmulA
 // The whole warp walks, one lane issues.  While the unit works off three of a
 // stage's four products the warp waits for the next stage: the waits take as
 // long as two products even when there is nothing to wait for.
-__device__ void issue_products(Control &C, unsigned char *stages, const MatmulArgs &a, int steps) {
+template <class S>
+__device__ void issue_products(Control<S> &C, unsigned char *stages, const MatmulArgs &a, int steps) {
     volatile int *abort = &C.abort;
     const uint32_t base = s_addr(stages), tmem = C.tmem_base;
-    const uint64_t a0 = smem_desc_k_sw128(base), b0 = smem_desc_k_sw128(base + kABytes),
-                   sf0 = smem_desc_atom(base + kABytes + kBBytes);
-    RingPos<kStages> ring;
+    const uint64_t a0 = smem_desc_k_sw128(base), b0 = smem_desc_k_sw128(base + S::kABytes),
+                   sf0 = smem_desc_atom(base + S::kABytes + S::kBBytes);
+    RingPos<S::kStages> ring;
     RingPos<2> accs;
     int consumed = 0;
     bool ready = false;  // whether the stage at `ring` has been waited for
-    auto wait_stage = [&](const RingPos<kStages> &at) {
+    auto wait_stage = [&](const RingPos<S::kStages> &at) {
         return warp_wait(&C.full[at.slot], at.turn, abort, a.status) &&
                warp_wait(&C.sf_full[at.slot], at.turn, abort, a.status);
     };
-    for (Walk t(C, a); t.at(C, a); t.next(), accs.next()) {
+    for (Walk<S> t(C, a); t.at(C, a); t.next(), accs.next()) {
         if (!warp_wait(&C.acc_empty[accs.slot], accs.turn ^ 1, abort, a.status)) return;
         tc_fence_after();
-        const uint32_t acc = tmem + accs.slot * kTileN;
+        const uint32_t acc = tmem + accs.slot * S::kTileN;
         const bool last_tile = t.t + (int)gridDim.x >= t.tiles;
         for (int kb = 0; kb < steps; ++kb) {
             if (!ready && !wait_stage(ring)) return;
             tc_fence_after();
             const int s = ring.slot;
             // addresses are in units of 16 bytes; 64 values are 32 bytes further along K
-            const uint64_t step = (uint64_t)(s * (kStageBytes >> 4));
+            const uint64_t step = (uint64_t)(s * (S::kStageBytes >> 4));
             const uint64_t da = a0 + step, db = b0 + step, ds = sf0 + step;
-            const uint32_t cols = tmem + kSfCol0 + s * kSfCols;
+            const uint32_t cols = tmem + S::kSfCol0 + s * S::kSfCols;
             auto product = [&](int kk) {
-                umma_mxf4(acc, da + kk * 2, db + kk * 2, idesc_mxf4(kTileM, kTileN, (kk & 1) * 2), cols + (kk >> 1) * 12,
-                          cols + (kk >> 1) * 12 + 4, kb | kk);
+                umma_mxf4(acc, da + kk * 2, db + kk * 2, idesc_mxf4(kTileM, S::kTileN, (kk & 1) * 2), cols + (kk >> 1) * S::kSfHalf,
+                          cols + (kk >> 1) * S::kSfHalf + 4, kb | kk);
             };
             if (elect_one()) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    copy_atom(cols + h * 12, ds + h * (kAtomBytes >> 4));
-                    copy_atom(cols + h * 12 + 4, ds + ((kSfABytes + h * 2 * kAtomBytes) >> 4));
-                    copy_atom(cols + h * 12 + 8, ds + ((kSfABytes + (h * 2 + 1) * kAtomBytes) >> 4));
+                    const uint32_t to = cols + h * S::kSfHalf;
+                    copy_atom(to, ds + h * (kAtomBytes >> 4));
+#pragma unroll
+                    for (int i = 0; i < S::kWAtoms; ++i)
+                        copy_atom(to + 4 + i * 4, ds + ((S::kSfABytes + (h * S::kWAtoms + i) * kAtomBytes) >> 4));
                 }
                 product(0);
                 product(1);
@@ -311,21 +331,22 @@ __device__ void issue_products(Control &C, unsigned char *stages, const MatmulAr
 // Epilogue warps: 64 columns at a time through shared memory (16-byte pieces
 // swizzled by the row), so that a store instruction writes 128 bytes of four
 // rows and not 16 bytes of 32.
-__device__ void store_tiles(Control &C, unsigned char *staging, const MatmulArgs &a) {
+template <class S>
+__device__ void store_tiles(Control<S> &C, unsigned char *staging, const MatmulArgs &a) {
     volatile int *abort = &C.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3;
     unsigned char *mine = staging + (warp - kEpiWarp) * kOutBytes;
     RingPos<2> accs;
-    for (Walk t(C, a); t.at(C, a); t.next(), accs.next()) {
+    for (Walk<S> t(C, a); t.at(C, a); t.next(), accs.next()) {
         if (!warp_wait(&C.acc_full[accs.slot], accs.turn, abort, a.status)) return;
         tc_fence_after();
-        const int rows = t.rows - quarter * 32, cols = min(kTileN, a.N - t.n0);
+        const int rows = t.rows - quarter * 32, cols = min(S::kTileN, a.N - t.n0);
         __nv_bfloat16 *out = a.out + ((int64_t)t.row0 + quarter * 32) * a.N + t.n0;
-        const uint32_t taddr = C.tmem_base + accs.slot * kTileN + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t taddr = C.tmem_base + accs.slot * S::kTileN + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
-        for (int c0 = 0; c0 < cols && rows > 0; c0 += 64) {
+        for (int c0 = 0; c0 < cols && rows > 0; c0 += S::kCols) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < S::kCols / 32; ++h) {
                 uint32_t v[32];
                 gemm::tmem_ld32(taddr + c0 + h * 32, v);
 #pragma unroll
@@ -338,12 +359,12 @@ __device__ void store_tiles(Control &C, unsigned char *staging, const MatmulArgs
                 }
             }
             __syncwarp();
-            const int c = c0 + (lane & 7) * 8;
+            const int c = c0 + (lane & 7) * 8, end = min(cols, c0 + S::kCols);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int r = i * 4 + (lane >> 3);
                 const uint4 v = *reinterpret_cast<const uint4 *>(mine + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-                if (r >= rows || c >= cols) continue;
+                if (r >= rows || c >= end) continue;
                 __nv_bfloat16 *at = out + (int64_t)r * a.N + c;
                 if (a.vec_out) {
                     *reinterpret_cast<uint4 *>(at) = v;
@@ -351,7 +372,7 @@ __device__ void store_tiles(Control &C, unsigned char *staging, const MatmulArgs
                     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                     for (int x = 0; x < 8; ++x)
-                        if (c + x < cols)
+                        if (c + x < end)
                             at[x] = __ushort_as_bfloat16((unsigned short)(x & 1 ? w[x / 2] >> 16 : w[x / 2]));
                 }
             }
@@ -363,16 +384,17 @@ __device__ void store_tiles(Control &C, unsigned char *staging, const MatmulArgs
     }
 }
 
+template <class S>
 __global__ void __launch_bounds__(kThreads, 1)
     matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                   const MatmulArgs a) {
     extern __shared__ unsigned char raw[];
     unsigned char *stages = raw + ((1024u - (s_addr(raw) & 1023u)) & 1023u);
-    unsigned char *staging = stages + kStages * kStageBytes;
-    Control &C = *reinterpret_cast<Control *>(staging + 4 * kOutBytes);
+    unsigned char *staging = stages + S::kStages * S::kStageBytes;
+    Control<S> &C = *reinterpret_cast<Control<S> *>(staging + 4 * kOutBytes);
     const int tid = threadIdx.x, warp = tid >> 5;
     if (tid == 0) {
-        for (int s = 0; s < kStages; ++s) {
+        for (int s = 0; s < S::kStages; ++s) {
             mbar_init(&C.full[s], 1);
             mbar_init(&C.sf_full[s], kScaleGroupWarps);
             mbar_init(&C.empty[s], 1);
@@ -408,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // after an abort: copies and products in flight end before the memory is given back
         volatile int no_abort = 0;
         for (int k = C.consumed; k < C.issued; ++k)
-            wait_tries(&C.full[k % kStages], (k / kStages) & 1, &no_abort);
+            wait_tries(&C.full[k % S::kStages], (k / S::kStages) & 1, &no_abort);
         wait_tries(&C.mma_done, 0, &no_abort);
     }
     __syncthreads();
@@ -417,8 +439,26 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 int *g_words[64] = {};  // address of g_status on each device
 
-constexpr int kSmemBytes = kStages * kStageBytes + 4 * kOutBytes + 1024 + sizeof(Control);
-static_assert(kSmemBytes <= 232448, "shared memory");
+template <class S>
+int launch(const CUtensorMap &ma, const void *w_codes, const MatmulArgs &a, int64_t tiles, int sms, cudaStream_t stream) {
+    constexpr int kSmemBytes = S::kStages * S::kStageBytes + 4 * kOutBytes + 1024 + sizeof(Control<S>);
+    static_assert(kSmemBytes <= 232448, "shared memory");
+    CUtensorMap mw;
+    if (const int rc = gemm::make_byte_map(&mw, w_codes, (uint64_t)a.groups * a.N, a.blocks * (kBlock / 2), S::kTileN))
+        return rc;
+    WISP_CUDA_TRY(cudaFuncSetAttribute(matmul_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+    matmul_kernel<S><<<(unsigned)(tiles < sms ? tiles : sms), kThreads, kSmemBytes, stream>>>(ma, mw, a);
+    WISP_CUDA_TRY(cudaGetLastError());
+    return WISP_OK;
+}
+using Wide = Shape<192, 4>;
+// Where the tiles are so few that SMs would go without: the time is then the
+// latency of a tile's steps, which narrow tiles, with more stages in flight,
+// shorten (us, narrow against wide, 16 rows x 4096 x 4096: 11.0, 12.3; 40
+// groups of 223 rows x 180 x 3200: 11.0, 12.4; 128 x 9472 x 2048: 8.8, 10.2).
+// With more narrow tiles than SMs the wide ones win (512 x 4096 x 4096: 18.4,
+// 13.8); 32 columns were no better anywhere (13.1 at the first size).
+using Narrow = Shape<64, 7>;
 
 }  // namespace
 
@@ -445,7 +485,7 @@ extern "C" int wisp_mx4_matmul(const void *a_codes, const void *a_scales, int64_
         k % kBlock || k > (1 << 24))
         return set_error("wisp_mx4_matmul: need 0 <= rows <= 2^30, 1 to 1024 groups, n >= 1, k a multiple of 32"),
                WISP_ERR_INVALID;
-    if ((int64_t)groups * n > INT32_MAX || rows * ((n + kTileN - 1) / kTileN) > ((int64_t)1 << 36))
+    if ((int64_t)groups * n > INT32_MAX || rows * ((n + Wide::kTileN - 1) / Wide::kTileN) > ((int64_t)1 << 36))
         return set_error("wisp_mx4_matmul: groups * n or rows * n too large"), WISP_ERR_INVALID;
     if (!offsets && groups != 1) return set_error("wisp_mx4_matmul: several groups need offsets"), WISP_ERR_INVALID;
     if (rows == 0) return WISP_OK;
@@ -455,9 +495,8 @@ extern "C" int wisp_mx4_matmul(const void *a_codes, const void *a_scales, int64_
         if (reinterpret_cast<uintptr_t>(p) % 16)
             return set_error("wisp_mx4_matmul: codes must be aligned to 16 bytes"), WISP_ERR_INVALID;
     if (reinterpret_cast<uintptr_t>(out) % 2) return set_error("wisp_mx4_matmul: unaligned out"), WISP_ERR_INVALID;
-    CUtensorMap ma, mw;
+    CUtensorMap ma;
     if (const int rc = gemm::make_byte_map(&ma, a_codes, rows, k / 2, kTileM)) return rc;
-    if (const int rc = gemm::make_byte_map(&mw, w_codes, (uint64_t)groups * n, k / 2, kTileN)) return rc;
     MatmulArgs a{};
     a.offsets = offsets;
     a.a_scales = reinterpret_cast<const uint8_t *>(a_scales);
@@ -471,13 +510,12 @@ extern "C" int wisp_mx4_matmul(const void *a_codes, const void *a_scales, int64_
     int dev = 0, sms = 0;
     WISP_CUDA_TRY(cudaGetDevice(&dev));
     WISP_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    WISP_CUDA_TRY(cudaFuncSetAttribute(matmul_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
-    // no more CTAs than tiles there can be (every group may end in a partial one)
-    const int64_t most = (rows / kTileM + groups) * ((n + kTileN - 1) / kTileN);
-    matmul_kernel<<<(unsigned)(most < sms ? most : sms), kThreads, kSmemBytes, reinterpret_cast<cudaStream_t>(stream)>>>(
-        ma, mw, a);
-    WISP_CUDA_TRY(cudaGetLastError());
-    return WISP_OK;
+    // no more tiles than this (every group may end in a partial one)
+    const int64_t row_tiles = rows / kTileM + groups;
+    auto tiles = [&](int width) { return row_tiles * ((n + width - 1) / width); };
+    const auto on = reinterpret_cast<cudaStream_t>(stream);
+    if (tiles(Narrow::kTileN) <= sms) return launch<Narrow>(ma, w_codes, a, tiles(Narrow::kTileN), sms, on);
+    return launch<Wide>(ma, w_codes, a, tiles(Wide::kTileN), sms, on);
 }
 
 extern "C" int wisp_mx4_sync(void *stream) {

@@ -79,6 +79,37 @@ def test_groups(counts, n, k, rest):
         assert bool((out[~done] == 7.0).all()) and int((~done).sum()) == rest * n
 
 
+def moved(q, offset):
+    """The same matrix with its scale bytes `offset` bytes behind a 256-byte boundary, between bytes of another value."""
+    from wisp_b200.mx4 import Mx4Tensor
+    n = q.scales.numel()
+    buffer = torch.full((n + 512,), 255, dtype=torch.uint8, device=DEV)
+    scales = buffer[256 + offset:256 + offset + n].view(q.scales.shape)
+    scales.copy_(q.scales)
+    return Mx4Tensor(q.codes, scales)
+
+
+@pytest.mark.parametrize("k", [32, 96, 256, 288, 1120, 2048])
+@pytest.mark.parametrize("offset", [1, 2, 3, 4, 7, 8, 16])
+def test_scale_rows_of_any_alignment(k, offset):
+    from wisp_b200.mx4 import mx4_matmul, mx4_synchronize
+    a, w = random_mx4((150, k), 3), random_mx4((210, k), 4)
+    want = mx4_matmul(a, w)
+    check(want, a, w)
+    for x, y in ((moved(a, offset), w), (a, moved(w, offset)), (moved(a, offset), moved(w, 3))):
+        assert torch.equal(mx4_matmul(x, y), want)
+    mx4_synchronize()
+
+
+@pytest.mark.parametrize("n,k", [(500, 672), (64, 32), (1000, 2048)])
+def test_bits_do_not_depend_on_the_rows_beside(n, k):
+    """Few rows go through narrow tiles, many through wide ones: the same sums in the same order."""
+    from wisp_b200.mx4 import mx4_matmul
+    a, w = random_mx4((20000, k), 5), random_mx4((n, k), 6)
+    few, many = mx4_matmul(a[300:333], w), mx4_matmul(a, w)
+    assert torch.equal(few, many[300:333])
+
+
 def test_special_scales():
     """Scales at both ends, a NaN scale in one row of each operand, rows of zeros."""
     from wisp_b200.mx4 import mx4_matmul

@@ -1,8 +1,11 @@
 """``mx4_moe`` against the 64-bit oracle over the dequantised experts.
 
 Tolerance, element by element.  The output is rounded to bf16 once: 2^-8 of
-it.  silu(g) u is rounded to bf16 once: 2^-8 of every term, so at most 2^-8 of
-``size``, the sum of the terms' magnitudes; the exponential and the quotient
+it.  x and silu(g) u go into the products as six MXFP4 terms, which leave at
+most 2^-12 of the largest value of a block of 32 (a term leaves less than a
+quarter); 2^-8 of ``size``, the sum of the terms' magnitudes, is what one
+rounding of silu(g) u to bf16 could cost, and holds the kernel to that.  The
+exponential and the quotient
 add less than 2^-18 of it, the routing weights (softmax of fp32 logits: the
 error of a logit is at most (H / 256 + 8) 2^-24 of the magnitudes that meet in
 it, here below 64) less than 2^-14, and the fp32 sums of the down product at
@@ -126,6 +129,25 @@ def test_activations_of_any_size(size):
         assert float(out.abs().max()) < 2.0 ** -110
     else:
         check(out, x, w13, w2, w, ids)
+
+
+@pytest.mark.parametrize("H,I", [(96, 32), (288, 160), (1056, 544), (512, 256)])
+@pytest.mark.parametrize("offset", [1, 2, 4, 8])
+def test_scale_rows_of_any_alignment(H, I, offset):
+    """Scale bytes that begin anywhere, between bytes of NaN: the same bits."""
+    from wisp_b200.mx4 import Mx4Tensor, mx4_moe, mx4_synchronize
+    w13, w2, router = layer(6, H, I, seed=9)
+    x = tokens(5, H)
+    want = mx4_moe(x, w13, w2, 3, router=router)
+
+    def moved(q):
+        buffer = torch.full((q.scales.numel() + 512,), 255, dtype=torch.uint8, device=DEV)
+        scales = buffer[256 + offset:256 + offset + q.scales.numel()].view(q.scales.shape)
+        return Mx4Tensor(q.codes, scales.copy_(q.scales))
+
+    assert torch.equal(mx4_moe(x, moved(w13), w2, 3, router=router), want)
+    assert torch.equal(mx4_moe(x, moved(w13), moved(w2), 3, router=router), want)
+    mx4_synchronize()
 
 
 def test_zero_token_and_non_finite_token_stay_apart():

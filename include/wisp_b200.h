@@ -149,7 +149,7 @@ WISP_API int wisp_mx4_matmul(const void *a_codes, const void *a_scales, int64_t 
                              void *out, void *stream);
 /*
  * Wait for `stream` and report (then clear) a bounded wait that ran out inside
- * wisp_mx4_matmul on the current device (WISP_ERR_TIMEOUT).
+ * wisp_mx4_matmul or wisp_mx4_moe on the current device (WISP_ERR_TIMEOUT).
  */
 WISP_API int wisp_mx4_sync(void *stream);
 
@@ -181,9 +181,9 @@ WISP_API int wisp_mx4_moe_workspace(int32_t num_tokens, int32_t num_experts, int
 WISP_API int wisp_mx4_moe(const void *x, int64_t x_stride, const void *router, const void *topk_ids,
                           int32_t ids_int64, const float *topk_weights, const int32_t *expert_map,
                           const void *w13_codes, const void *w13_scales, const void *w2_codes, const void *w2_scales,
-                          const int64_t *slot_strides, int32_t num_slots, int32_t num_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,
-                          int32_t inter, int32_t renormalize, void *workspace, int64_t workspace_bytes, void *out,
-                          void *stream);
+                          const int64_t *slot_strides, int32_t num_slots, int32_t num_tokens, int32_t num_experts,
+                          int32_t top_k, int32_t hidden, int32_t inter, int32_t renormalize, void *workspace,
+                          int64_t workspace_bytes, void *out, void *stream);
 
 /*
  * The step between two blocks of a decoder layer:

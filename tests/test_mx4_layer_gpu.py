@@ -92,6 +92,26 @@ def test_resident_layer_and_errors():
     st.close()
 
 
+@pytest.mark.parametrize("mode,cap", [("paged", 3), ("resident", 6)])
+def test_routing_of_other_lengths_is_refused(mode, cap):
+    """Fewer rows of routing than tokens would leave rows of the result unwritten."""
+    from wisp_b200.integrations.vllm import WispMoEStateMX4
+    st = WispMoEStateMX4(*experts(6, 64, 32), cap, DEV, 0, mode=mode)
+    if mode == "resident":
+        st.prime_identity()
+    x = tokens(5, 64, 1)
+    for rows in (4, 6):
+        w, ids = routing(rows, 6, 2, rows)
+        with pytest.raises(ValueError, match="topk_weights"):
+            st.forward(x, w, ids)
+    w, ids = routing(5, 6, 2, 5)
+    with pytest.raises(ValueError, match="topk_weights"):
+        st.forward(x, w[:, :1], ids)
+    assert st.forward(x, w, ids).shape == (5, 64)
+    st.synchronize()
+    st.close()
+
+
 def test_a_token_does_not_depend_on_the_others():
     from wisp_b200.mx4 import mx4_moe
     w13, w2 = experts(20, 384, 4160)                      # several pieces of the intermediate size

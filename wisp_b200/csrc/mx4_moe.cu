@@ -929,9 +929,9 @@ extern "C" int wisp_mx4_moe_workspace(int32_t num_tokens, int32_t num_experts, i
 extern "C" int wisp_mx4_moe(const void *x, int64_t x_stride, const void *router, const void *topk_ids,
                             int32_t ids_int64, const float *topk_weights, const int32_t *expert_map,
                             const void *w13_codes, const void *w13_scales, const void *w2_codes, const void *w2_scales,
-                            const int64_t *slot_strides, int32_t num_slots, int32_t num_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,
-                            int32_t inter, int32_t renormalize, void *workspace, int64_t workspace_bytes, void *out,
-                            void *stream) {
+                            const int64_t *slot_strides, int32_t num_slots, int32_t num_tokens, int32_t num_experts,
+                            int32_t top_k, int32_t hidden, int32_t inter, int32_t renormalize, void *workspace,
+                            int64_t workspace_bytes, void *out, void *stream) {
     if (const int rc = check_shape(num_tokens, num_experts, top_k, hidden, inter, num_slots)) return rc;
     if (num_tokens == 0) return WISP_OK;
     if (!x || !w13_codes || !w13_scales || !w2_codes || !w2_scales || !workspace || !out)

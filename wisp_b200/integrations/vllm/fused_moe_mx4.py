@@ -68,6 +68,9 @@ class WispMoEStateMX4(WispMoEState):
             self._check_primed()
         if x.dim() != 2 or x.shape[1] != hidden:
             raise ValueError(f"x must be [T, {hidden}]; got {tuple(x.shape)}")
+        if topk_ids.dim() != 2 or topk_ids.shape[0] != x.shape[0] or topk_weights.shape != topk_ids.shape:
+            raise ValueError(f"topk_weights and topk_ids must be [{x.shape[0]}, k]; got {tuple(topk_weights.shape)} and "
+                             f"{tuple(topk_ids.shape)}")
         if out is None:
             out = torch.empty((x.shape[0], hidden), dtype=x.dtype, device=x.device)
         for a, b in self._groups(topk_ids):

@@ -51,6 +51,9 @@ def test_block_norm_refusals():
     refused(call(kind=4, gate=P), "gate_kind")
     refused(call(y=None), "NULL")
     refused(call(rows=2, stride=-64), "stride")
+    refused(call(y=P + 1), "aligned")
+    refused(call(gate=P + 1, kind=2), "aligned")
+    refused(call(y=P + 2, dtype=2, rdtype=2, wdtype=2), "aligned")
     assert call(rows=0) == _lib.WISP_OK
 
 

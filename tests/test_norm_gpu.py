@@ -67,6 +67,37 @@ def test_types(dtype, rdtype, wdtype, cols):
     run(*inputs(9, cols, dtype, rdtype, wdtype, True, "full"))
 
 
+@pytest.mark.parametrize("dtype,rdtype,wdtype", [(BF, BF, BF), (HF, FP, HF), (FP, FP, FP)])
+@pytest.mark.parametrize("gate,post", [("full", True), ("channel", False), ("token", True)])
+@pytest.mark.parametrize("cols", [2, 5, 8, 9, 131, 255, 257, 513, 770, 1025, 2047, 2049, 2562, 3329, 4097, 8191, 8194, 11001,
+                                  14001, 16383])
+def test_widths(cols, gate, post, dtype, rdtype, wdtype):
+    """Rows that begin anywhere in a 16-byte granule, of every length class."""
+    run(*inputs(11, cols, dtype, rdtype, wdtype, post, gate))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 4, 5, 700, 20000])
+@pytest.mark.parametrize("cols", [33, 301, 801, 1203])
+def test_many_short_rows(rows, cols):
+    run(*inputs(rows, cols, BF, BF, BF, True, "none"))
+
+
+def test_outputs_leave_their_neighbours_alone():
+    """Outputs in the middle of a buffer, each beginning at an odd value: nothing beside them changes."""
+    from wisp_b200.norm import block_norm
+    for cols in (7, 301, 2803):
+        y, res = torch.randn(5, cols, device=DEV).bfloat16(), torch.randn(5, cols, device=DEV).bfloat16()
+        w = torch.randn(cols, device=DEV).bfloat16()
+        n = 5 * cols
+        buffer = torch.full((2 * n + 64,), 7.0, dtype=torch.bfloat16, device=DEV)
+        out, res_out = buffer[13:13 + n].view(5, cols), buffer[n + 29:2 * n + 29].view(5, cols)
+        block_norm(y, res, w, out=out, residual_out=res_out)
+        want, want_res = block_norm(y, res, w)
+        assert torch.equal(out, want) and torch.equal(res_out, want_res)
+        beside = torch.cat((buffer[:13], buffer[13 + n:n + 29], buffer[2 * n + 29:]))
+        assert bool((beside == 7.0).all())
+
+
 def test_zero_rows_and_row_of_zeros():
     from wisp_b200.norm import block_norm
     y, r, w, p, gt = inputs(4, 256, BF, BF, BF, True, "token")

@@ -21,11 +21,12 @@
 // arrangement.
 //
 // Measured: 128 experts x 128 rows x 1536 x 2048 (282 MB to read and write)
-// 56 us, 5.1 TB/s, the weights read once (232 MB from HBM, 709 MB through L2),
-// two to three tiles a CTA and their first and last steps not hidden.  8
-// experts x 512 rows x 28672 x 4096 (962 GFLOP) 281 us, 3.4 PFLOP/s; back to
-// back the power limit makes that 330 us.  One small product is latency: 16 x
-// 4096 x 4096 takes 10.7 us, of which a launch and the first loads are 6.
+// 56 us, 5.1 TB/s, the weights read once (232 MB from HBM, 709 MB through L2:
+// a ragged group has one or two row tiles).  8 experts x 512 rows x 28672 x
+// 4096 (962 GFLOP) 281 us, 3.4 PFLOP/s, 43 KB of L2 a stage and SM, 11.7 TB/s
+// over the chip; back to back the power limit makes that 340 us.  One small
+// product is latency: 16 x 4096 x 4096 takes 10.7 us, of which a launch and the
+// first loads are 6.
 #include "mx4_mma.cuh"
 
 namespace wisp {

@@ -55,7 +55,7 @@ def run(y, r, w, p, gt, scale=0.5, eps=1e-6):
 @pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
 @pytest.mark.parametrize("post", [False, True])
 @pytest.mark.parametrize("rows,cols", [(1, 2048), (7, 2050), (301, 4096), (1200, 63), (3, 1), (2, 16384), (5, 16383),
-                                       (4, 8192), (3, 5122)])
+                                       (4, 8192), (3, 5122), (300, 5120), (300, 8192), (200, 12288)])
 def test_matches_oracle(rows, cols, post, gate):
     run(*inputs(rows, cols, BF, BF, BF, post, gate))
 
@@ -127,6 +127,16 @@ def test_strides_dims_and_unaligned():
     compare(block_norm(y.to(DEV), r.to(DEV), w.to(DEV), gate=t2), y, r, w, None, gt[:, 3:4], 1.0, 1e-6)
     v = block_norm(y[0].to(DEV), r[0].to(DEV), w.to(DEV))
     compare(v, y[0], r[0], w, None, None, 1.0, 1e-6)
+
+
+@pytest.mark.parametrize("cols", [33, 301, 1147, 2803, 4104, 6144, 7168])
+def test_in_place_rows_of_any_width(cols):
+    """Rows share 16-byte granules with their neighbours, which other CTAs overwrite."""
+    from wisp_b200.norm import block_norm
+    y, r, w, p, gt = (None if t is None else t.to(DEV) for t in inputs(3000, cols, BF, BF, BF, True, "full"))
+    n, rn = block_norm(y, r, w, post_weight=p, gate=gt)
+    n2, rn2 = block_norm(y, r, w, post_weight=p, gate=gt, out=y, residual_out=r)
+    assert n2.data_ptr() == y.data_ptr() and torch.equal(n2, n) and torch.equal(rn2, rn)
 
 
 def test_in_place_and_deterministic():

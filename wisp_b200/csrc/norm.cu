@@ -505,6 +505,16 @@ int dispatch(const NormArgs &a, cudaStream_t stream) {
         if (cols <= 8 * 64) return launch<T, R, W, 8, 64, 1>(a, stream);
         if (cols <= 8 * 256) return launch<T, R, W, 8, 256, 1>(a, stream);
         if (cols <= 8 * 512) return launch<T, R, W, 8, 256, 2>(a, stream);
+        // more threads a row cost more in the reductions, more pieces a thread registers (of fp32 first): 4000 x 7168 bf16
+        // 42 us with 256 x 4, 48 with 512 x 2, 67 with 1024 x 2; 2863 x 7296 fp32 90, 78, 95; 3000 x 12288 bf16 54 with
+        // 512 x 3, 75 with 1024 x 2
+        if (sizeof(T) == 4) {
+            if (cols <= 8 * 1024) return launch<T, R, W, 8, 512, 2>(a, stream);
+        } else {
+            if (cols <= 8 * 768) return launch<T, R, W, 8, 256, 3>(a, stream);
+            if (cols <= 8 * 1024) return launch<T, R, W, 8, 256, 4>(a, stream);
+        }
+        if (cols <= 8 * 1536) return launch<T, R, W, 8, 512, 3>(a, stream);
         return launch<T, R, W, 8, 1024, 2>(a, stream);
     }
     // pairs of values: 8191 x 2050 48 us, shifted 62 to 68; but 9000 x 3074 68 us, shifted 57

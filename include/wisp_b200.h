@@ -213,6 +213,16 @@ WISP_API int wisp_ensure_resident(wisp_layer *layer, const void *ids, int32_t id
                          void *stream);
 
 /*
+ * Kernels of the caller read the slots or the expert map of a paged layer:
+ * called once they are queued on `stream`, before anything else is asked of
+ * the layer.  Page-ins, prefetches, resizes and the layer's end then wait for
+ * them; experts (host, n ids) become the layer's last unique set, which a
+ * prefetch keeps out of its victims.  (wisp_moe_forward does this for its
+ * own kernels.)  Not for a stream that is being captured.
+ */
+WISP_API int wisp_layer_used(wisp_layer *layer, const int32_t *experts, int32_t n, void *stream);
+
+/*
  * Pager side of one forward without the expert compute: first-fit groups, one
  * LRU step per group, page-in, finished before returning; writes the slot each
  * (token, k) read to slots_out (host, [T][k]; may be NULL).  The test and replay

@@ -1,0 +1,146 @@
+"""What else is asked of a layer of 4-bit experts while a forward's kernels are still queued: prefetches, forwards on
+other streams, other threads.  A kernel is held up by a spin on its stream, put between a forward's admission and its
+launch, so that whatever does not wait for it comes first."""
+import threading
+
+import pytest
+import torch
+
+from oracle.pager import PagerOracle
+from tests.test_mx4_layer_gpu import DEV, experts, tokens
+
+pytestmark = pytest.mark.gpu
+E, H, I = 12, 256, 128
+
+
+@pytest.fixture()
+def held_up(monkeypatch):
+    """mx4_moe as the layer calls it, behind a spin of some 30 ms on its stream."""
+    from wisp_b200.integrations.vllm import fused_moe_mx4 as m
+    real = m.mx4_moe
+
+    def late(x, *args, **kwargs):
+        torch.cuda._sleep(50_000_000)
+        return real(x, *args, **kwargs)
+    monkeypatch.setattr(m, "mx4_moe", late)
+    return real
+
+
+def route_to(sets, seed=0):
+    """(weights, ids) of one token for each set of experts."""
+    ids = torch.tensor([list(s) for s in sets], dtype=torch.int32, device=DEV)
+    w = torch.rand(ids.shape, generator=torch.Generator().manual_seed(seed)).to(DEV)
+    return w, ids
+
+
+def test_prefetch_waits_for_a_queued_forward_and_spares_its_experts(held_up):
+    from wisp_b200.integrations.vllm import WispMoEStateMX4
+    w13, w2 = experts(E, H, I)
+    st, oracle = WispMoEStateMX4(w13, w2, 6, DEV, 0), PagerOracle(E, 6)
+    x = tokens(2, H, 1)
+    assert st.last_unique_experts == set()
+    for step, (sets, predicted) in enumerate([
+            (((0, 1, 2), (1, 2, 3)), {8, 9, 10, 11}),      # 4 in use, 2 free: the prediction is cut to 2
+            (((4, 5, 0), (5, 0, 1)), {6, 7}),              # those of the forward are no victims
+            (((4, 5, 0), (3, 2, 1)), {8, 9, 10}),          # every slot in use: nothing is loaded
+    ]):
+        w, ids = route_to(sets, step)
+        out = st.forward(x, w, ids)
+        done = torch.cuda.Event()
+        done.record()
+        st.prefetch_async(predicted)
+        assert done.query(), "the prefetch did not wait for the forward"
+        st.synchronize()
+        assert torch.equal(out, held_up(x, w13, w2, topk_weights=w, topk_ids=ids))
+        used = set().union(*sets)
+        assert st.last_unique_experts == used
+        oracle.ensure_resident(ids.cpu().numpy())
+        oracle.prefetch_async(predicted, used)
+        s2e, tick, clock, stats = st._read()
+        assert (s2e, tick, clock) == (oracle.slot_to_expert, oracle.lru_tick, oracle.lru_clock)
+        assert stats[1:] == oracle.stats()[1:]
+    st.close()
+
+
+def test_forwards_on_two_streams_wait_for_one_another(held_up):
+    """Each evicts every expert of the one before it."""
+    from wisp_b200.integrations.vllm import WispMoEStateMX4
+    w13, w2 = experts(E, H, I, 1)
+    st = WispMoEStateMX4(w13, w2, 4, DEV, 0)
+    x = tokens(1, H, 2)
+    jobs = []
+    for n in range(6):
+        w, ids = route_to([[4 * (n % 3) + j for j in range(4)]], n)
+        jobs.append((torch.cuda.Stream(), w, ids))
+    torch.cuda.synchronize()
+    outs = []
+    for stream, w, ids in jobs:
+        with torch.cuda.stream(stream):
+            outs.append(st.forward(x, w, ids))
+    torch.cuda.synchronize()
+    for out, (_, w, ids) in zip(outs, jobs):
+        assert torch.equal(out, held_up(x, w13, w2, topk_weights=w, topk_ids=ids))
+    st.close()
+
+
+def test_threads_share_a_layer(held_up):
+    """Forwards and prefetches of two threads: an admission and its kernels belong together."""
+    from wisp_b200.integrations.vllm import WispMoEStateMX4
+    w13, w2 = experts(E, H, I, 2)
+    st = WispMoEStateMX4(w13, w2, 4, DEV, 0)
+    x = tokens(3, H, 3)
+    jobs = [route_to([[(5 * n + 3 * t + j) % E for j in range(3)] for t in range(3)], n) for n in range(12)]
+    torch.cuda.synchronize()
+    outs, errors = [None] * len(jobs), []
+
+    def work(first):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for n in range(first, len(jobs), 2):
+                    outs[n] = st.forward(x, *jobs[n])
+                    st.prefetch_async({(7 * n + j) % E for j in range(4)})
+        except Exception as e:                              # noqa: BLE001  (reported below)
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for out, (w, ids) in zip(outs, jobs):
+        assert torch.equal(out, held_up(x, w13, w2, topk_weights=w, topk_ids=ids))
+    st.close()
+
+
+def test_a_failed_forward_leaves_its_first_groups_covered(held_up):
+    from wisp_b200 import _lib
+    from wisp_b200.integrations.vllm import WispMoEStateMX4
+    st = WispMoEStateMX4(*experts(E, H, I, 3), 3, DEV, 0)
+    x = tokens(2, H, 4)
+    w, ids = route_to([(0, 1, 2), (3, 4, E)])
+    out = torch.empty_like(x)
+    with pytest.raises(_lib.WispError, match="outside"):
+        st.forward(x, w, ids, out=out)
+    assert st.last_unique_experts == {0, 1, 2}
+    st.synchronize()
+    st.close()
+
+
+def test_used_refuses_what_it_cannot_cover():
+    import ctypes
+
+    from wisp_b200 import _lib
+    from wisp_b200.integrations.vllm import WispMoEStateMX4
+    L = _lib.lib()
+    st = WispMoEStateMX4(*experts(4, 64, 32), 2, DEV, 0)
+    ids = (ctypes.c_int32 * 2)(1, 4)
+    assert L.wisp_layer_used(None, ids, 1, None) == _lib.WISP_ERR_INVALID
+    assert L.wisp_layer_used(st._h, None, 1, None) == _lib.WISP_ERR_INVALID
+    assert L.wisp_layer_used(st._h, ids, -1, None) == _lib.WISP_ERR_INVALID
+    assert L.wisp_layer_used(st._h, ids, 2, None) == _lib.WISP_ERR_BAD_EXPERT
+    assert L.wisp_layer_used(st._h, ids, 1, None) == _lib.WISP_OK and st.last_unique_experts == {1}
+    st.close()
+    st = WispMoEStateMX4(*experts(4, 64, 32), 4, DEV, 0, mode="resident")
+    assert L.wisp_layer_used(st._h, ids, 1, None) == _lib.WISP_ERR_INVALID
+    st.close()

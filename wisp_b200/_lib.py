@@ -61,6 +61,7 @@ SIGNATURES = {
                                        _c_int32, _c_int32, _c_int64, _c_int32, ctypes.c_float, ctypes.c_float,
                                        _vp, _vp, _vp]),
     "wisp_ensure_resident": (ctypes.c_int, [_vp, _vp, _c_int32, _c_int32, _vp]),
+    "wisp_layer_used": (ctypes.c_int, [_vp, _p32, _c_int32, _vp]),
     "wisp_pager_step": (ctypes.c_int, [_vp, _vp, _c_int32, _c_int32, _c_int32, _vp, _vp]),
     "wisp_prefetch_async": (ctypes.c_int, [_vp, _p32, _c_int32, _vp]),
     "wisp_prime_identity": (ctypes.c_int, [_vp, _vp]),

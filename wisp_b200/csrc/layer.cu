@@ -146,7 +146,7 @@ struct wisp_layer {
     uint32_t *d_last_unique = nullptr;  // bitmap of the last paged forward's unique experts
     uint32_t h_last_unique[32] = {};    // host copy, valid when the host read the last forward's mailbox
     bool last_unique_host = false;
-    int32_t *h_pf = nullptr, *d_pf = nullptr;  // prefetch: predicted ids [E], then status / records (mapped)
+    int32_t *h_pf = nullptr, *d_pf = nullptr;  // prefetch: predicted ids [E], status / records, unique set (mapped)
     cudaEvent_t ev_pf = nullptr;
     unsigned int *d_bar = nullptr;
     unsigned int *d_flow = nullptr;  // forward-kernel dataflow words (kFlowWords)
@@ -1045,7 +1045,7 @@ static int layer_create_impl(int32_t num_experts, int32_t cap_experts, int32_t h
         cudaEventCreateWithFlags(&L->ev_copies, cudaEventDisableTiming) != cudaSuccess ||
         cudaEventCreateWithFlags(&L->ev_last, cudaEventDisableTiming) != cudaSuccess ||
         cudaEventCreateWithFlags(&L->ev_pf, cudaEventDisableTiming) != cudaSuccess ||
-        cudaHostAlloc(&L->h_pf, sizeof(int32_t) * ((size_t)num_experts + kMbRec * (num_experts + 1)),
+        cudaHostAlloc(&L->h_pf, sizeof(int32_t) * ((size_t)num_experts + kMbRec * (num_experts + 1) + 32),
                       cudaHostAllocMapped) != cudaSuccess ||
         cudaHostGetDevicePointer((void **)&L->d_pf, L->h_pf, 0) != cudaSuccess)
         return bail(fail(WISP_ERR_CUDA, "wisp_layer_create: buffer/stream/event setup failed"));
@@ -1185,6 +1185,27 @@ int wisp_ensure_resident(wisp_layer *L, const void *ids, int32_t ids_int64, int3
     return WISP_OK;
 }
 
+int wisp_layer_used(wisp_layer *L, const int32_t *experts, int32_t n, void *stream) {
+    if (!L) return fail(WISP_ERR_INVALID, "wisp_layer_used: NULL layer");
+    if (n < 0 || (n > 0 && !experts)) return fail(WISP_ERR_INVALID, "wisp_layer_used: bad experts");
+    if (L->mode != WISP_MODE_PAGED) return fail(WISP_ERR_INVALID, "wisp_layer_used: layer is not paged");
+    uint32_t words[32] = {};
+    for (int i = 0; i < n; ++i) {
+        if (experts[i] < 0 || experts[i] >= L->E)
+            return fail(WISP_ERR_BAD_EXPERT, "wisp_layer_used: expert id outside [0, " + std::to_string(L->E) + ")");
+        words[experts[i] >> 5] |= 1u << (experts[i] & 31);
+    }
+    std::lock_guard<std::mutex> lk(L->mu);
+    DeviceGuard guard(L->dev);
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    WISP_CUDA_TRY(cudaStreamWaitEvent(s, L->ev_last, 0));  // the event goes on to cover what it covered
+    WISP_CUDA_TRY(cudaEventRecord(L->ev_last, s));
+    L->last_stream_set = false;
+    std::copy(words, words + 32, L->h_last_unique);
+    L->last_unique_host = true;
+    return WISP_OK;
+}
+
 int wisp_pager_step(wisp_layer *L, const void *topk_ids, int32_t ids_int64, int32_t num_tokens,
                     int32_t top_k, int32_t *slots_out, void *stream) {
     if (!L) return fail(WISP_ERR_INVALID, "wisp_pager_step: NULL layer");
@@ -1232,6 +1253,11 @@ int wisp_prefetch_async(wisp_layer *L, const int32_t *predicted, int32_t n, void
     p.hdr = L->d_hdr;
     p.slot_gen = L->d_slot_gen;
     p.last_unique = L->d_last_unique;
+    if (L->last_unique_host) {  // the host's copy is the newer one after wisp_layer_used
+        const size_t at = (size_t)L->E + kMbRec * ((size_t)L->E + 1);
+        std::copy(L->h_last_unique, L->h_last_unique + 32, reinterpret_cast<uint32_t *>(L->h_pf + at));
+        p.last_unique = reinterpret_cast<const uint32_t *>(L->d_pf + at);
+    }
     p.out = L->d_pf + L->E;
     // on the copy stream, after this layer's last forward is done with its
     // slots and state; the next forward's pager waits for these copies

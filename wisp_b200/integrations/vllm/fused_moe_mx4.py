@@ -10,6 +10,9 @@ projection; the compute (:func:`wisp_b200.mx4.mx4_moe`) reads the slots as they 
 """
 from __future__ import annotations
 
+import ctypes
+import threading
+
 import torch
 
 from wisp_b200 import _lib
@@ -29,7 +32,11 @@ class WispMoEStateMX4(WispMoEState):
     :class:`~wisp_b200.mx4.Mx4Tensor` (``H`` and ``I`` multiples of 32), on the CPU or a GPU; they are copied into
     pinned host memory.  The pager, counters and paging methods are those of :class:`WispMoEState`;
     ``slots_w13`` / ``slots_w2`` view the slots as ``Mx4Tensor``.  ``mode``: ``"paged"`` or ``"resident"``.  Hits,
-    misses and evictions are counted; forwards are not (a forward here is one or more admission steps)."""
+    misses and evictions are counted; forwards are not (a forward here is one or more admission steps).
+
+    A paged forward's kernels read the slots after it has returned.  The layer knows of them (``wisp_layer_used``), so
+    that later page-ins, prefetches and resizes wait for them, on whichever stream they run; a lock keeps another
+    thread's calls from coming between a forward's admission and its kernels."""
 
     def __init__(self, w13: Mx4Tensor, w2: Mx4Tensor, cap_experts: int, device, layer_idx: int,
                  mode: str = _Mode.PAGED) -> None:
@@ -38,6 +45,7 @@ class WispMoEStateMX4(WispMoEState):
             raise ValueError(f"w13 [E, 2I, H] and w2 [E, H, I] do not match: {tuple(w13.shape)} and {tuple(w2.shape)}")
         self._mx4_shape = (int(hidden), int(inter2) // 2)
         self._primed = False
+        self._lock = threading.RLock()
         super().__init__(_blocks(w13), _blocks(w2), cap_experts, mode, device, layer_idx)
 
     def _refresh_views(self) -> None:
@@ -61,8 +69,7 @@ class WispMoEStateMX4(WispMoEState):
         (int32 or int64).  A paged call admits the experts of its tokens group by group: consecutive tokens, at most
         64 and as many as the cap holds the experts of (first fit, fused_moe.py:1102-1168); a token that routes to
         more experts than the cap raises ``RuntimeError`` (mentioning sub-batch).  A token's result does not depend
-        on the groups, the cap or the slots.  Calls on several streams have to be ordered by the caller: a page-in
-        waits for the work of the stream of its own call."""
+        on the groups, the cap or the slots."""
         hidden, _ = self._mx4_shape
         if self.mode == _Mode.RESIDENT:
             self._check_primed()
@@ -73,21 +80,37 @@ class WispMoEStateMX4(WispMoEState):
                              f"{tuple(topk_ids.shape)}")
         if out is None:
             out = torch.empty((x.shape[0], hidden), dtype=x.dtype, device=x.device)
-        for a, b in self._groups(topk_ids):
-            if self.mode != _Mode.RESIDENT:
-                self.ensure_resident(topk_ids[a:b])
+
+        def compute(a, b):
             mx4_moe(x[a:b], self.slots_w13, self.slots_w2, topk_weights=topk_weights[a:b], topk_ids=topk_ids[a:b],
                     expert_map=self.expert_map_device, out=out[a:b])
+
+        if self.mode == _Mode.RESIDENT:
+            for a in range(0, x.shape[0], MOE_MAX_TOKENS):
+                compute(a, min(a + MOE_MAX_TOKENS, x.shape[0]))
+            return out
+        rows = topk_ids.tolist()        # the pager's step waits for the device too
+        with self._lock:
+            done = 0
+            try:
+                for a, b in self._groups(rows):
+                    self.ensure_resident(topk_ids[a:b])
+                    compute(a, b)
+                    done = b
+            finally:
+                if done:
+                    self._used(set().union(*rows[:done]))
         return out
 
-    def _groups(self, topk_ids: torch.Tensor):
+    def _used(self, experts: set) -> None:
+        """The kernels queued on the current stream read the slots of ``experts``."""
+        ids = (ctypes.c_int32 * len(experts))(*experts)
+        _lib.check(_lib.lib().wisp_layer_used(self._h, ids, len(ids), _lib.stream_ptr(
+            torch.cuda.current_stream(self.device))), "layer_used")
+
+    def _groups(self, rows: list):
         """Ranges of tokens that one kernel call takes."""
-        tokens = topk_ids.shape[0]
-        if self.mode == _Mode.RESIDENT:
-            yield from ((a, min(a + MOE_MAX_TOKENS, tokens)) for a in range(0, tokens, MOE_MAX_TOKENS))
-            return
-        rows = topk_ids.tolist()        # the pager's step waits for the device too
-        a, held = 0, set()
+        tokens, a, held = len(rows), 0, set()
         for t, row in enumerate(rows):
             both = held | set(row)
             if t > a and (t - a == MOE_MAX_TOKENS or len(both) > self.cap_experts):
@@ -111,6 +134,22 @@ class WispMoEStateMX4(WispMoEState):
         """Resident mode: identity map and full copy (fused_moe.py:242-258)."""
         super().prime_identity()
         self._primed = True
+
+    def ensure_resident(self, needed_experts: torch.Tensor) -> None:
+        with self._lock:
+            super().ensure_resident(needed_experts)
+
+    def pager_step(self, topk_ids: torch.Tensor):
+        with self._lock:
+            return super().pager_step(topk_ids)
+
+    def prefetch_async(self, predicted_experts) -> None:
+        with self._lock:
+            super().prefetch_async(predicted_experts)
+
+    def resize_cap(self, new_cap: int) -> None:
+        with self._lock:
+            super().resize_cap(new_cap)
 
     def _check_primed(self) -> None:
         if not self._primed:

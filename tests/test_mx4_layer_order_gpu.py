@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle.pager import PagerOracle
-from tests.test_mx4_layer_gpu import DEV, experts, tokens
+from tests.test_mx4_layer_gpu import DEV, experts, routing, tokens
 
 pytestmark = pytest.mark.gpu
 E, H, I = 12, 256, 128
@@ -124,6 +124,23 @@ def test_a_failed_forward_leaves_its_first_groups_covered(held_up):
         st.forward(x, w, ids, out=out)
     assert st.last_unique_experts == {0, 1, 2}
     st.synchronize()
+    st.close()
+
+
+def test_primed_experts_are_there_for_every_stream():
+    from wisp_b200.integrations.vllm import WispMoEStateMX4
+    from wisp_b200.mx4 import mx4_moe
+    w13, w2 = experts(48, 1024, 1024, 4)                    # 80 MB: the copy takes more than a millisecond
+    x = tokens(4, 1024, 5)
+    w, ids = routing(4, 48, 8, 6)
+    want = mx4_moe(x, w13, w2, topk_weights=w, topk_ids=ids)
+    torch.cuda.synchronize()
+    st = WispMoEStateMX4(w13, w2, 48, DEV, 0, mode="resident")
+    st.prime_identity()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        out = st.forward(x, w, ids)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
     st.close()
 
 

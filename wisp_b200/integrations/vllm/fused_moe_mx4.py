@@ -131,8 +131,11 @@ class WispMoEStateMX4(WispMoEState):
                        expert_map=self.expert_map_device, out=out)
 
     def prime_identity(self) -> None:
-        """Resident mode: identity map and full copy (fused_moe.py:242-258)."""
+        """Resident mode: identity map and full copy (fused_moe.py:242-258).  Waits for the layer's forwards before
+        the copy and for the copy itself, so that forwards on any stream find the experts in their slots."""
+        torch.cuda.synchronize(self.device)
         super().prime_identity()
+        torch.cuda.current_stream(self.device).synchronize()
         self._primed = True
 
     def ensure_resident(self, needed_experts: torch.Tensor) -> None:

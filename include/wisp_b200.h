@@ -154,6 +154,19 @@ WISP_API int wisp_mx4_matmul(const void *a_codes, const void *a_scales, int64_t 
 WISP_API int wisp_mx4_sync(void *stream);
 
 /*
+ * Of the two kernels: WISP_MX4_TRIES, the limit of one wait inside them on the
+ * current device, in tries (the default, also the largest, is several
+ * seconds; set it while none of them runs there), and WISP_MX4_DROP, a test
+ * fault: the launches that follow wait for scale bytes or for terms of
+ * activations that never come, give up at the limit and leave an incomplete
+ * output (WISP_MX4_DROP_NONE ends that).
+ */
+enum wisp_mx4_key { WISP_MX4_TRIES = 1, WISP_MX4_DROP = 2 };
+enum wisp_mx4_drop { WISP_MX4_DROP_NONE = 0, WISP_MX4_DROP_SCALES = 1, WISP_MX4_DROP_TERMS = 2 };
+enum { WISP_MX4_DEFAULT_TRIES = 1 << 22 };
+WISP_API int wisp_mx4_config(int32_t key, int64_t value);
+
+/*
  * A whole MoE layer for a few tokens from MXFP4 experts, in one (cooperative)
  * launch: out[t] = sum over the token's experts e of p_e W2[e] (silu(g) u),
  * [g; u] = W13[e] x[t].  x [T][hidden] bf16 (rows x_stride values apart).

@@ -29,6 +29,10 @@ CFG_DROP_PAGEINS = 4
 CFG_TRACE_BUFFER = 5
 CFG_TC_MIN_PAIRS = 6
 CFG_COMPUTE_CLASS = 7
+MX4_TRIES = 1
+MX4_DROP = 2
+MX4_DROP_NONE, MX4_DROP_SCALES, MX4_DROP_TERMS = 0, 1, 2
+MX4_DEFAULT_TRIES = 1 << 22
 PREFILL_MIN_PAIRS = 513     # calls from this size always run on the tensor cores (token-major GEMMs)
 
 _c_int32 = ctypes.c_int32
@@ -53,6 +57,7 @@ SIGNATURES = {
     "wisp_mx4_quantize": (ctypes.c_int, [_vp, _c_int32, _c_int64, _c_int64, _c_int64, _vp, _vp, _vp]),
     "wisp_mx4_dequantize": (ctypes.c_int, [_vp, _vp, _c_int64, _c_int64, _vp, _c_int32, _vp]),
     "wisp_mx4_matmul": (ctypes.c_int, [_vp, _vp, _c_int64, _vp, _vp, _c_int32, _c_int32, _c_int32, _vp, _vp, _vp]),
+    "wisp_mx4_config": (ctypes.c_int, [_c_int32, _c_int64]),
     "wisp_mx4_sync": (ctypes.c_int, [_vp]),
     "wisp_mx4_moe_workspace": (ctypes.c_int, [_c_int32] * 5 + [_p64]),
     "wisp_mx4_moe": (ctypes.c_int, [_vp, _c_int64, _vp, _vp, _c_int32, _vp, _vp, _vp, _vp, _vp, _vp, _p64] +

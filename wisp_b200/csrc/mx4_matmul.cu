@@ -27,6 +27,8 @@
 // over the chip; back to back the power limit makes that 340 us.  One small
 // product is latency: 16 x 4096 x 4096 takes 10.7 us, of which a launch and the
 // first loads are 6.
+#include <atomic>
+
 #include "mx4_mma.cuh"
 
 namespace wisp {
@@ -34,7 +36,8 @@ namespace mx4 {
 
 namespace {
 
-__device__ int g_status = 0;
+__device__ int g_status[2] = {0, WISP_MX4_DEFAULT_TRIES};  // see status_word
+std::atomic<int> g_dropped{0};
 
 constexpr int kTileM = 128;
 constexpr int kEpiWarp = 2, kSfWarp = 6;
@@ -68,6 +71,7 @@ struct MatmulArgs {
     int64_t rows;
     int *status;
     int groups, N, blocks, align, vec_out;
+    int drop;  // tests: arrivals that every stage's scale bytes wait for in vain
 };
 
 template <class S>
@@ -399,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0) {
         for (int s = 0; s < S::kStages; ++s) {
             mbar_init(&C.full[s], 1);
-            mbar_init(&C.sf_full[s], kScaleGroupWarps);
+            mbar_init(&C.sf_full[s], kScaleGroupWarps + a.drop);
             mbar_init(&C.empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -433,14 +437,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         // after an abort: copies and products in flight end before the memory is given back
         volatile int no_abort = 0;
         for (int k = C.consumed; k < C.issued; ++k)
-            wait_tries(&C.full[k % S::kStages], (k / S::kStages) & 1, &no_abort);
-        wait_tries(&C.mma_done, 0, &no_abort);
+            wait_tries(&C.full[k % S::kStages], (k / S::kStages) & 1, &no_abort, a.status);
+        wait_tries(&C.mma_done, 0, &no_abort, a.status);
     }
     __syncthreads();
     if (warp == 0) gemm::tmem_dealloc(C.tmem_base, kTmemCols);
 }
 
-int *g_words[64] = {};  // address of g_status on each device
+int *g_words[64] = {};  // address of g_status on each device, as found
 
 template <class S>
 int launch(const CUtensorMap &ma, const void *w_codes, const MatmulArgs &a, int64_t tiles, int sms, cudaStream_t stream) {
@@ -474,6 +478,7 @@ int status_word(int **word) {
     if (dev < 64) g_words[dev] = reinterpret_cast<int *>(p);  // the same value from every thread
     return *word = reinterpret_cast<int *>(p), WISP_OK;
 }
+int dropped() { return g_dropped.load(std::memory_order_relaxed); }
 
 }  // namespace mx4
 }  // namespace wisp
@@ -507,6 +512,7 @@ extern "C" int wisp_mx4_matmul(const void *a_codes, const void *a_scales, int64_
     a.out = reinterpret_cast<__nv_bfloat16 *>(out);
     a.rows = rows, a.groups = groups, a.N = n, a.blocks = k / kBlock;
     if (const int rc = status_word(&a.status)) return rc;
+    a.drop = dropped() == WISP_MX4_DROP_SCALES;
     const int aa = scale_align(a_scales, a.blocks), wa = scale_align(w_scales, a.blocks);
     a.align = aa < wa ? aa : wa;
     a.vec_out = n % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
@@ -530,4 +536,14 @@ extern "C" int wisp_mx4_sync(void *stream) {
     WISP_CUDA_TRY(cudaMemcpyToSymbol(g_status, &zero, sizeof(zero)));
     set_error("wisp_mx4: a wait inside a kernel ran out; its output is not complete");
     return status;
+}
+
+extern "C" int wisp_mx4_config(int32_t key, int64_t value) {
+    if (key == WISP_MX4_TRIES && value >= 1 && value <= WISP_MX4_DEFAULT_TRIES) {
+        const int tries = (int)value;
+        WISP_CUDA_TRY(cudaMemcpyToSymbol(g_status, &tries, sizeof(tries), sizeof(int)));
+        return WISP_OK;
+    }
+    if (key == WISP_MX4_DROP && value >= 0 && value <= WISP_MX4_DROP_TERMS) return g_dropped = (int)value, WISP_OK;
+    return set_error("wisp_mx4_config: unknown key or value"), WISP_ERR_INVALID;
 }

@@ -30,10 +30,12 @@ using gemm::umma_commit;
 constexpr int kStepK = 256;                 // values of K in a stage: 128 bytes a row
 constexpr int kStepBlocks = kStepK / kBlock;  // scale bytes of a row in a stage
 constexpr int kAtomBytes = 512;             // scales of 128 rows x 128 values
-constexpr uint32_t kTries = 1u << 22;       // limit of one wait
 
-// Device word of the kernels' sticky status on the current device (mx4_matmul.cu).
+// The current device's words of the kernels' waits (mx4_matmul.cu): [0] sticky
+// status, [1] limit of one wait in tries.
 int status_word(int **word);
+// What a test lets a launch wait for in vain (wisp_mx4_config).
+int dropped();
 
 // Instruction descriptor: E2M1 A and B, K-major, E8M0 scales, fp32 D, M x N;
 // `sf` 0 or 2: which half of the scale words (K 64 of 128).
@@ -94,21 +96,31 @@ __device__ __forceinline__ int atom_at(int r) { return (r & 31) * 16 + (r >> 5) 
 
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Bounded wait: kTries attempts, each of which suspends the thread for a while
-// (seconds in all; no wait here is longer than a few memory latencies).
-__device__ __forceinline__ bool wait_tries(uint64_t *bar, uint32_t parity, const volatile int *abort) {
+// Whether a wait gives up after its i-th try: `abort` was set, or the limit is
+// reached.  Looked at after every 256th only; the usual wait is far shorter.
+__device__ __forceinline__ bool gives_up(uint32_t i, const volatile int *abort, const int *status) {
+    return i % 256 == 0 && (*abort || i >= (uint32_t) reinterpret_cast<const volatile int *>(status)[1]);
+}
+// Waits until the barrier's phase is over.  A try suspends the thread for a
+// while: the limit is seconds, where no wait here is longer than a few memory
+// latencies.
+__device__ __forceinline__ bool wait_tries(uint64_t *bar, uint32_t parity, const volatile int *abort,
+                                           const int *status) {
     for (uint32_t i = 1; !mbar_try(bar, parity); ++i)
-        if (i % 256 == 0 && (*abort || i >= kTries)) return false;
+        if (gives_up(i, abort, status)) return false;
     return true;
 }
-// The same; a wait that runs out sets the status and the CTA's abort word.
+__device__ __forceinline__ void give_up(volatile int *abort, int *status) {
+    *abort = 1;
+    *reinterpret_cast<volatile int *>(status) = WISP_ERR_TIMEOUT;
+}
+// The wait of a role; one that runs out sets the status and the CTA's abort word.
 // (One copy of the loop for a kernel's many waits: roles that run at the same
 // time share one instruction cache.  A kernel of 228 KB, everything inlined and
 // unrolled, spent as long on fetching instructions as on memory.)
 static __device__ __noinline__ bool wait_long(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
-    if (wait_tries(bar, parity, abort)) return true;
-    *abort = 1;
-    *reinterpret_cast<volatile int *>(status) = WISP_ERR_TIMEOUT;
+    if (wait_tries(bar, parity, abort, status)) return true;
+    give_up(abort, status);
     return false;
 }
 __device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {

@@ -100,6 +100,7 @@ struct MoeArgs {
     int *status;
     int T, E, k, H, I, slots, ids64, renormalize, s13_align, s2_align;
     uint32_t inv_k;               // p / k = p * inv_k >> 16 for every pair p
+    int drop;                     // tests: what is waited for in vain
 };
 
 // What the lists are built from; lies where the ring will be.
@@ -442,16 +443,13 @@ __device__ __forceinline__ bool wait_terms(const Phase &ph, int group, volatile 
     uint32_t n;
     bool ok = false;
 #pragma unroll 1
-    for (uint32_t i = 1; !ok && i < kTries; ++i) {
+    for (uint32_t i = 1;; ++i) {
         asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(ph.done + group) : "memory");
         ok = n >= ph.done_tiles;
-        if (i % 256 == 0 && *abort) break;
+        if (ok || gives_up(i, abort, status)) break;
     }
     asm volatile("fence.proxy.async;" ::: "memory");
-    if (!ok) {
-        *abort = 1;
-        *reinterpret_cast<volatile int *>(status) = WISP_ERR_TIMEOUT;
-    }
+    if (!ok) give_up(abort, status);
     return __all_sync(0xFFFFFFFFu, ok);
 }
 
@@ -475,8 +473,11 @@ __device__ void run_copies(Control &C, unsigned char *stages, const Phase &ph, c
     const int lane = threadIdx.x & 31;
     int issued = C.issued;
     for (Walk t(ph); t.at(ph, L, C); t.next()) {
-        // (weights that need no terms are on their way: copy_early)
-        if (!wait_terms(ph, t.g, abort, status)) return;
+        // The weights of the first `early` steps are on their way (copy_early), announced together with the terms.
+        // Where a wait for terms gives up, what lies in their place is copied for these steps all the same, so that
+        // their barriers complete: the copies have to be over before the CTA ends.
+        const bool ok = wait_terms(ph, t.g, abort, status);
+        if (!ok && early == 0) return;
         const uint8_t *terms =
             lane < t.n ? ph.b_codes + ((size_t)(L.pair[t.off + lane] * ph.inv_div >> 16) * ph.steps + t.kb0) * kTermBytes
                        : nullptr;
@@ -487,7 +488,7 @@ __device__ void run_copies(Control &C, unsigned char *stages, const Phase &ph, c
             if (early > 0) {
                 --early;
             } else {
-                if (!warp_wait(&C.empty[cur.ring.slot], cur.ring.turn ^ 1, abort, status)) return;
+                if (!ok || !warp_wait(&C.empty[cur.ring.slot], cur.ring.turn ^ 1, abort, status)) return;
                 if (lane == 0) {
                     mbar_expect_tx(full, bytes);
                     load_weights(st, ph, t, kb, full);
@@ -746,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&C.full[s], 1);
-            mbar_init(&C.sf_full[s], kScaleGroupWarps);
+            mbar_init(&C.sf_full[s], kScaleGroupWarps + (a.drop == WISP_MX4_DROP_SCALES));
             mbar_init(&C.empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -805,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         down.groups = L.n, down.m_tiles = (a.H + 127) / 128, down.rows_m = 128;
         down.split = pieces_of(down.steps);
         down.rows = a.H, down.slot_rows = a.w2_rows, down.scale_slot_rows = a.s2_rows, down.second = 64;
-        down.inv_div = 65536, down.done = a.done, down.done_tiles = up.m_tiles;
+        down.inv_div = 65536, down.done = a.done, down.done_tiles = up.m_tiles + (a.drop == WISP_MX4_DROP_TERMS);
         // (pieces of D begin at whole 16-byte loads of scale bytes)
         up.term_align = up.steps % 2 ? 8 : 16, down.term_align = down.steps % 2 ? 8 : 16;
         const int unit = down.align >= 16 || down.term_align >= 16 ? 2 : 1;
@@ -865,8 +866,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // after an abort: copies and products in flight end before the memory is given back
         volatile int no_abort = 0;
         for (int k = C.consumed; k < C.issued; ++k)
-            wait_tries(&C.full[k % kStages], (k / kStages) & 1, &no_abort);
-        wait_tries(&C.mma_done, 0, &no_abort);
+            wait_tries(&C.full[k % kStages], (k / kStages) & 1, &no_abort, a.status);
+        wait_tries(&C.mma_done, 0, &no_abort, a.status);
     }
     __syncthreads();
     if (warp == 0) gemm::tmem_dealloc(C.tmem_base, kTmemCols);
@@ -983,6 +984,7 @@ extern "C" int wisp_mx4_moe(const void *x, int64_t x_stride, const void *router,
     a.s2_align = std::min(a.s2_align, scale_align(nullptr, (int)(st[3] & 15)));
     a.T = num_tokens, a.E = num_experts, a.k = top_k, a.H = hidden, a.I = inter, a.slots = num_slots;
     a.ids64 = ids_int64, a.renormalize = renormalize, a.inv_k = 65536 / top_k + 1;
+    a.drop = dropped();
     int dev = 0, sms = 0;
     WISP_CUDA_TRY(cudaGetDevice(&dev));
     WISP_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));

@@ -148,10 +148,14 @@ WISP_API int wisp_mx4_matmul(const void *a_codes, const void *a_scales, int64_t 
                              const void *w_scales, int32_t groups, int32_t n, int32_t k, const int32_t *offsets,
                              void *out, void *stream);
 /*
- * Wait for `stream` and report (then clear) a bounded wait that ran out inside
- * wisp_mx4_matmul or wisp_mx4_moe on the current device (WISP_ERR_TIMEOUT).
+ * Wait for `stream`; WISP_ERR_TIMEOUT when a bounded wait inside
+ * wisp_mx4_matmul or wisp_mx4_moe has run out on the current device since
+ * this stream last asked, whichever stream the kernel ran on.  Every stream
+ * is told of it once: the answer to one takes nothing from another.
  */
 WISP_API int wisp_mx4_sync(void *stream);
+/* Wait for `stream`; how many waits have run out on the current device so far. */
+WISP_API int wisp_mx4_timeouts(void *stream, int64_t *count);
 
 /*
  * Of the two kernels: WISP_MX4_TRIES, the limit of one wait inside them on the

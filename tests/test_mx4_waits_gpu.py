@@ -80,3 +80,47 @@ def test_unknown_keys_and_values_are_refused():
     for key, value in ((0, 0), (3, 0), (_lib.MX4_DROP, 3), (_lib.MX4_DROP, -1), (_lib.MX4_TRIES, 0),
                        (_lib.MX4_TRIES, 1 << 32)):
         assert L.wisp_mx4_config(key, value) == _lib.WISP_ERR_INVALID
+
+
+def test_every_stream_is_told():
+    """The streams of other calls, asked first, do not take the report from the stream of the call that gave up."""
+    from wisp_b200 import _lib
+    from wisp_b200.mx4 import mx4_moe, mx4_synchronize
+    w13, w2, router = layer(4, 64, 32)
+    x = tokens(2, 64)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    with in_vain(_lib.MX4_DROP_TERMS):
+        with torch.cuda.stream(streams[0]):
+            mx4_moe(x, w13, w2, 2, router=router)
+        torch.cuda.synchronize()
+        for s in (streams[1], streams[2], streams[0], torch.cuda.current_stream()):
+            with torch.cuda.stream(s):
+                assert timed_out()
+    for s in (*streams, torch.cuda.current_stream()):
+        with torch.cuda.stream(s):
+            mx4_synchronize()
+
+
+def test_every_layer_is_told():
+    from wisp_b200 import _lib
+    from wisp_b200.integrations.vllm import WispMoEStateMX4
+    from wisp_b200.mx4 import mx4_synchronize
+    w13, w2, _ = layer(4, 64, 32)
+    x, w = tokens(2, 64), torch.ones(2, 2, device=DEV)
+    ids = torch.tensor([[0, 1], [1, 0]], device=DEV)
+    a, b = (WispMoEStateMX4(w13, w2, 2, DEV, i) for i in range(2))
+    with in_vain(_lib.MX4_DROP_TERMS):
+        a.forward(x, w, ids)
+        torch.cuda.synchronize()
+        for st in (b, a):
+            with pytest.raises(_lib.WispError, match="ran out") as e:
+                st.synchronize()
+            assert e.value.code == _lib.WISP_ERR_TIMEOUT
+        assert timed_out()
+    want = b.forward(x, w, ids)
+    late = WispMoEStateMX4(w13, w2, 2, DEV, 2)
+    assert torch.equal(a.forward(x, w, ids), want) and torch.equal(late.forward(x, w, ids), want)
+    for st in (a, b, late):
+        st.synchronize()
+        st.close()
+    mx4_synchronize()

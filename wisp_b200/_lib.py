@@ -57,6 +57,7 @@ SIGNATURES = {
     "wisp_mx4_quantize": (ctypes.c_int, [_vp, _c_int32, _c_int64, _c_int64, _c_int64, _vp, _vp, _vp]),
     "wisp_mx4_dequantize": (ctypes.c_int, [_vp, _vp, _c_int64, _c_int64, _vp, _c_int32, _vp]),
     "wisp_mx4_matmul": (ctypes.c_int, [_vp, _vp, _c_int64, _vp, _vp, _c_int32, _c_int32, _c_int32, _vp, _vp, _vp]),
+    "wisp_mx4_timeouts": (ctypes.c_int, [_vp, _p64]),
     "wisp_mx4_config": (ctypes.c_int, [_c_int32, _c_int64]),
     "wisp_mx4_sync": (ctypes.c_int, [_vp]),
     "wisp_mx4_moe_workspace": (ctypes.c_int, [_c_int32] * 5 + [_p64]),

@@ -31,8 +31,8 @@ constexpr int kStepK = 256;                 // values of K in a stage: 128 bytes
 constexpr int kStepBlocks = kStepK / kBlock;  // scale bytes of a row in a stage
 constexpr int kAtomBytes = 512;             // scales of 128 rows x 128 values
 
-// The current device's words of the kernels' waits (mx4_matmul.cu): [0] sticky
-// status, [1] limit of one wait in tries.
+// The current device's words of the kernels' waits (mx4_matmul.cu): [0] how many
+// ran out, [1] limit of one wait in tries.
 int status_word(int **word);
 // What a test lets a launch wait for in vain (wisp_mx4_config).
 int dropped();
@@ -112,7 +112,7 @@ __device__ __forceinline__ bool wait_tries(uint64_t *bar, uint32_t parity, const
 }
 __device__ __forceinline__ void give_up(volatile int *abort, int *status) {
     *abort = 1;
-    *reinterpret_cast<volatile int *>(status) = WISP_ERR_TIMEOUT;
+    atomicAdd(status, 1);
 }
 // The wait of a role; one that runs out sets the status and the CTA's abort word.
 // (One copy of the loop for a kernel's many waits: roles that run at the same

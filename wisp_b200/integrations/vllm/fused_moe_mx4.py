@@ -47,6 +47,7 @@ class WispMoEStateMX4(WispMoEState):
         self._primed = False
         self._lock = threading.RLock()
         super().__init__(_blocks(w13), _blocks(w2), cap_experts, mode, device, layer_idx)
+        self._timeouts_told = self._timeouts()
 
     def _refresh_views(self) -> None:
         super()._refresh_views()
@@ -159,12 +160,22 @@ class WispMoEStateMX4(WispMoEState):
             raise _lib.WispError(_lib.WISP_ERR_INVALID, "resident layer has no expert in its slots; call prime_identity "
                                                         "first")
 
+    def _timeouts(self) -> int:
+        """Waits inside 4-bit kernels that have run out on the layer's device so far."""
+        n = ctypes.c_int64(0)
+        with torch.cuda.device(self.device):
+            _lib.check(_lib.lib().wisp_mx4_timeouts(_lib.stream_ptr(torch.cuda.current_stream()), ctypes.byref(n)))
+        return n.value
+
     def synchronize(self) -> None:
-        """Wait for this layer's queued work and raise the first error of its page-ins or kernels."""
+        """Wait for this layer's queued work and raise the first error of its page-ins or kernels.  A wait that ran out
+        inside a 4-bit kernel is counted for the device, not for the layer: every layer there raises for it once."""
         torch.cuda.current_stream(self.device).synchronize()
         super().synchronize()
-        from wisp_b200.mx4 import mx4_synchronize
-        mx4_synchronize(self.device)
+        told, self._timeouts_told = self._timeouts_told, self._timeouts()
+        if self._timeouts_told != told:
+            raise _lib.WispError(_lib.WISP_ERR_TIMEOUT, "a wait inside a 4-bit kernel ran out; its output is not "
+                                                        "complete")
 
 
 __all__ = ["WispMoEStateMX4"]

@@ -97,7 +97,7 @@ def mx4_matmul(a: Mx4Tensor, w: Mx4Tensor, offsets: torch.Tensor | None = None,
 
 def mx4_synchronize(device: torch.device | None = None) -> None:
     """Wait for the device's current stream and raise if a bounded wait inside an :func:`mx4_matmul` or
-    :func:`mx4_moe` ran out."""
+    :func:`mx4_moe` has run out on the device, on whichever stream, since this was last called on this stream."""
     index = None if device is None else torch.device(device).index
     native.mx4_synchronize(torch.cuda.current_device() if index is None else index)
 

@@ -111,7 +111,7 @@ __device__ __forceinline__ float block_sum(float v, float *buf) {
     return s;
 }
 
-constexpr size_t kMostShared = 226 * 1024;
+constexpr size_t kMostShared = 226 * 1024;  // beside the sums
 constexpr int kRowsAhead = 2;  // 1 where the memory of two rows is more than an SM has
 
 template <typename T, typename R, typename W, int VEC, int THREADS, int NV>
@@ -456,8 +456,9 @@ template <typename K>
 int launch_rows(K kernel, int threads, int rows_of_cta, size_t smem, const NormArgs &a, cudaStream_t stream) {
     int dev = 0, sms = 0, per = 0;
     WISP_CUDA_TRY(cudaGetDevice(&dev));
+    // the limit is the same in every call: another thread's launch of this kernel may come between it and this one
     if (smem > 47 * 1024)
-        WISP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        WISP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostShared));
     int64_t grid = (a.rows + rows_of_cta - 1) / rows_of_cta;
     if (grid > 148) {  // fewer than SMs need no count of what runs together
         WISP_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));

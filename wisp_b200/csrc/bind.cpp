@@ -38,7 +38,9 @@ int type_code(at::ScalarType t) {
 int32_t to_int(int64_t v) { return (int32_t)std::clamp<int64_t>(v, INT32_MIN, INT32_MAX); }
 // The library's error, raised as its Python binding raises it.
 void check(int rc, const char *what) {
-    if (rc != WISP_OK) py::module_::import("wisp_b200._lib").attr("check")(rc, what);
+    if (rc == WISP_OK) return;
+    const py::gil_scoped_acquire gil;
+    py::module_::import("wisp_b200._lib").attr("check")(rc, what);
 }
 void need_cuda(const char *name, const Tensor &t) {
     if (!t.is_cuda()) value_error(std::string(name) + " must be on a CUDA device; got " + t.device().str());
@@ -271,11 +273,14 @@ std::tuple<Tensor, Tensor> block_norm(const Tensor &y, const Tensor &residual, c
 
 }  // namespace
 
+// Without the interpreter's lock, as torch's own calls: a launch waits where the
+// stream's queue is full, and what it waits for may need another Python thread.
 PYBIND11_MODULE(_wisp_bind, m) {
-    m.def("mx4_quantize", &mx4_quantize);
-    m.def("mx4_dequantize", &mx4_dequantize);
-    m.def("mx4_matmul", &mx4_matmul);
-    m.def("mx4_moe", &mx4_moe);
-    m.def("mx4_synchronize", &mx4_synchronize);
-    m.def("block_norm", &block_norm);
+    const auto unlocked = py::call_guard<py::gil_scoped_release>();
+    m.def("mx4_quantize", &mx4_quantize, unlocked);
+    m.def("mx4_dequantize", &mx4_dequantize, unlocked);
+    m.def("mx4_matmul", &mx4_matmul, unlocked);
+    m.def("mx4_moe", &mx4_moe, unlocked);
+    m.def("mx4_synchronize", &mx4_synchronize, unlocked);
+    m.def("block_norm", &block_norm, unlocked);
 }

@@ -185,8 +185,8 @@ WISP_API int wisp_mx4_config(int32_t key, int64_t value);
  * counts once, with the sum of the weights.  slot_strides: bytes from slot to
  * slot of w13's codes, w13's scales, w2's codes and w2's scales, each a whole
  * number of its rows (NULL: the slots follow one another).  Activations take
- * part as sums of six MXFP4 terms (at least 12 bits of a block's largest
- * value), the rest is fp32, out is rounded once.  A token's result depends on
+ * part as sums of eight MXFP4 terms (exact to 2^-23 of the largest value in a
+ * block of 32, and to 2^-129), the rest is fp32, out is rounded once.  A token's result depends on
  * nothing but its own row, weights and experts: not on the slots, nor on the
  * other tokens of the call.  T <= 64, top_k <= 16, num_experts <= 1024, hidden and inter
  * multiples of 32 up to 32768 and 65536.  workspace:

@@ -8,14 +8,21 @@
 // Weights are MXFP4 in checkpoint layout and go to the block-scaled tensor
 // cores (tcgen05.mma kind::mxf4) as they are: nothing is unpacked on the way.
 // Activations keep their precision: a block of 32 of them is written as a sum
-// of six MXFP4 terms, each the rounding of what the terms before it left.  A
-// term's scale is the smallest power of two under which the remainder's
-// largest value is at most 6, so a term leaves less than a quarter of it (a
-// sixth, mostly): six leave between 2^-12 and 2^-15 of the block's largest
-// value, below the 2^-9 that bf16 activations carry.  The terms of a token are
-// rows of the product's small operand: 8 rows a token (the rows of a swizzle
-// pattern, two of them unused), 16 tokens a tile; weights take the 128 rows of
-// the other side, a token's result is the sum of its six accumulator columns.
+// of eight MXFP4 terms, each the rounding of what the terms before it left.  A
+// term's scale s is the smallest power of two under which the remainder's
+// largest value is at most 6, so that this value m lies above 3 s.  The first
+// term leaves at most 0.5 s where m <= 4.5 s, and s (1 of 5) above.  What is
+// left, r <= s, has a scale of s / 8 where r <= 0.75 s, and at most that is left
+// of it; else s / 4, under which it is at most 4, and half of that is left: s / 8
+// again.  (From 0.5 s it is s / 16, likewise.)  So eight terms leave at most
+// 8^-7 / 4.5 < 2^-23 of the block's largest value, or 2^-129, half the smallest
+// code, where that is more.  A remainder is a whole number of its value's last
+// places: a bf16 value that is at least 2^-15 of the largest is held exactly.
+// The terms of a token are the 8 rows of a swizzle pattern of the product's
+// small operand, 16 tokens a tile; weights take the 128 rows of the other side,
+// a token's result is the sum of its eight accumulator columns.  (Six terms,
+// with two rows unused, were 0.4 us faster at one token of the layer below, 2 at
+// 64, and lost 2e-4 of the small values in blocks with one 1000 times larger.)
 // h, the SiLU and the weighted sum are fp32; out is rounded to bf16 once.
 // (Unpacking to fp16 for mma.sync instead cost 110 us at 16 tokens of a
 // Qwen3-30B-A3B layer, twice this kernel: it is bound by the four hundred
@@ -45,7 +52,7 @@
 // tokens: 129 us (675 MB, 5.2 TB/s).  With many tokens an expert the terms, 8
 // rows each, are as many bytes from L2 as the weights (64 tokens there: 289).
 // Writing the terms of two or four blocks together in G, for their chains of
-// six roundings to overlap, was 1 to 6 us slower everywhere.
+// six roundings (as it was then) to overlap, was 1 to 6 us slower everywhere.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -62,8 +69,8 @@ constexpr int kEpiWarp = 2, kSfWarp = 6;       // four warps and two groups of f
 constexpr int kWarps = 16;                     // two of them in R, S and C only
 static_assert(kSfWarp + kScaleGroups * kScaleGroupWarps <= kWarps, "roles");
 constexpr int kThreads = kWarps * 32;
-constexpr int kTerms = 6;                      // terms of an activation
-constexpr int kRows = 8;                       // rows of a token in the small operand
+constexpr int kTerms = 8;                      // terms of an activation
+constexpr int kRows = kTerms;                  // rows of a token in the small operand, those of a swizzle pattern
 constexpr int kGroup = 16;                     // tokens of a tile
 constexpr int kStages = 5;
 constexpr int kTermBytes = kRows * 128;        // terms of a token in a stage
@@ -134,7 +141,7 @@ __device__ __forceinline__ uint32_t transpose_nibbles(uint32_t w, int r) {
 // One block of 32 values, one a lane, as terms: codes to `codes` (16 bytes of
 // row 0, rows 128 bytes apart, 16-byte pieces swizzled by the row) and scale
 // bytes to `scales` (rows `stride` apart).  A term needs the one before it, so
-// only that chain is in the loop: a lane collects its six codes in a word and
+// only that chain is in the loop: a lane collects its eight codes in a word and
 // the words are transposed together.
 __device__ __forceinline__ void write_terms(float v, uint8_t *codes, uint8_t *scales, int stride, int piece, int lane) {
     uint32_t word = 0, my_byte = 0;
@@ -157,7 +164,7 @@ __device__ __forceinline__ void write_terms(float v, uint8_t *codes, uint8_t *sc
     }
     const int q = lane & 7;
     word = transpose_nibbles(word, q);
-    if (q < kTerms) *reinterpret_cast<uint32_t *>(codes + q * 128 + ((piece ^ q) << 4) + (lane >> 3) * 4) = word;
+    *reinterpret_cast<uint32_t *>(codes + q * 128 + ((piece ^ q) << 4) + (lane >> 3) * 4) = word;
     if (lane < kTerms) scales[lane * stride] = (uint8_t)my_byte;
 }
 
@@ -542,7 +549,7 @@ __device__ void run_scales(Control &C, unsigned char *stages, const Phase &ph, c
         const int row = ahead.m0 + my_row;
         pw = row < ph.rows ? ph.w_scales + ((int64_t)ahead.slot * ph.scale_slot_rows + row) * ph.blocks : nullptr;
         const int i = tid / kRows, q = tid % kRows;
-        pb = i < ahead.n && q < kTerms
+        pb = i < ahead.n
                  ? ph.b_scales + (size_t)((L.pair[ahead.off + i] * ph.inv_div >> 16) * kRows + q) * term_stride
                  : nullptr;
     };

@@ -110,8 +110,9 @@ def mx4_moe(x: torch.Tensor, w13: Mx4Tensor, w2: Mx4Tensor, top_k: int | None = 
             topk_ids: torch.Tensor | None = None, expert_map: torch.Tensor | None = None,
             out: torch.Tensor | None = None) -> torch.Tensor:
     """A whole MoE layer for at most 64 tokens, in one launch (``wisp_mx4_moe``): routing, gate-up, SiLU, down and the
-    weighted sum, from MXFP4 experts and bf16 activations.  Inside the products activations are sums of six MXFP4 terms,
-    which hold a value to 2^-12 of the largest one in its block of 32 or better (bf16 holds that one to 2^-9).
+    weighted sum, from MXFP4 experts and bf16 activations.  Inside the products a block of
+    32 activations is a sum of eight MXFP4 terms, which hold a value to 2^-23 of the largest one in its block (and to
+    2^-129 at best), a bf16 value of at least 2^-15 of it exactly.
 
     ``x [T, H]`` bf16; ``w13 [S, 2I, H]`` (gate rows, then up rows) and ``w2 [S, H, I]``.  Routing is either the
     layer's ``router [E, H]`` (bf16) with ``top_k``: softmax over the ``top_k`` largest products (over all of them and

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import argparse
 import glob
+import importlib.metadata
 import os
 import shutil
 import subprocess
@@ -24,6 +25,7 @@ LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libwisp_b200.so")
 BIND_SRC = os.path.join(CSRC, "bind.cpp")
 BIND = os.path.join(LIBDIR, "_wisp_bind.so")
+BIND_STAMP = os.path.join(LIBDIR, "_wisp_bind.stamp")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -51,15 +53,30 @@ def _stale() -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def build_bind(force: bool = False) -> str:
-    """The Python binding; it finds ``libwisp_b200.so`` beside itself."""
+def _bind_made_for() -> str:
+    """What the binding depends on besides its sources: the interpreter's and torch's binary interfaces."""
+    try:
+        torch_version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        torch_version = "none"
+    return f"{sys.implementation.cache_tag} torch {torch_version}"
+
+
+def build_bind(force: bool = False) -> str | None:
+    """The Python binding; it finds ``libwisp_b200.so`` beside itself.  Rebuilt when its sources, the interpreter or
+    torch's version changed.  Without torch there is nothing to build it against, and nothing to use it with: None."""
     header = os.path.join(INCLUDE, "wisp_b200.h")
+    made_for = _bind_made_for()
     if not force and os.path.exists(BIND) and all(os.path.getmtime(p) <= os.path.getmtime(BIND)
                                                   for p in (BIND_SRC, header)):
-        return BIND
+        if os.path.exists(BIND_STAMP) and open(BIND_STAMP).read() == made_for:
+            return BIND
+    try:
+        import torch
+    except ImportError:
+        print("wisp_b200: no torch, so the Python binding of the stateless operators is not built", file=sys.stderr)
+        return None
     import sysconfig
-
-    import torch
     tree = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
     inc = [os.path.join(tree, "include"), os.path.join(tree, "include", "torch", "csrc", "api", "include"),
@@ -71,6 +88,8 @@ def build_bind(force: bool = False) -> str:
            "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
     subprocess.run(cmd, check=True)
     os.replace(tmp, BIND)
+    with open(BIND_STAMP, "w") as f:
+        f.write(made_for)
     return BIND
 
 

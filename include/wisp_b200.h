@@ -211,8 +211,10 @@ WISP_API int wisp_mx4_moe(const void *x, int64_t x_stride, const void *router, c
  * residual_out of residual_dtype, pre_weight and post_weight [cols] of
  * weight_dtype, each `dtype` or fp32.  gate: none, one for each channel
  * [cols], one for each token (gate_stride values apart) or [rows][cols].
- * Rows are *_stride values apart; normed and residual_out are contiguous and
- * may be y's and the residual's own memory where those are contiguous too.
+ * Rows are *_stride values apart; normed and residual_out are contiguous.
+ * Either may lie row by row in the place of y, the residual or a [rows][cols]
+ * gate of its own type and stride; any other overlap with an input, or with
+ * one another, is refused.
  */
 enum wisp_gate { WISP_GATE_NONE = 0, WISP_GATE_TOKEN = 1, WISP_GATE_CHANNEL = 2, WISP_GATE_FULL = 3 };
 WISP_API int wisp_block_norm(const void *y, int64_t y_stride, const void *residual, int64_t residual_stride,

@@ -21,7 +21,7 @@
 // The terms of a token are the 8 rows of a swizzle pattern of the product's
 // small operand, 16 tokens a tile; weights take the 128 rows of the other side,
 // a token's result is the sum of its eight accumulator columns.  (Six terms,
-// with two rows unused, were 0.4 us faster at one token of the layer below, 2 at
+// with two rows unused, were 0.4 us faster at one token of the layer below, 0.8 at 16, 2 at
 // 64, and lost 2e-4 of the small values in blocks with one 1000 times larger.)
 // h, the SiLU and the weighted sum are fp32; out is rounded to bf16 once.
 // (Unpacking to fp16 for mma.sync instead cost 110 us at 16 tokens of a

@@ -19,8 +19,9 @@ def block_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, *,
 
     in fp32, ``r`` and ``normed`` rounded once each.  ``y`` is bf16, fp16 or fp32 (``normed`` likewise); ``residual``
     and the weights have its type or fp32.  ``gate`` has ``y``'s type: one value for each channel (``[H]``), for each
-    token (``[..., 1]``) or for each element (``[..., H]``).  ``residual_out=residual`` updates the residual in place.
-    At most 16384 channels.  No autograd: for serving."""
+    token (``[..., 1]``) or for each element (``[..., H]``).  ``residual_out=residual`` updates the residual in place; an
+    output that overlaps an input in another way, or the other output, is refused.  At most 16384 channels.  No
+    autograd: for serving."""
     return native.block_norm(y, residual, weight, post_weight, gate, scale, eps, out, residual_out)
 
 

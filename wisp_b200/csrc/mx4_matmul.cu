@@ -60,7 +60,7 @@ struct Shape {
     static constexpr int kSfHalf = 4 + 4 * kWAtoms;  // columns of tensor memory: A's atom, W's
     static constexpr int kSfCols = 2 * kSfHalf;      // of a stage
     static constexpr int kSfCol0 = 2 * kTileN;       // behind the two accumulators
-    static constexpr int kCols = kTileN < 64 ? kTileN : 64;  // the epilogue's piece
+    static constexpr int kCols = 64;                 // the epilogue's piece
     static_assert(kSfCol0 + kStages * kSfCols <= kTmemCols, "tensor memory");
     static_assert(kStages > kWindow, "a parity wait has to know its phase");
     static_assert(kTileN % kCols == 0 && kTileN <= 256, "tile");

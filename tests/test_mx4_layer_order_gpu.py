@@ -161,3 +161,26 @@ def test_used_refuses_what_it_cannot_cover():
     st = WispMoEStateMX4(*experts(4, 64, 32), 4, DEV, 0, mode="resident")
     assert L.wisp_layer_used(st._h, ids, 1, None) == _lib.WISP_ERR_INVALID
     st.close()
+
+
+@pytest.mark.parametrize("mode,cap", [("paged", 3), ("resident", E)])
+def test_arguments_are_refused_before_anything_is_paged_in(mode, cap):
+    from wisp_b200.integrations.vllm import WispMoEStateMX4
+    st = WispMoEStateMX4(*experts(E, H, I, 5), cap, DEV, 0, mode=mode)
+    if mode == "resident":
+        st.prime_identity()
+    x = tokens(3, H, 1)
+    w, ids = routing(3, E, 2, 1)
+    before = st._read()
+    wide = torch.empty(3, 2 * H, dtype=torch.bfloat16, device=DEV)
+    for error, args, out in [
+            (TypeError, (x.half(), w, ids), None), (TypeError, (x, w, ids.to(torch.int16)), None),
+            (ValueError, (x.cpu(), w, ids), None), (ValueError, (x, w.cpu(), ids), None),
+            (ValueError, (x, w, ids.cpu()), None), (ValueError, (x, w, ids), torch.empty_like(x).cpu()),
+            (ValueError, (x, w, ids), torch.empty(4, H, dtype=torch.bfloat16, device=DEV)),
+            (ValueError, (x, w, ids), torch.empty(2, H, dtype=torch.bfloat16, device=DEV)),
+            (ValueError, (x, w, ids), torch.empty(3, H, device=DEV)), (ValueError, (x, w, ids), wide[:, :H])]:
+        with pytest.raises(error):
+            st.forward(*args, out=out)
+    assert st._read() == before
+    st.close()

@@ -79,9 +79,17 @@ class WispMoEStateMX4(WispMoEState):
         if topk_ids.dim() != 2 or topk_ids.shape[0] != x.shape[0] or topk_weights.shape != topk_ids.shape:
             raise ValueError(f"topk_weights and topk_ids must be [{x.shape[0]}, k]; got {tuple(topk_weights.shape)} and "
                              f"{tuple(topk_ids.shape)}")
+        for name, t in (("x", x), ("topk_weights", topk_weights), ("topk_ids", topk_ids), ("out", out)):
+            if t is not None and t.device != self.device:
+                raise ValueError(f"{name} must be on {self.device}; got {t.device}")
+        if x.dtype != torch.bfloat16:
+            raise TypeError(f"a layer of 4-bit experts computes from bf16 activations; got {x.dtype}")
+        if topk_ids.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"topk_ids must be int32 or int64; got {topk_ids.dtype}")
         if out is None:
             out = torch.empty((x.shape[0], hidden), dtype=x.dtype, device=x.device)
-
+        elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
+            raise ValueError(f"out must be contiguous bf16 {tuple(x.shape)}; got {out.dtype} {tuple(out.shape)}")
         def compute(a, b):
             mx4_moe(x[a:b], self.slots_w13, self.slots_w2, topk_weights=topk_weights[a:b], topk_ids=topk_ids[a:b],
                     expert_map=self.expert_map_device, out=out[a:b])

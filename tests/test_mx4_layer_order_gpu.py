@@ -184,3 +184,21 @@ def test_arguments_are_refused_before_anything_is_paged_in(mode, cap):
             st.forward(*args, out=out)
     assert st._read() == before
     st.close()
+
+
+@pytest.mark.parametrize("mode,cap,T", [("paged", 3, 9), ("paged", E, 100), ("resident", E, 150)])
+def test_result_in_the_memory_of_the_tokens(mode, cap, T):
+    """In their place, and a row further on, where a group's rows are the next one's tokens."""
+    from wisp_b200.integrations.vllm import WispMoEStateMX4
+    st = WispMoEStateMX4(*experts(E, H, I, 6), cap, DEV, 0, mode=mode)
+    if mode == "resident":
+        st.prime_identity()
+    w, ids = routing(T, E, 2, 3)
+    buf = tokens(T + 1, H, 2)
+    keep = buf.clone()
+    for a, b in ((0, 0), (0, 1), (1, 0)):
+        buf.copy_(keep)
+        want = st.forward(buf[a:a + T].clone(), w, ids)
+        assert torch.equal(st.forward(buf[a:a + T], w, ids, out=buf[b:b + T]), want), (a, b)
+    st.synchronize()
+    st.close()

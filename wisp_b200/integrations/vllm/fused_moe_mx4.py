@@ -90,6 +90,10 @@ class WispMoEStateMX4(WispMoEState):
             out = torch.empty((x.shape[0], hidden), dtype=x.dtype, device=x.device)
         elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
             raise ValueError(f"out must be contiguous bf16 {tuple(x.shape)}; got {out.dtype} {tuple(out.shape)}")
+        if (out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr()
+                and (out.data_ptr(), out.stride()) != (x.data_ptr(), x.stride())):
+            x = x.clone()               # a group's rows of out may lie where a later group's rows of x do
+
         def compute(a, b):
             mx4_moe(x[a:b], self.slots_w13, self.slots_w2, topk_weights=topk_weights[a:b], topk_ids=topk_ids[a:b],
                     expert_map=self.expert_map_device, out=out[a:b])

@@ -202,3 +202,21 @@ def test_result_in_the_memory_of_the_tokens(mode, cap, T):
         assert torch.equal(st.forward(buf[a:a + T], w, ids, out=buf[b:b + T]), want), (a, b)
     st.synchronize()
     st.close()
+
+
+@pytest.mark.parametrize("mode,cap", [("paged", 4), ("resident", E)])
+def test_synchronize_waits_for_forwards_on_any_stream(held_up, mode, cap):
+    from wisp_b200.integrations.vllm import WispMoEStateMX4
+    st = WispMoEStateMX4(*experts(E, H, I, 7), cap, DEV, 0, mode=mode)
+    if mode == "resident":
+        st.prime_identity()
+    x = tokens(1, H, 1)
+    w, ids = routing(1, E, 2, 1)
+    torch.cuda.synchronize()
+    done = torch.cuda.Event()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        st.forward(x, w, ids)
+        done.record()
+    st.synchronize()
+    assert done.query()
+    st.close()

@@ -180,9 +180,10 @@ class WispMoEStateMX4(WispMoEState):
         return n.value
 
     def synchronize(self) -> None:
-        """Wait for this layer's queued work and raise the first error of its page-ins or kernels.  A wait that ran out
-        inside a 4-bit kernel is counted for the device, not for the layer: every layer there raises for it once."""
-        torch.cuda.current_stream(self.device).synchronize()
+        """Wait for this layer's queued work, on whichever streams, and raise the first error of its page-ins or kernels.
+        A wait that ran out inside a 4-bit kernel is counted for the device, not for the layer: every layer there raises
+        for it once."""
+        torch.cuda.synchronize(self.device)
         super().synchronize()
         told, self._timeouts_told = self._timeouts_told, self._timeouts()
         if self._timeouts_told != told:

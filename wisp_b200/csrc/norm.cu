@@ -518,8 +518,14 @@ int dispatch(const NormArgs &a, cudaStream_t stream) {
         if (cols <= 8 * 1536) return launch<T, R, W, 8, 512, 3>(a, stream);
         return launch<T, R, W, 8, 1024, 2>(a, stream);
     }
-    // pairs of values: 8191 x 2050 48 us, shifted 62 to 68; but 9000 x 3074 68 us, shifted 57
-    if (cols <= 2 * 1280 && fits(2)) {
+    // Pairs of values against shifted granules (us for 100 MB, floor 15.3, both norms and a token gate; bf16 | bf16 with a
+    // fp32 residual | fp32): 258 columns 40.5, 56.3 | 28.9, 42.0 | 23.2, 34.5; 514 67.0, 43.9 | 46.4, 35.2 | 36.1, 32.4;
+    // 770 48.5, 39.7 | 34.7, 33.1 | 27.6, 35.2; 900 43.6, 38.0 | 31.6, 38.0 | 25.8; 1026 39.9, 41.2 | 28.9, 31.9 | 24.3, 29.6;
+    // 1538 35.1, 35.8 | 25.6, 30.5 | 23.0, 29.5; 2558 28.3, 35.4 | 21.8, 30.1 | 21.8, 31.1.  So pairs, but for 16-bit rows from
+    // 513 columns to 1024 (768 with a fp32 residual), which one warp has without barriers.  Longer rows would take more than
+    // five pairs a thread (9000 x 3074 bf16: 68 us, 57).
+    const bool one_warp = sizeof(T) == 2 && cols > 2 * 256 && cols <= (sizeof(R) == 4 ? 8 * 96 : 8 * 128);
+    if (cols <= 2 * 1280 && !one_warp && fits(2)) {
         if (cols <= 2 * 256) return launch<T, R, W, 2, 64, 4>(a, stream);
         if (cols <= 2 * 768) return launch<T, R, W, 2, 256, 3>(a, stream);
         return launch<T, R, W, 2, 256, 5>(a, stream);
@@ -527,13 +533,18 @@ int dispatch(const NormArgs &a, cudaStream_t stream) {
     if constexpr (std::is_same<T, float>::value)  // the longest rows in fp32 leave no room for the output buffers
         if (row_buffer(cols, 4) * (a.gate_kind == WISP_GATE_FULL ? 5 : 4) > kMostShared)
             return launch<T, R, W, 1, 1024, 16>(a, stream);
-    // a row of one warp needs no barriers; above, two pieces a thread and few threads without any (us, 3000 x 6221 bf16:
-    // 53 with 416 x 2, 58 with 384 x 3, 74 with 512 x 2, 82 with 1024 x 1; 16000 x 1147: 62 with 96 x 2, 82 with 256 x 1)
+    // A row of one warp needs no barriers; above, as few warps as hold the row in two pieces a thread (us as above): 513
+    // columns 43.7 with 32 x 4, 53.4 with 64 x 2 | 35.1, 40.2 | 32.6, 33.2 (771: 39.7, 39.5 | 33.0, 32.2 | 34.7, 30.3); 1025
+    // 41.0 with 96 x 2, 41.3 with 128 x 2, 58.3 with 256 x 2 | 31.9, 32.1, 43.3 | 29.3, 30.3, 40.2; 1795 34.1 with 128 x 2, 35.4
+    // with 64 x 4 | 30.2, 37.2 | 30.1, 35.3; 2051 40.0 with 224 x 2, 40.5 with 256 x 2, 49.2 with 320 x 2 | 33.0, 32.7, 37.3 |
+    // 31.0, 32.4, 36.8; 4097 37.3 with 320 x 2, 43.1 with 416 x 2, 61.8 with 512 x 2 | 33.2, 36.3, 35.2 | 33.3, 44.3, 42.4;
+    // 5121 38.7 with 416 x 2, 54.5 with 512 x 2 | 35.0, 34.5 | 43.4, 40.8; 6657 46.1 with 512 x 2, 52.0 with 1024 x 1 | 38.9,
+    // 42.9 | 38.1, 38.9.
     if (cols <= 8 * 32) return launch_any<T, R, W, 32, 1>(a, stream);
     if (cols <= 8 * 64) return launch_any<T, R, W, 32, 2>(a, stream);
     if (cols <= 8 * 128) return launch_any<T, R, W, 32, 4>(a, stream);
     if (cols <= 8 * 192) return launch_any<T, R, W, 96, 2>(a, stream);
-    if (cols <= 8 * 256) return launch_any<T, R, W, 64, 4>(a, stream);
+    if (cols <= 8 * 256) return launch_any<T, R, W, 128, 2>(a, stream);
     if (cols <= 8 * 448) return launch_any<T, R, W, 224, 2>(a, stream);
     if (cols <= 8 * 512) return launch_any<T, R, W, 256, 2>(a, stream);
     if (cols <= 8 * 640) return launch_any<T, R, W, 320, 2>(a, stream);

@@ -115,7 +115,8 @@ WISP_API int wisp_route_topk(const void *logits, int32_t logits_bf16, int32_t nu
 /*
  * Stateless operators around a layer of 4-bit experts (no counterparts in the
  * reference).  They run on the current device, asynchronously on `stream`,
- * allocate nothing and may be captured into a CUDA graph.
+ * allocate nothing and may be captured into a CUDA graph.  An output that
+ * overlaps an input is refused, but where an operator allows it.
  *
  * MXFP4: a matrix [rows][K], K a multiple of 32, is codes [rows][K / 2] (two
  * E2M1 values a byte, the even column in the low nibble) and scales
@@ -188,7 +189,8 @@ WISP_API int wisp_mx4_config(int32_t key, int64_t value);
  * part as sums of eight MXFP4 terms (exact to 2^-23 of the largest value in a
  * block of 32, and to 2^-129), the rest is fp32, out is rounded once.  A token's result depends on
  * nothing but its own row, weights and experts: not on the slots, nor on the
- * other tokens of the call.  T <= 64, top_k <= 16, num_experts <= 1024, hidden and inter
+ * other tokens of the call.  out may lie over x (its overlap with anything
+ * else is not looked for).  T <= 64, top_k <= 16, num_experts <= 1024, hidden and inter
  * multiples of 32 up to 32768 and 65536.  workspace:
  * wisp_mx4_moe_workspace() bytes, aligned to 16, any contents; calls that may
  * overlap on the GPU need one each.

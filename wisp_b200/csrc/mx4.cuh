@@ -13,6 +13,24 @@
 #include "common.cuh"
 
 namespace wisp {
+
+// Rows of `bytes` bytes, `stride` bytes apart.
+struct ByteRows {
+    uintptr_t at;
+    int64_t rows, stride, bytes;
+    // Whether one of them has a byte of the `n` bytes at `p`.
+    bool meets(uintptr_t p, int64_t n) const {
+        const int64_t lo = (int64_t)(p - at), hi = lo + n;  // relative to the first row
+        if (hi <= 0) return false;
+        if (stride == 0 || rows == 1) return lo < bytes;
+        const int64_t i = lo < bytes ? 0 : (lo - bytes) / stride + 1;  // the first row that ends behind lo
+        return i < rows && i * stride < hi;
+    }
+};
+inline bool meets(const void *p, int64_t bytes, const void *q, int64_t more) {
+    return ByteRows{reinterpret_cast<uintptr_t>(p), 1, 0, bytes}.meets(reinterpret_cast<uintptr_t>(q), more);
+}
+
 namespace mx4 {
 
 constexpr int kBlock = 32;  // values that share a scale

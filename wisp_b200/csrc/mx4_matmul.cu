@@ -505,6 +505,11 @@ extern "C" int wisp_mx4_matmul(const void *a_codes, const void *a_scales, int64_
         if (reinterpret_cast<uintptr_t>(p) % 16)
             return set_error("wisp_mx4_matmul: codes must be aligned to 16 bytes"), WISP_ERR_INVALID;
     if (reinterpret_cast<uintptr_t>(out) % 2) return set_error("wisp_mx4_matmul: unaligned out"), WISP_ERR_INVALID;
+    const int64_t wrows = (int64_t)groups * n, out_bytes = rows * n * 2;
+    if (meets(a_codes, rows * (k / 2), out, out_bytes) || meets(a_scales, rows * (k / kBlock), out, out_bytes) ||
+        meets(w_codes, wrows * (k / 2), out, out_bytes) || meets(w_scales, wrows * (k / kBlock), out, out_bytes) ||
+        (offsets && meets(offsets, 4 * (int64_t)(groups + 1), out, out_bytes)))
+        return set_error("wisp_mx4_matmul: out overlaps an input"), WISP_ERR_INVALID;
     CUtensorMap ma;
     if (const int rc = gemm::make_byte_map(&ma, a_codes, rows, k / 2, kTileM)) return rc;
     MatmulArgs a{};

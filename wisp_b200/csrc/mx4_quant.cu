@@ -181,6 +181,11 @@ extern "C" int wisp_mx4_quantize(const void *x, int32_t dtype, int64_t rows, int
         reinterpret_cast<uintptr_t>(codes) % 4)
         return set_error("wisp_mx4_quantize: rows must not overlap and must start on 16-byte boundaries"),
                WISP_ERR_INVALID;
+    const int64_t code_bytes = rows * (cols / 2), scale_bytes = rows * (cols / kBlock);
+    const ByteRows in{reinterpret_cast<uintptr_t>(x), rows, row_stride * size, cols * size};
+    if (in.meets(reinterpret_cast<uintptr_t>(codes), code_bytes) ||
+        in.meets(reinterpret_cast<uintptr_t>(scales), scale_bytes) || meets(codes, code_bytes, scales, scale_bytes))
+        return set_error("wisp_mx4_quantize: codes, scales and x overlap"), WISP_ERR_INVALID;
     const int64_t pieces = rows * (cols / 8);
     const unsigned grid = (unsigned)((pieces + kThreads * kUnroll - 1) / (kThreads * kUnroll));
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -211,6 +216,9 @@ extern "C" int wisp_mx4_dequantize(const void *codes, const void *scales, int64_
     if (!codes || !scales || !out) return set_error("wisp_mx4_dequantize: NULL tensor"), WISP_ERR_INVALID;
     if (reinterpret_cast<uintptr_t>(codes) % 4 || reinterpret_cast<uintptr_t>(out) % 16)
         return set_error("wisp_mx4_dequantize: codes must be aligned to 4 bytes, out to 16"), WISP_ERR_INVALID;
+    const int64_t out_bytes = rows * cols * (dtype == WISP_FP32 ? 4 : 2);
+    if (meets(codes, rows * (cols / 2), out, out_bytes) || meets(scales, rows * (cols / kBlock), out, out_bytes))
+        return set_error("wisp_mx4_dequantize: out overlaps codes or scales"), WISP_ERR_INVALID;
     const int64_t pieces = rows * (cols / 8);
     const unsigned grid = (unsigned)((pieces + kThreads * kUnroll - 1) / (kThreads * kUnroll));
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

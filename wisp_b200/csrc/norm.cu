@@ -561,20 +561,6 @@ int dispatch_types(const NormArgs &a, int32_t residual_dtype, int32_t weight_dty
     return wf ? dispatch<T, T, float>(a, stream) : dispatch<T, T, T>(a, stream);
 }
 
-// Rows of `bytes` bytes, `stride` bytes apart.
-struct Rows {
-    uintptr_t at;
-    int64_t rows, stride, bytes;
-    // Whether one of them has a byte of the `n` bytes at `p`.
-    bool meets(uintptr_t p, int64_t n) const {
-        const int64_t lo = (int64_t)(p - at), hi = lo + n;  // relative to the first row
-        if (hi <= 0) return false;
-        if (stride == 0 || rows == 1) return lo < bytes;
-        const int64_t i = lo < bytes ? 0 : (lo - bytes) / stride + 1;  // the first row that ends behind lo
-        return i < rows && i * stride < hi;
-    }
-};
-
 }  // namespace
 }  // namespace wisp
 
@@ -606,22 +592,22 @@ extern "C" int wisp_block_norm(const void *y, int64_t y_stride, const void *resi
     // A row's outputs are written while other rows are still to be read.  In place is fine: a CTA reads a row before it
     // writes it, each thread its own columns.
     const auto span = [&](const void *p, int64_t stride, int64_t n, size_t of) {
-        return Rows{reinterpret_cast<uintptr_t>(p), rows, stride * (int64_t)of, n * (int64_t)of};
+        return ByteRows{reinterpret_cast<uintptr_t>(p), rows, stride * (int64_t)of, n * (int64_t)of};
     };
     const bool full = gate_kind == WISP_GATE_FULL || (gate_kind == WISP_GATE_TOKEN && cols == 1);
-    const Rows row_inputs[] = {span(y, y_stride, cols, size), span(residual, residual_stride, cols, res_size),
-                               full ? span(gate, gate_stride, cols, size) : Rows{0, 1, 0, 0}};
-    const Rows others[] = {span(pre_weight, 0, cols, w_size), post_weight ? span(post_weight, 0, cols, w_size) : Rows{0, 1, 0, 0},
+    const ByteRows row_inputs[] = {span(y, y_stride, cols, size), span(residual, residual_stride, cols, res_size),
+                               full ? span(gate, gate_stride, cols, size) : ByteRows{0, 1, 0, 0}};
+    const ByteRows others[] = {span(pre_weight, 0, cols, w_size), post_weight ? span(post_weight, 0, cols, w_size) : ByteRows{0, 1, 0, 0},
                            gate && !full ? span(gate, gate_stride, gate_kind == WISP_GATE_CHANNEL ? cols : 1, size)
-                                         : Rows{0, 1, 0, 0}};
-    const Rows outputs[] = {span(normed, cols, cols, size), span(residual_out, cols, cols, res_size)};
+                                         : ByteRows{0, 1, 0, 0}};
+    const ByteRows outputs[] = {span(normed, cols, cols, size), span(residual_out, cols, cols, res_size)};
     bool clash = outputs[0].meets(outputs[1].at, rows * outputs[1].bytes);
-    for (const Rows &o : outputs) {
-        for (const Rows &in : row_inputs) {
+    for (const ByteRows &o : outputs) {
+        for (const ByteRows &in : row_inputs) {
             const bool in_place = in.at == o.at && in.bytes == o.bytes && (in.stride == o.stride || rows == 1);
             clash |= !in_place && in.meets(o.at, rows * o.bytes);
         }
-        for (const Rows &in : others) clash |= in.meets(o.at, rows * o.bytes);
+        for (const ByteRows &in : others) clash |= in.meets(o.at, rows * o.bytes);
     }
     if (clash)
         return set_error("wisp_block_norm: an output overlaps an input (other than row by row in its place) or the other "

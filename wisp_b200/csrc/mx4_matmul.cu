@@ -20,13 +20,14 @@
 // memory through registers, ahead of their use; no TMA box can make that
 // arrangement.
 //
-// Measured: 128 experts x 128 rows x 1536 x 2048 (282 MB to read and write)
-// 56 us, 5.1 TB/s, the weights read once (232 MB from HBM, 709 MB through L2:
-// a ragged group has one or two row tiles).  8 experts x 512 rows x 28672 x
-// 4096 (962 GFLOP) 281 us, 3.4 PFLOP/s, 43 KB of L2 a stage and SM, 11.7 TB/s
-// over the chip; back to back the power limit makes that 340 us.  One small
-// product is latency: 16 x 4096 x 4096 takes 10.7 us, of which a launch and the
-// first loads are 6.
+// Measured (in a graph of calls whose inputs, in turn, exceed L2): 128 experts
+// x 128 rows x 1536 x 2048 (282 MB to read and write) 57 us, 4.9 TB/s, the weights
+// read once (232 MB from HBM, 709 MB through L2: a ragged group has one or two
+// row tiles).  8 experts x 512 rows x 28672 x 4096 (962 GFLOP) 293 us, 3.3
+// PFLOP/s, 43 KB of L2 a stage and SM, 11.2 TB/s over the chip (281 on one input;
+// back to back the power limit makes that up to 340).  One small product is
+// latency: 16 x 4096 x 4096 takes 12.0 us (10.7 with its weights in L2), of which
+// a launch and the first loads are 6.
 #include <atomic>
 #include <map>
 #include <mutex>
@@ -463,7 +464,7 @@ int launch(const CUtensorMap &ma, const void *w_codes, const MatmulArgs &a, int6
 using Wide = Shape<192, 4>;
 // Where the tiles are so few that SMs would go without: the time is then the
 // latency of a tile's steps, which narrow tiles, with more stages in flight,
-// shorten (us, narrow against wide, 16 rows x 4096 x 4096: 11.0, 12.3; 40
+// shorten (us on one input, narrow against wide, 16 rows x 4096 x 4096: 11.0, 12.3; 40
 // groups of 223 rows x 180 x 3200: 11.0, 12.4; 128 x 9472 x 2048: 8.8, 10.2).
 // With more narrow tiles than SMs the wide ones win (512 x 4096 x 4096: 18.4,
 // 13.8); 32 columns were no better anywhere (13.1 at the first size).

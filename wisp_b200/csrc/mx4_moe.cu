@@ -46,13 +46,14 @@
 // as the swizzle wants them) and issues the products, eight bring the scale
 // bytes (mx4_mma.cuh), four read the accumulators.
 //
-// Measured, 128 experts of 2048 x 768, top-8: 18.7 us for one token (21 MB;
-// three phases that wait for one another, 2 to 3 us each, and the launch), 53.5
-// for 16 (207 MB, 3.9 TB/s), 90 for 64.  8 experts of 4096 x 14336, top-2, 8
-// tokens: 129 us (675 MB, 5.2 TB/s).  With many tokens an expert the terms, 8
-// rows each, are as many bytes from L2 as the weights (64 tokens there: 289).
-// Writing the terms of two or four blocks together in G, for their chains of
-// six roundings (as it was then) to overlap, was 1 to 6 us slower everywhere.
+// Measured (in a graph of calls whose inputs, in turn, exceed L2), 128 experts
+// of 2048 x 768, top-8: 21.5 us for one token (21 MB; three phases that wait for
+// one another, 2 to 3 us each, and the launch), 53 for 16 (207 MB, 3.9 TB/s), 95
+// for 64.  8 experts of 4096 x 14336, top-2, 8 tokens: 127 us (675 MB, 5.3 TB/s).
+// With many tokens an expert the terms, 8 rows each, are as many bytes from L2
+// as the weights (64 tokens there: 293).  Writing the terms of two or four
+// blocks together in G, for their chains of roundings (six then) to overlap, was
+// 1 to 6 us slower everywhere.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -13,9 +13,11 @@
 // takes two shuffles, and the codes leave as one 32-bit store a thread, so a
 // warp's loads and stores are whole lines.  The values stay as loaded until
 // they are rounded: widened at once they took twice the registers, and the
-// loads in flight of half as many threads.  49152 x 2048 bf16: 37 us to MXFP4
-// and 40 back, 255 MB each, 6.6 TB/s, what a copy has; 1021 x 4096 fp16: 5.3 us
-// for both (21 MB, 4 TB/s); one row of 2048: 1.2 us each, a launch.
+// loads in flight of half as many threads.  In a graph of calls whose inputs, in
+// turn, exceed L2: 49152 x 2048 bf16 36 us to MXFP4 and 41 back, 255 MB each, 6.6
+// TB/s together, what a copy has; rows that lie apart 48 (a division of 64 bits
+// for 8 values); fp32 64 and 108 back (456 MB, 7.1 and 4.2 TB/s); 1021 x 4096 fp16
+// 6.1 us for both (21 MB, 3.5 TB/s); one row of 2048: 1.2 us each, a launch.
 #include "mx4.cuh"
 
 namespace wisp {

@@ -25,11 +25,12 @@
 // back (4000 x 2803 fp16, fp32 residual, a full gate: 49 us, 114 value by
 // value; 3000 x 6221 fp32: 106, 160).
 //
-// Measured: a row of 2048 bf16 2.0 us, a launch; 2048 x 4096 bf16 with both
-// norms and a gate 16.3 us (67 MB, 4.1 TB/s; 4 to 5 rows a CTA, whose first
-// loads and last reductions nothing hides; 512 threads 16.7, 128 threads 20.9);
-// 8191 x 2050 bf16 with a fp32 residual, pairs of values, 48 us (201 MB, 4.2
-// TB/s), by its instructions (60 % of the issue slots).
+// Measured (in a graph of calls whose inputs, in turn, exceed L2): a row of 2048
+// bf16 2.2 us, a launch; 2048 x 4096 bf16 with both norms and a gate 16.7 us (67
+// MB, 4.0 TB/s; 4 to 5 rows a CTA, whose first loads and last reductions nothing
+// hides; on one input 16.3, with 512 threads 16.7, with 128 threads 20.9); 8191 x
+// 2050 bf16 with a fp32 residual, pairs of values, 48.6 us (201 MB, 4.1 TB/s), by
+// its instructions (60 % of the issue slots).
 #include <algorithm>
 #include <type_traits>
 

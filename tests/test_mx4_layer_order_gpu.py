@@ -220,3 +220,24 @@ def test_synchronize_waits_for_forwards_on_any_stream(held_up, mode, cap):
     st.synchronize()
     assert done.query()
     st.close()
+
+
+@pytest.mark.parametrize("T", [1, 70])
+def test_resident_forward_in_a_graph(T):
+    """One launch, and two of them; between replays the layer is used as usual."""
+    from wisp_b200.integrations.vllm import WispMoEStateMX4
+    st = WispMoEStateMX4(*experts(E, H, I, 8), E, DEV, 0, mode="resident")
+    st.prime_identity()
+    x, out = tokens(T, H, 9), torch.empty(T, H, dtype=torch.bfloat16, device=DEV)
+    w, ids = routing(T, E, 3, 10)
+    st.forward(x, w, ids)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        st.forward(x, w, ids, out=out)
+    for _ in range(3):
+        x.mul_(-0.75)
+        graph.replay()
+        assert torch.equal(out, st.forward(x, w, ids))
+        st.synchronize()
+    st.close()

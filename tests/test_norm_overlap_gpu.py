@@ -84,3 +84,24 @@ def test_refusals():
                    dict(residual=y, gate=buf[2], out=buf[:8]), dict(residual=y, gate=buf[:8, 3:4], out=buf[:8])):
         with pytest.raises(_lib.WispError, match="overlaps"):
             block_norm(y, weight=w, **kwargs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", COLS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_in_place_with_a_fp32_residual(cols, dtype):
+    """y and the residual updated where they lie, rows of different lengths in bytes; replayed from a graph as well."""
+    from wisp_b200.norm import block_norm
+    y, r, w, g = tensors(900, cols, True)
+    y, r, w, g = y.to(dtype), r.float(), w.float(), g.to(dtype)
+    first = block_norm(y, r, w, post_weight=w, gate=g)
+    second = block_norm(*first, w, post_weight=w, gate=g)
+    ys, rs = y.clone(), r.clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        block_norm(ys, rs, w, post_weight=w, gate=g, out=ys, residual_out=rs)
+    for want in (first, second):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(ys, want[0]) and torch.equal(rs, want[1])

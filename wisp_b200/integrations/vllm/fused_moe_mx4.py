@@ -108,8 +108,8 @@ class WispMoEStateMX4(WispMoEState):
             try:
                 for a, b in self._groups(rows):
                     self.ensure_resident(topk_ids[a:b])
-                    compute(a, b)
                     done = b
+                    compute(a, b)
             finally:
                 if done:
                     self._used(set().union(*rows[:done]))
